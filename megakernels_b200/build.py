@@ -1,8 +1,8 @@
 """Native libraries and how they are compiled (nvcc, sm_100a, in-tree).
 
 ``build(name)`` compiles one library if it is missing or older than its sources; every source is
-its own nvcc process, so a library takes as long as its slowest file.  The llama megakernel and
-the hybrid models' kernels are separate libraries: a user of one does not compile the other.
+its own nvcc process, so a library takes as long as its slowest file.  The llama megakernel, the
+hybrid models' kernels and what happens to sequences between steps are separate libraries: a user of one does not compile the others.
 Run as ``python -m megakernels_b200.build [name ...]``.
 """
 
@@ -58,6 +58,12 @@ LIBRARIES = {
         ("hybrid_decode.cu", "hybrid_decode_rotary.cu", "hybrid_decode_mixed.cu", "hybrid_prefill.cu",
          "hybrid_attention.cu", "hybrid_flash.cu", "hybrid_plain.cu", "hybrid_gemm_bf16.cu", "hybrid_gemm_f32.cu", "hybrid_host.cu"),
         ("hybrid_common.cuh", "hybrid_kernels.h", "hybrid_product.h", "hybrid_decode.cu", "hybrid_tcgen05.cuh", "mk_common.cuh", "../../include/mkb200.h",
+         "../../include/mkb200_hybrid.h"),
+    ),
+    "sequences": Library(
+        "libmkb200_sequences.so",
+        ("sequence_host.cu", "sequence_beam.cu", "sequence_rows.cu", "sequence_weights.cu"),
+        ("sequence_kernels.h", "../../include/mkb200_sequences.h", "hybrid_common.cuh", "mk_common.cuh", "../../include/mkb200.h",
          "../../include/mkb200_hybrid.h"),
     ),
 }

@@ -1,0 +1,344 @@
+"""Importable ``mk_sequences`` module: a ctypes shim over ``libmkb200_sequences.so``.
+
+What happens to sequences between two decoding steps (``include/mkb200_sequences.h``): beam search's
+selection and the reordering of states, the attention weight that cached keys receive, and the
+eviction of the others.  No counterpart in the reference.  As the other shims it marshals pointers and
+sizes; a missing library is an ImportError, never a fallback.
+
+Every function enqueues its work on ``stream`` (a stream, a handle, or None for the current one) of the
+current device, where all tensors must live, and neither synchronises nor reads anything back, so all of
+them can be captured into a CUDA graph.  Arguments that the library does not take raise ``ValueError`` /
+``TypeError`` here or ``SequenceError`` from its own checks, before anything is launched.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from pathlib import Path
+
+import torch
+from torch import Tensor
+
+_HERE = Path(__file__).resolve().parent
+LIB_PATH = _HERE / "libmkb200_sequences.so"
+
+MKBS_ABI_VERSION = 1
+MAX_BEAMS, MAX_BEST, MAX_REGIONS, MAX_SLOTS = 64, 128, 48, 256
+ERROR_NAMES = {0: "MKBS_OK", 1: "MKBS_ERR_INVALID_ARGUMENT", 2: "MKBS_ERR_CUDA", 3: "MKBS_ERR_DEVICE_TIMEOUT", 5: "MKBS_ERR_UNSUPPORTED"}
+
+_i32, _f32, _ptr, _i64, _u32, _size = ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, ctypes.c_size_t
+
+
+class MkbsBeams(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", _u32), *[(n, _i32) for n in ("dtype", "groups", "beams", "vocab", "k")], ("row_stride", _i64),
+        ("logits", _ptr), ("scores", _ptr), ("done", _ptr), ("eos", _i32), ("reserved", _i32),
+        *[(n, _ptr) for n in ("out_scores", "out_parents", "out_tokens", "out_done", "workspace")], ("workspace_bytes", _size),
+    ]
+
+
+class MkbsRegion(ctypes.Structure):
+    _fields_ = [("base", _ptr), ("outer", _i32), ("rows", _i32), ("outer_stride", _i64), ("slot_stride", _i64), ("row_bytes", _i64)]
+
+
+class MkbsReorder(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", _u32), ("slots", _i32), ("num_regions", _i32), ("first", _i32), ("regions", ctypes.POINTER(MkbsRegion)),
+        ("parents", _ptr), ("lengths", _ptr),
+    ]
+
+
+class MkbsKeyWeights(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", _u32),
+        *[(n, _i32) for n in ("layers", "sequences", "queries", "heads", "kv_heads", "dim", "positions", "length")],
+        ("scale", _f32), ("lengths", _ptr), ("q", _ptr), ("q_layer", _i64), ("q_sequence", _i64),
+        ("k", _ptr), ("k_layer", _i64), ("k_sequence", _i64), ("weights", _ptr), ("w_layer", _i64), ("w_sequence", _i64), ("w_head", _i64),
+        ("workspace", _ptr), ("workspace_bytes", _size), ("status", _ptr), ("wait_timeout_ms", _u32), ("reserved", _u32),
+    ]
+
+
+class MkbsSelect(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", _u32),
+        *[(n, _i32) for n in ("layers", "sequences", "kv_heads", "positions", "length", "keep", "sinks", "recent", "reserved")],
+        ("lengths", _ptr), ("weights", _ptr), ("w_layer", _i64), ("w_sequence", _i64), ("w_head", _i64), ("rows", _ptr), ("kept", _ptr),
+    ]
+
+
+class MkbsMove(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", _u32), *[(n, _i32) for n in ("layers", "sequences", "kv_heads", "positions", "length", "keep", "head_bytes")],
+        ("lengths", _ptr), ("rows", _ptr), ("caches", _ptr * 2), ("c_layer", _i64), ("c_sequence", _i64),
+    ]
+
+
+STRUCTS = (MkbsBeams, MkbsRegion, MkbsReorder, MkbsKeyWeights, MkbsSelect, MkbsMove)
+
+
+class SequenceError(RuntimeError):
+    def __init__(self, code: int, message: str):
+        super().__init__(f"{ERROR_NAMES.get(code, code)}: {message}")
+        self.code = code
+
+
+_lib = None
+
+
+def load_library() -> ctypes.CDLL:
+    global _lib
+    if _lib is not None:
+        return _lib
+    if not LIB_PATH.exists():
+        raise ImportError(f"{LIB_PATH} is missing: build it with `python -m megakernels_b200.build sequences`. "
+                          "There is no CPU fallback.")
+    lib = ctypes.CDLL(str(LIB_PATH))
+    for name, struct in (("beam_select", MkbsBeams), ("reorder_slots", MkbsReorder), ("key_weights", MkbsKeyWeights),
+                         ("select_rows", MkbsSelect), ("move_rows", MkbsMove)):
+        fn = getattr(lib, f"mkb_{name}")
+        fn.argtypes, fn.restype = [ctypes.POINTER(struct), _ptr], ctypes.c_int
+    for name, struct in (("beam", MkbsBeams), ("key_weights", MkbsKeyWeights)):
+        fn = getattr(lib, f"mkb_{name}_bytes")
+        fn.argtypes, fn.restype = [ctypes.POINTER(struct)], _size
+    lib.mkb_sequences_last_error.restype = ctypes.c_char_p
+    lib.mkb_sequences_struct_bytes.argtypes, lib.mkb_sequences_struct_bytes.restype = [_i32], _size
+    if lib.mkb_sequences_abi_version() != MKBS_ABI_VERSION:
+        raise ImportError(f"{LIB_PATH.name} has ABI {lib.mkb_sequences_abi_version()}, expected {MKBS_ABI_VERSION}")
+    sizes = [lib.mkb_sequences_struct_bytes(i) for i in range(len(STRUCTS))]
+    if sizes != [ctypes.sizeof(s) for s in STRUCTS]:
+        raise ImportError(f"struct layouts of {LIB_PATH.name} {sizes} differ from this shim")
+    _lib = lib
+    return lib
+
+
+def _check(name: str, t, dtype, shape=None, inner: int | None = None) -> int:
+    """Address of a tensor on the current device.  ``shape``: what it must be; ``inner``: trailing dimensions that
+    must lie one behind the other (None: all)."""
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device")
+    if t.device.index != torch.cuda.current_device():  # (the launch goes to the current device)
+        raise ValueError(f"{name} lives on cuda:{t.device.index} but the current device is cuda:{torch.cuda.current_device()} "
+                         "(wrap the call in torch.cuda.device(...))")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if inner is None:
+        dense = t.is_contiguous()
+    else:
+        part = t[(0,) * (t.ndim - inner)] if t.numel() else t
+        dense = part.is_contiguous()
+    if not dense:
+        raise ValueError(f"{name} must be contiguous" + ("" if inner is None else f" in its last {inner} dimensions"))
+    return t.data_ptr()
+
+
+def _stream(stream, device) -> torch.cuda.Stream:
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    if isinstance(stream, int):
+        return torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    return stream
+
+
+def _workspace(nbytes: int, stream: torch.cuda.Stream, device) -> Tensor:
+    with torch.cuda.stream(stream):  # (given back when the call returns, to that stream alone: later work on it runs after the kernels)
+        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+
+
+def _keep_alive(stream: torch.cuda.Stream, *tensors) -> None:
+    """Tensors of another stream are not given out again before this stream has used them."""
+    for t in tensors:
+        if t is not None and stream != torch.cuda.current_stream(t.device):
+            t.record_stream(stream)
+
+
+def _call(name: str, struct, stream: torch.cuda.Stream) -> None:
+    lib = load_library()
+    code = getattr(lib, f"mkb_{name}")(ctypes.byref(struct), ctypes.c_void_p(stream.cuda_stream))
+    if code:
+        raise SequenceError(code, lib.mkb_sequences_last_error().decode())
+
+
+def _struct(kind):
+    s = kind()
+    s.struct_bytes = ctypes.sizeof(kind)
+    return s
+
+
+def _lengths(s, lengths, sequences: int, positions: int):
+    """Rows that each sequence holds: an int32 tensor on the device, or one number for all."""
+    if isinstance(lengths, Tensor):
+        s.lengths = _check("lengths", lengths, torch.int32, (sequences,))
+        return lengths
+    s.lengths, s.length = None, int(lengths)
+    if not 0 <= s.length <= positions:
+        raise ValueError(f"length {lengths} outside a cache of {positions} rows")
+    return None
+
+
+def beam_select(logits: Tensor, scores: Tensor | None = None, *, beams: int, k: int, done: Tensor | None = None, eos: int | None = None,
+                stream=None) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """The ``k`` best continuations of every group of ``beams`` rows of ``logits`` (``[groups * beams, vocab]`` bf16 or
+    float32, rows any stride apart), best first: ``scores[b] + log_softmax(logits[b])[v]``, ties to the lowest ``(b, v)``.
+
+    ``scores`` float32 ``[groups, beams]`` (None: zero); ``done`` uint8 ``[groups, beams]``: beams whose only
+    continuation is ``eos``, at their score.  Returns scores float32, parents int32 (rows of ``logits``), tokens int32
+    and done uint8, each ``[groups, k]``.
+    """
+    if not isinstance(logits, Tensor) or logits.ndim != 2:
+        raise ValueError("logits must be [groups * beams, vocab]")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"logits must be bfloat16 or float32, got {logits.dtype}")
+    if beams < 1 or logits.shape[0] < 1 or logits.shape[0] % beams:
+        raise ValueError(f"{logits.shape[0]} rows of logits are no groups of {beams}")
+    s = _struct(MkbsBeams)
+    rows, s.vocab = logits.shape
+    s.groups, s.beams, s.k, s.dtype = rows // beams, beams, k, int(logits.dtype == torch.float32)
+    s.row_stride = logits.stride(0) if rows > 1 else s.vocab
+    s.logits = _check("logits", logits, logits.dtype, inner=1)
+    s.scores = _check("scores", scores, torch.float32, (s.groups, beams)) if scores is not None else None
+    s.done = _check("done", done, torch.uint8, (s.groups, beams)) if done is not None else None
+    s.eos = -1 if eos is None else int(eos)
+    lib, where = load_library(), _stream(stream, logits.device)
+    with torch.cuda.stream(where):
+        out = [torch.empty(s.groups, max(k, 0), dtype=t, device=logits.device) for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+    s.out_scores, s.out_parents, s.out_tokens, s.out_done = (t.data_ptr() for t in out)
+    s.workspace_bytes = lib.mkb_beam_bytes(ctypes.byref(s))
+    workspace = _workspace(s.workspace_bytes, where, logits.device)
+    s.workspace = workspace.data_ptr()
+    _call("beam_select", s, where)
+    _keep_alive(where, logits, scores, done)
+    return tuple(out)
+
+
+def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first: int = 0, lengths: Tensor | None = None, stream=None) -> None:
+    """``t[..., slot, ...] <- t[..., parents[slot], ...]`` for every slot at once and in place, ``dim`` being the slots'
+    dimension (0, or 1 behind the layers') of every tensor.
+
+    With ``lengths`` (int32 ``[slots]``) the dimension behind it is rows: a slot takes its parent's rows ``first ..
+    lengths[parent] - 1``; the others stay.  ``parents`` int32 ``[slots]``; one outside the slots leaves its slot as it is.
+    """
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("no tensors to reorder")
+    if dim not in (0, 1):
+        raise ValueError("the slots' dimension is 0 or 1")
+    if first < 0 or (first and lengths is None):
+        raise ValueError("first counts rows: it is not negative and needs lengths")
+    if not isinstance(parents, Tensor) or parents.ndim != 1:
+        raise ValueError("parents must be int32 [slots]")
+    slots = parents.shape[0]
+    base = _struct(MkbsReorder)
+    base.slots, base.first = slots, first
+    base.parents = _check("parents", parents, torch.int32)
+    base.lengths = _check("lengths", lengths, torch.int32, (slots,)) if lengths is not None else None
+    regions = []
+    for i, t in enumerate(tensors):
+        if not isinstance(t, Tensor):
+            raise TypeError(f"tensor {i} must be a torch.Tensor")
+        if t.ndim < dim + 1 + (lengths is not None) or t.shape[dim] != slots:
+            raise ValueError(f"tensor {i} {list(t.shape)} does not have {slots} slots in dimension {dim}" + (" and rows behind it" if lengths is not None else ""))
+        if t.numel() == 0:
+            raise ValueError(f"tensor {i} is empty")
+        r = MkbsRegion()
+        r.base = _check(f"tensor {i}", t, t.dtype, inner=t.ndim - dim - 1)
+        size = t.element_size()
+        r.outer, r.outer_stride = (t.shape[0], t.stride(0) * size) if dim else (1, 0)
+        r.slot_stride = t.stride(dim) * size if slots > 1 else t[(0,) * (dim + 1)].numel() * size
+        r.rows = t.shape[dim + 1] if lengths is not None else 1
+        r.row_bytes = t[(0,) * (dim + 1)].numel() * size // r.rows
+        regions.append(r)
+    where = _stream(stream, parents.device)
+    for at in range(0, len(regions), MAX_REGIONS):
+        some = regions[at : at + MAX_REGIONS]
+        array = (MkbsRegion * len(some))(*some)
+        base.num_regions, base.regions = len(some), ctypes.cast(array, ctypes.POINTER(MkbsRegion))
+        _call("reorder_slots", base, where)
+    _keep_alive(where, parents, lengths, *tensors)
+
+
+def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int, *, scale: float, status: Tensor | None = None, wait_timeout_ms: int = 0,
+                stream=None) -> None:
+    """Add to ``weights`` (float32 ``[layers, sequences, kv_heads, positions]``) the softmax weight that each cached key
+    receives from the queries, summed over them and over the query heads that share the key.
+
+    ``q`` bf16 ``[layers, sequences, queries, heads, dim]``: the queries of the sequences' last rows; ``keys`` bf16 ``[layers,
+    sequences, positions, kv_heads, dim]``, dim 64 or 128; ``lengths``: rows that each sequence holds, an int32 tensor
+    ``[sequences]`` or one number for all.  Query t sees the rows up to its own, ``length - queries + t``.
+    """
+    bf16 = torch.bfloat16
+    s = _struct(MkbsKeyWeights)
+    if not all(isinstance(t, Tensor) for t in (q, keys, weights)) or q.ndim != 5 or keys.ndim != 5:
+        raise ValueError("q must be [layers, sequences, queries, heads, dim], keys [layers, sequences, positions, kv_heads, dim]")
+    s.layers, s.sequences, s.queries, s.heads, s.dim = q.shape
+    s.positions, s.kv_heads = keys.shape[2], keys.shape[3]
+    s.q = _check("q", q, bf16, inner=3)
+    s.k = _check("keys", keys, bf16, (s.layers, s.sequences, s.positions, s.kv_heads, s.dim), inner=3)
+    s.weights = _check("weights", weights, torch.float32, (s.layers, s.sequences, s.kv_heads, s.positions), inner=1)
+    s.q_layer, s.q_sequence, s.k_layer, s.k_sequence = q.stride(0), q.stride(1), keys.stride(0), keys.stride(1)
+    s.w_layer, s.w_sequence, s.w_head = weights.stride()[:3]
+    lengths = _lengths(s, lengths, s.sequences, s.positions)
+    s.scale, s.wait_timeout_ms = float(scale), wait_timeout_ms
+    s.status = _check("status", status, torch.int32) if status is not None else None
+    if status is not None and status.numel() < 16:
+        raise ValueError("status must hold 16 words")
+    where = _stream(stream, q.device)
+    s.workspace_bytes = load_library().mkb_key_weights_bytes(ctypes.byref(s))
+    workspace = _workspace(s.workspace_bytes, where, q.device)
+    s.workspace = workspace.data_ptr()
+    _call("key_weights", s, where)
+    _keep_alive(where, q, keys, weights, lengths, status)
+
+
+def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int = 0, recent: int = 0, kept: Tensor | None = None, stream=None) -> Tensor:
+    """Rows that stay when sequences are cut to ``keep`` rows: all of a sequence that has no more, else its first
+    ``sinks``, its last ``recent`` and the heaviest others by ``weights`` (float32 ``[layers, sequences, kv_heads, positions]``;
+    equal weights: the lowest row).
+
+    Returns int32 ``[layers, sequences, kv_heads, keep]``: the rows, ascending, and -1 behind them.  ``kept`` (shape and strides of
+    ``weights``, or ``weights`` itself) receives the weights of these rows in their new places.
+    """
+    if not isinstance(weights, Tensor) or weights.ndim != 4:
+        raise ValueError("weights must be [layers, sequences, kv_heads, positions]")
+    s = _struct(MkbsSelect)
+    s.layers, s.sequences, s.kv_heads, s.positions = weights.shape
+    s.weights = _check("weights", weights, torch.float32, inner=1)
+    s.w_layer, s.w_sequence, s.w_head = weights.stride()[:3]
+    s.keep, s.sinks, s.recent = keep, sinks, recent
+    lengths = _lengths(s, lengths, s.sequences, s.positions)
+    if kept is not None:
+        s.kept = _check("kept", kept, torch.float32, weights.shape, inner=1)
+        if kept.stride() != weights.stride():
+            raise ValueError("kept must have the strides of weights")
+    where = _stream(stream, weights.device)
+    with torch.cuda.stream(where):
+        rows = torch.empty(s.layers, s.sequences, s.kv_heads, max(keep, 0), dtype=torch.int32, device=weights.device)
+    s.rows = rows.data_ptr()
+    _call("select_rows", s, where)
+    _keep_alive(where, weights, lengths, kept)
+    return rows
+
+
+def move_rows(keys: Tensor, values: Tensor | None, rows: Tensor, lengths: Tensor | int, *, stream=None) -> None:
+    """Row r of every key/value head <- its row ``rows[..., r]``, in place, in caches ``[layers, sequences, positions,
+    kv_heads, dim]`` of one shape; ``rows`` as :func:`select_rows` returns them, ``lengths`` as it was given there."""
+    s = _struct(MkbsMove)
+    if not all(isinstance(t, Tensor) for t in (keys, rows)) or keys.ndim != 5 or rows.ndim != 4:
+        raise ValueError("caches must be [layers, sequences, positions, kv_heads, dim], rows [layers, sequences, kv_heads, keep]")
+    s.layers, s.sequences, s.positions, s.kv_heads, dim = keys.shape
+    s.caches[0] = _check("keys", keys, keys.dtype, inner=3)
+    if values is not None:
+        s.caches[1] = _check("values", values, keys.dtype, keys.shape, inner=3)
+        if values.stride() != keys.stride():
+            raise ValueError("keys and values must have the same strides")
+    size = keys.element_size()
+    s.head_bytes, s.c_layer, s.c_sequence = dim * size, keys.stride(0) * size, keys.stride(1) * size
+    s.keep = rows.shape[3]
+    s.rows = _check("rows", rows, torch.int32, (s.layers, s.sequences, s.kv_heads, s.keep))
+    lengths = _lengths(s, lengths, s.sequences, s.positions)
+    where = _stream(stream, keys.device)
+    _call("move_rows", s, where)
+    _keep_alive(where, keys, values, rows, lengths)
