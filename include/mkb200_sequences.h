@@ -103,7 +103,8 @@ int mkb_reorder_slots(const MkbsReorder *r, void *cuda_stream);
  */
 typedef struct MkbsKeyWeights {
     uint32_t struct_bytes;
-    int32_t layers, sequences, queries, heads, kv_heads;
+    int32_t layers, sequences, queries;
+    int32_t heads, kv_heads;   /* at most 128 query heads per key/value head */
     int32_t dim;               /* 64 or 128 */
     int32_t positions;         /* rows of a sequence's cache */
     int32_t length;            /* rows that every sequence holds, where `lengths` is NULL */

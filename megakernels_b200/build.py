@@ -63,8 +63,8 @@ LIBRARIES = {
     "sequences": Library(
         "libmkb200_sequences.so",
         ("sequence_host.cu", "sequence_beam.cu", "sequence_rows.cu", "sequence_weights.cu"),
-        ("sequence_kernels.h", "../../include/mkb200_sequences.h", "hybrid_common.cuh", "mk_common.cuh", "../../include/mkb200.h",
-         "../../include/mkb200_hybrid.h"),
+        ("sequence_kernels.h", "../../include/mkb200_sequences.h", "hybrid_common.cuh", "hybrid_kernels.h", "hybrid_tcgen05.cuh", "mk_common.cuh",
+         "../../include/mkb200.h", "../../include/mkb200_hybrid.h"),
     ),
 }
 

@@ -90,8 +90,8 @@ int check_shape(const MkbsKeyWeights* w) {
     if (!w || w->struct_bytes != sizeof(MkbsKeyWeights)) return invalid("key weights: NULL or another struct size");
     if (const int rc = check_items("key weights", w->layers, w->sequences, w->kv_heads, w->positions, w->length, w->lengths)) return rc;
     if (w->queries < 1 || w->heads < w->kv_heads || w->heads % w->kv_heads) return invalid("key weights: queries must be positive, heads a multiple of kv_heads");
-    if ((w->dim != 64 && w->dim != 128) || w->heads > 1024 || (int64_t)w->queries * (w->heads / w->kv_heads) > 1 << 20)
-        return fail(MKBS_ERR_UNSUPPORTED, "key weights: dim 64 or 128, at most 1024 heads and 2^20 queries * heads of a key");
+    if ((w->dim != 64 && w->dim != 128) || w->heads / w->kv_heads > 128 || (int64_t)w->queries * (w->heads / w->kv_heads) > 1 << 20)
+        return fail(MKBS_ERR_UNSUPPORTED, "key weights: dim 64 or 128, at most 128 heads of a key and 2^20 queries times them");
     return MKBS_OK;
 }
 int check(const MkbsKeyWeights* w) {
@@ -100,8 +100,9 @@ int check(const MkbsKeyWeights* w) {
     if (!aligned(w->q, 16) || !aligned(w->k, 16) || !aligned(w->weights, 4) || (w->status && !aligned(w->status, 4)))
         return invalid("key weights: q, k or weights missing or unaligned");
     if (w->q_layer % 8 || w->q_sequence % 8 || w->k_layer % 8 || w->k_sequence % 8) return invalid("key weights: strides of q and k are multiples of 8");
-    if (w->q_layer < 0 || w->k_layer < 0 || w->w_layer < 0 || (w->sequences > 1 && (w->q_sequence < w->queries * q_row || w->k_sequence < w->positions * k_row)))
-        return invalid("key weights: sequences overlap");
+    if ((w->layers > 1 && (w->q_layer < w->queries * q_row || w->k_layer < w->positions * k_row)) ||
+        (w->sequences > 1 && (w->q_sequence < w->queries * q_row || w->k_sequence < w->positions * k_row)))
+        return invalid("key weights: sequences or layers of q or k overlap");
     if ((w->kv_heads > 1 && w->w_head < w->positions) || (w->sequences > 1 && w->w_sequence < w->positions) || (w->layers > 1 && w->w_layer < w->positions))
         return invalid("key weights: weights overlap");
     if (!(w->scale - w->scale == 0.f)) return invalid("key weights: scale is not finite");

@@ -120,7 +120,7 @@ REFUSED = [
     ]),
     ("key_weights", weights_struct, [
         (dict(struct_bytes=8), 1, "struct size"), (dict(layers=0), 1, "positive"), (dict(positions=0), 1, "positive"), (dict(queries=0), 1, "queries"), (dict(heads=7), 1, "multiple"),
-        (dict(heads=0), 1, "multiple"), (dict(dim=96), 5, "dim"), (dict(length=101), 1, "length"), (dict(length=-1), 1, "length"), (dict(lengths=FAKE + 2), 1, "length"),
+        (dict(heads=0), 1, "multiple"), (dict(dim=96), 5, "dim"), (dict(heads=258), 5, "128 heads"), (dict(q_layer=1528), 1, "overlap"), (dict(k_layer=12792), 1, "overlap"), (dict(length=101), 1, "length"), (dict(length=-1), 1, "length"), (dict(lengths=FAKE + 2), 1, "length"),
         (dict(layers=60000), 5, "65535"), (dict(positions=1 << 29), 5, "positions"), (dict(queries=1 << 20), 5, "2^20"), (dict(q=FAKE + 8), 1, "unaligned"), (dict(k=None), 1, "missing"),
         (dict(weights=FAKE + 2), 1, "unaligned"), (dict(q_layer=4), 1, "multiples of 8"), (dict(k_sequence=12804), 1, "multiples of 8"), (dict(k_sequence=12792), 1, "overlap"),
         (dict(q_sequence=1528), 1, "overlap"), (dict(w_head=99), 1, "overlap"), (dict(w_sequence=99), 1, "overlap"), (dict(w_layer=99), 1, "overlap"), (dict(scale=math.nan), 1, "finite"),
@@ -425,7 +425,7 @@ def test_key_weights(queries, positions, lengths, heads, kv_heads, dim):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("per", [3, 5, 7, 12])
+@pytest.mark.parametrize("per", [3, 5, 7, 12, 24, 100])
 def test_key_weights_of_odd_numbers_of_heads(per):
     q, k, w, scale = weights_case(per, 1, 2, 21, 2 * per, 2, 64, 333, [333, 200])
     check_weights(q, k, w, [333, 200], scale)
