@@ -333,7 +333,7 @@ template <typename T>
 cudaError_t launch(const BeamPlan& p, const MkbsBeams& b, const BeamArgs& a, cudaStream_t s) {
     const size_t smem = p.merge_smem();
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = allow_shared_memory<beam_merge_kernel<T>>();
         if (e != cudaSuccess) return e;
     }
     beam_scan_kernel<T><<<dim3((p.parts + kScanWarps - 1) / kScanWarps, p.rows), 32 * kScanWarps, 0, s>>>(a);

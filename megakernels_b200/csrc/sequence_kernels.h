@@ -1,5 +1,7 @@
 // Launchers of the operators between two decoding steps (one translation unit per group); arguments have been checked.
 #pragma once
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -11,6 +13,7 @@ namespace mkbs {
 using bf16 = __nv_bfloat16;
 
 constexpr int kSms = 148;  // what grids and splits are sized by
+constexpr int kStaticShared = 16 * 1024;  // most that a kernel has besides
 
 // Total order of floats as whole numbers; 0 is below all of them.  Minus zero counts as zero.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -22,6 +25,18 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 // Rows that sequence `b` holds.
 __device__ __forceinline__ int length_of(const int32_t* lengths, int length, int positions, int b) {
     return min(max(lengths != nullptr ? __ldg(lengths + b) : length, 0), positions);
+}
+
+// Lets `kernel` have all of an SM's shared memory, once per device.
+template <auto kernel>
+inline cudaError_t allow_shared_memory() {
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || set[dev & 63].load(std::memory_order_relaxed)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStaticShared);
+    if (e == cudaSuccess) set[dev & 63].store(dev < 64, std::memory_order_relaxed);
+    return e;
 }
 
 cudaError_t beam_launch(const MkbsBeams& b, cudaStream_t s);

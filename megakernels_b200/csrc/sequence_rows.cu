@@ -196,6 +196,13 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MkbsMove m) {
     }
 }
 
+template <typename V>
+cudaError_t reorder(const ReorderArgs& a, cudaStream_t s) {
+    if (const cudaError_t e = allow_shared_memory<reorder_kernel<V>>(); e != cudaSuccess) return e;
+    reorder_kernel<V><<<2 * kSms, kReorderThreads, kReorderBytes, s>>>(a);
+    return cudaGetLastError();
+}
+
 }  // namespace
 
 cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
@@ -205,10 +212,7 @@ cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
         const MkbsRegion& g = a.regions[i] = r.regions[i];
         bits |= reinterpret_cast<uintptr_t>(g.base) | (uintptr_t)g.outer_stride | (uintptr_t)g.slot_stride | (uintptr_t)g.row_bytes;
     }
-    const auto kernel = bits % 16 == 0 ? reorder_kernel<uint4> : bits % 4 == 0 ? reorder_kernel<uint32_t> : reorder_kernel<uint8_t>;
-    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kReorderBytes); e != cudaSuccess) return e;
-    kernel<<<2 * kSms, kReorderThreads, kReorderBytes, s>>>(a);
-    return cudaGetLastError();
+    return bits % 16 == 0 ? reorder<uint4>(a, s) : bits % 4 == 0 ? reorder<uint32_t>(a, s) : reorder<uint8_t>(a, s);
 }
 
 cudaError_t select_launch(const MkbsSelect& a, cudaStream_t s) {

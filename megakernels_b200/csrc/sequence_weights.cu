@@ -95,7 +95,7 @@ struct Smem {
         total = ctl + 16;
     }
 };
-static_assert((6 + 2) * kSlab + 6 * 512 + 4096 + 1024 < 227 * 1024 && (4 + 2) * 2 * kSlab + 4 * 512 + 4096 + 1024 + 512 < 227 * 1024, "shared memory of a block");
+static_assert((6 + 2) * kSlab + 6 * 512 + 4096 + 2048 < 227 * 1024 - kStaticShared && (4 + 2) * 2 * kSlab + 4 * 512 + 4096 + 2048 < 227 * 1024 - kStaticShared, "shared memory of a block");
 
 // What the roles of both kernels share.
 template <int kDim, bool kKeys>
@@ -600,8 +600,8 @@ cudaError_t launch(const MkbsKeyWeights& w, const Plan& p, cudaStream_t s) {
     const cuuint32_t k_box[4] = {64, kTile, 1, 1};
     if ((e = encode(&maps.k, a.k, 4, k_size, k_stride, k_box)) != cudaSuccess) return e;
     const int rows_smem = Smem<kDim>(false).total + 1024, keys_smem = Smem<kDim>(true).total + 1024;
-    if ((e = cudaFuncSetAttribute(weights_rows_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem)) != cudaSuccess) return e;
-    if ((e = cudaFuncSetAttribute(weights_keys_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, keys_smem)) != cudaSuccess) return e;
+    if ((e = allow_shared_memory<weights_rows_kernel<kDim>>()) != cudaSuccess) return e;
+    if ((e = allow_shared_memory<weights_keys_kernel<kDim>>()) != cudaSuccess) return e;
     weights_rows_kernel<kDim><<<dim3(a.splits, a.row_tiles, p.items), kThreads, rows_smem, s>>>(maps, a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     if (a.splits > 1 && (e = launch_early(weights_join_kernel, dim3(p.items * a.row_tiles), dim3(kTile), 0, s, a)) != cudaSuccess) return e;

@@ -14,6 +14,7 @@ them can be captured into a CUDA graph.  Arguments that the library does not tak
 from __future__ import annotations
 
 import ctypes
+import math
 from pathlib import Path
 
 import torch
@@ -111,55 +112,65 @@ def load_library() -> ctypes.CDLL:
     return lib
 
 
-def _check(name: str, t, dtype, shape=None, inner: int | None = None) -> int:
-    """Address of a tensor on the current device.  ``shape``: what it must be; ``inner``: trailing dimensions that
-    must lie one behind the other (None: all)."""
+def _refuse_host(name: str, t: Tensor):
+    if not t.is_cuda:  # (before anything asks for a current device, which there may not be)
+        raise ValueError(f"{name} must live on a CUDA device")
+
+
+def _refuse(name: str, t, dtype, device: int, shape, inner: int | None):
+    """Why a tensor is not what a call needs."""
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must live on a CUDA device")
-    if t.device.index != torch.cuda.current_device():  # (the launch goes to the current device)
-        raise ValueError(f"{name} lives on cuda:{t.device.index} but the current device is cuda:{torch.cuda.current_device()} "
-                         "(wrap the call in torch.cuda.device(...))")
+    if t.get_device() != device:  # (the launch goes to the current device)
+        raise ValueError(f"{name} lives on cuda:{t.get_device()} but the current device is cuda:{device} (wrap the call in torch.cuda.device(...))")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if inner is None:
-        dense = t.is_contiguous()
-    else:
-        part = t[(0,) * (t.ndim - inner)] if t.numel() else t
-        dense = part.is_contiguous()
-    if not dense:
-        raise ValueError(f"{name} must be contiguous" + ("" if inner is None else f" in its last {inner} dimensions"))
-    return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous" + ("" if inner is None else f" in its last {inner} dimensions"))
 
 
-def _stream(stream, device) -> torch.cuda.Stream:
-    if stream is None:
-        return torch.cuda.current_stream(device)
-    if isinstance(stream, int):
-        return torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
-    return stream
+def _check(name: str, t, dtype, device: int, shape=None, inner: int | None = None) -> int:
+    """Address of a tensor on the current device.  ``shape``: what it must be; ``inner``: how many of its last dimensions
+    must lie one behind the other (None: all)."""
+    # (a call's checks cost more than its launch, so what is right passes through one condition)
+    if (isinstance(t, Tensor) and t.dtype is dtype and t.get_device() == device and (shape is None or t.shape == shape)
+            and (t.is_contiguous() or (inner is not None and t.numel() and t[(0,) * (t.ndim - inner)].is_contiguous()))):
+        return t.data_ptr()
+    _refuse(name, t, dtype, device, shape, inner)
 
 
-def _workspace(nbytes: int, stream: torch.cuda.Stream, device) -> Tensor:
-    with torch.cuda.stream(stream):  # (given back when the call returns, to that stream alone: later work on it runs after the kernels)
-        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+class _Where:
+    """The stream of a call, and the tensors that it allocates there: given back when the call returns they go to
+    that stream alone, whose later work runs after the kernels."""
 
+    def __init__(self, stream):
+        self.device = torch.cuda.current_device()
+        if stream is None:
+            self.other, self.handle = None, torch.cuda.current_stream(self.device).cuda_stream
+        elif isinstance(stream, int):  # (an external stream of handle 0 would be another one from torch's pool)
+            self.other = torch.cuda.ExternalStream(stream, device=self.device) if stream else torch.cuda.default_stream(self.device)
+            self.handle = stream
+        else:
+            self.other, self.handle = stream, stream.cuda_stream
 
-def _keep_alive(stream: torch.cuda.Stream, *tensors) -> None:
-    """Tensors of another stream are not given out again before this stream has used them."""
-    for t in tensors:
-        if t is not None and stream != torch.cuda.current_stream(t.device):
-            t.record_stream(stream)
+    def empty(self, *shape, dtype) -> Tensor:
+        if self.other is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.other):
+            return torch.empty(shape, dtype=dtype, device=self.device)
 
-
-def _call(name: str, struct, stream: torch.cuda.Stream) -> None:
-    lib = load_library()
-    code = getattr(lib, f"mkb_{name}")(ctypes.byref(struct), ctypes.c_void_p(stream.cuda_stream))
-    if code:
-        raise SequenceError(code, lib.mkb_sequences_last_error().decode())
+    def launch(self, name: str, struct, *used) -> None:
+        """``used``: tensors that are not given out again before this stream has used them."""
+        code = getattr(_lib, name)(ctypes.byref(struct), self.handle)
+        if code:
+            raise SequenceError(code, _lib.mkb_sequences_last_error().decode())
+        if self.other is not None and self.other != torch.cuda.current_stream(self.device):
+            for t in used:
+                if t is not None:
+                    t.record_stream(self.other)
 
 
 def _struct(kind):
@@ -168,12 +179,12 @@ def _struct(kind):
     return s
 
 
-def _lengths(s, lengths, sequences: int, positions: int):
+def _set_lengths(s, lengths, device: int, sequences: int, positions: int):
     """Rows that each sequence holds: an int32 tensor on the device, or one number for all."""
     if isinstance(lengths, Tensor):
-        s.lengths = _check("lengths", lengths, torch.int32, (sequences,))
+        s.lengths = _check("lengths", lengths, torch.int32, device, (sequences,))
         return lengths
-    s.lengths, s.length = None, int(lengths)
+    s.length = int(lengths)
     if not 0 <= s.length <= positions:
         raise ValueError(f"length {lengths} outside a cache of {positions} rows")
     return None
@@ -192,25 +203,28 @@ def beam_select(logits: Tensor, scores: Tensor | None = None, *, beams: int, k: 
         raise ValueError("logits must be [groups * beams, vocab]")
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"logits must be bfloat16 or float32, got {logits.dtype}")
-    if beams < 1 or logits.shape[0] < 1 or logits.shape[0] % beams:
-        raise ValueError(f"{logits.shape[0]} rows of logits are no groups of {beams}")
-    s = _struct(MkbsBeams)
-    rows, s.vocab = logits.shape
-    s.groups, s.beams, s.k, s.dtype = rows // beams, beams, k, int(logits.dtype == torch.float32)
-    s.row_stride = logits.stride(0) if rows > 1 else s.vocab
-    s.logits = _check("logits", logits, logits.dtype, inner=1)
-    s.scores = _check("scores", scores, torch.float32, (s.groups, beams)) if scores is not None else None
-    s.done = _check("done", done, torch.uint8, (s.groups, beams)) if done is not None else None
+    rows, vocab = logits.shape
+    if beams < 1 or rows < 1 or rows % beams:
+        raise ValueError(f"{rows} rows of logits are no groups of {beams}")
+    _refuse_host("logits", logits)
+    lib, where, groups = load_library(), _Where(stream), rows // beams
+    s, device = _struct(MkbsBeams), where.device
+    s.groups, s.beams, s.vocab, s.k, s.dtype = groups, beams, vocab, k, int(logits.dtype is torch.float32)
+    s.row_stride = logits.stride(0) if rows > 1 else vocab
+    s.logits = _check("logits", logits, logits.dtype, device, inner=1)
+    if scores is not None:
+        s.scores = _check("scores", scores, torch.float32, device, (groups, beams))
+    if done is not None:
+        s.done = _check("done", done, torch.uint8, device, (groups, beams))
     s.eos = -1 if eos is None else int(eos)
-    lib, where = load_library(), _stream(stream, logits.device)
-    with torch.cuda.stream(where):
-        out = [torch.empty(s.groups, max(k, 0), dtype=t, device=logits.device) for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+    size = lib.mkb_beam_bytes(s)
+    if not size:
+        where.launch("mkb_beam_select", s)  # (says what is wrong)
+    out = [where.empty(groups, k, dtype=t) for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+    workspace = where.empty(size, dtype=torch.uint8)
     s.out_scores, s.out_parents, s.out_tokens, s.out_done = (t.data_ptr() for t in out)
-    s.workspace_bytes = lib.mkb_beam_bytes(ctypes.byref(s))
-    workspace = _workspace(s.workspace_bytes, where, logits.device)
-    s.workspace = workspace.data_ptr()
-    _call("beam_select", s, where)
-    _keep_alive(where, logits, scores, done)
+    s.workspace, s.workspace_bytes = workspace.data_ptr(), size
+    where.launch("mkb_beam_select", s, logits, scores, done)
     return tuple(out)
 
 
@@ -230,34 +244,35 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
         raise ValueError("first counts rows: it is not negative and needs lengths")
     if not isinstance(parents, Tensor) or parents.ndim != 1:
         raise ValueError("parents must be int32 [slots]")
-    slots = parents.shape[0]
-    base = _struct(MkbsReorder)
+    _refuse_host("parents", parents)
+    load_library()
+    slots, where = parents.shape[0], _Where(stream)
+    base, device = _struct(MkbsReorder), where.device
     base.slots, base.first = slots, first
-    base.parents = _check("parents", parents, torch.int32)
-    base.lengths = _check("lengths", lengths, torch.int32, (slots,)) if lengths is not None else None
-    regions = []
-    for i, t in enumerate(tensors):
+    base.parents = _check("parents", parents, torch.int32, device)
+    by_rows = lengths is not None
+    if by_rows:
+        base.lengths = _check("lengths", lengths, torch.int32, device, (slots,))
+    regions = (MkbsRegion * len(tensors))()
+    for r, (i, t) in zip(regions, enumerate(tensors)):
         if not isinstance(t, Tensor):
             raise TypeError(f"tensor {i} must be a torch.Tensor")
-        if t.ndim < dim + 1 + (lengths is not None) or t.shape[dim] != slots:
-            raise ValueError(f"tensor {i} {list(t.shape)} does not have {slots} slots in dimension {dim}" + (" and rows behind it" if lengths is not None else ""))
+        shape = t.shape
+        if len(shape) < dim + 1 + by_rows or shape[dim] != slots:
+            raise ValueError(f"tensor {i} {list(shape)} does not have {slots} slots in dimension {dim}" + (" and rows behind it" if by_rows else ""))
         if t.numel() == 0:
             raise ValueError(f"tensor {i} is empty")
-        r = MkbsRegion()
-        r.base = _check(f"tensor {i}", t, t.dtype, inner=t.ndim - dim - 1)
+        r.base = _check(f"tensor {i}", t, t.dtype, device, inner=len(shape) - dim - 1)
         size = t.element_size()
-        r.outer, r.outer_stride = (t.shape[0], t.stride(0) * size) if dim else (1, 0)
-        r.slot_stride = t.stride(dim) * size if slots > 1 else t[(0,) * (dim + 1)].numel() * size
-        r.rows = t.shape[dim + 1] if lengths is not None else 1
-        r.row_bytes = t[(0,) * (dim + 1)].numel() * size // r.rows
-        regions.append(r)
-    where = _stream(stream, parents.device)
-    for at in range(0, len(regions), MAX_REGIONS):
-        some = regions[at : at + MAX_REGIONS]
-        array = (MkbsRegion * len(some))(*some)
-        base.num_regions, base.regions = len(some), ctypes.cast(array, ctypes.POINTER(MkbsRegion))
-        _call("reorder_slots", base, where)
-    _keep_alive(where, parents, lengths, *tensors)
+        slot_bytes = math.prod(shape[dim + 1 :]) * size
+        r.outer, r.outer_stride = (shape[0], t.stride(0) * size) if dim else (1, 0)
+        r.slot_stride = t.stride(dim) * size if slots > 1 else slot_bytes
+        r.rows = shape[dim + 1] if by_rows else 1
+        r.row_bytes = slot_bytes // r.rows
+    for at in range(0, len(tensors), MAX_REGIONS):
+        base.num_regions = min(MAX_REGIONS, len(tensors) - at)
+        base.regions = ctypes.cast(ctypes.byref(regions, at * ctypes.sizeof(MkbsRegion)), ctypes.POINTER(MkbsRegion))
+        where.launch("mkb_reorder_slots", base, parents, lengths, *tensors)
 
 
 def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int, *, scale: float, status: Tensor | None = None, wait_timeout_ms: int = 0,
@@ -269,28 +284,32 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
     sequences, positions, kv_heads, dim]``, dim 64 or 128; ``lengths``: rows that each sequence holds, an int32 tensor
     ``[sequences]`` or one number for all.  Query t sees the rows up to its own, ``length - queries + t``.
     """
-    bf16 = torch.bfloat16
-    s = _struct(MkbsKeyWeights)
     if not all(isinstance(t, Tensor) for t in (q, keys, weights)) or q.ndim != 5 or keys.ndim != 5:
         raise ValueError("q must be [layers, sequences, queries, heads, dim], keys [layers, sequences, positions, kv_heads, dim]")
-    s.layers, s.sequences, s.queries, s.heads, s.dim = q.shape
-    s.positions, s.kv_heads = keys.shape[2], keys.shape[3]
-    s.q = _check("q", q, bf16, inner=3)
-    s.k = _check("keys", keys, bf16, (s.layers, s.sequences, s.positions, s.kv_heads, s.dim), inner=3)
-    s.weights = _check("weights", weights, torch.float32, (s.layers, s.sequences, s.kv_heads, s.positions), inner=1)
-    s.q_layer, s.q_sequence, s.k_layer, s.k_sequence = q.stride(0), q.stride(1), keys.stride(0), keys.stride(1)
+    _refuse_host("q", q)
+    lib, where, bf16 = load_library(), _Where(stream), torch.bfloat16
+    s, device = _struct(MkbsKeyWeights), where.device
+    layers, sequences, s.queries, s.heads, dim = q.shape
+    positions, kv_heads = keys.shape[2:4]
+    s.layers, s.sequences, s.dim, s.positions, s.kv_heads = layers, sequences, dim, positions, kv_heads
+    s.q = _check("q", q, bf16, device, inner=3)
+    s.k = _check("keys", keys, bf16, device, (layers, sequences, positions, kv_heads, dim), inner=3)
+    s.weights = _check("weights", weights, torch.float32, device, (layers, sequences, kv_heads, positions), inner=1)
+    s.q_layer, s.q_sequence = q.stride()[:2]
+    s.k_layer, s.k_sequence = keys.stride()[:2]
     s.w_layer, s.w_sequence, s.w_head = weights.stride()[:3]
-    lengths = _lengths(s, lengths, s.sequences, s.positions)
-    s.scale, s.wait_timeout_ms = float(scale), wait_timeout_ms
-    s.status = _check("status", status, torch.int32) if status is not None else None
-    if status is not None and status.numel() < 16:
-        raise ValueError("status must hold 16 words")
-    where = _stream(stream, q.device)
-    s.workspace_bytes = load_library().mkb_key_weights_bytes(ctypes.byref(s))
-    workspace = _workspace(s.workspace_bytes, where, q.device)
-    s.workspace = workspace.data_ptr()
-    _call("key_weights", s, where)
-    _keep_alive(where, q, keys, weights, lengths, status)
+    lengths = _set_lengths(s, lengths, device, sequences, positions)
+    s.scale, s.wait_timeout_ms = scale, wait_timeout_ms
+    if status is not None:
+        s.status = _check("status", status, torch.int32, device)
+        if status.numel() < 16:
+            raise ValueError("status must hold 16 words")
+    size = lib.mkb_key_weights_bytes(s)
+    if not size:
+        where.launch("mkb_key_weights", s)  # (says what is wrong)
+    workspace = where.empty(size, dtype=torch.uint8)
+    s.workspace, s.workspace_bytes = workspace.data_ptr(), size
+    where.launch("mkb_key_weights", s, q, keys, weights, lengths, status)
 
 
 def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int = 0, recent: int = 0, kept: Tensor | None = None, stream=None) -> Tensor:
@@ -303,42 +322,45 @@ def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int
     """
     if not isinstance(weights, Tensor) or weights.ndim != 4:
         raise ValueError("weights must be [layers, sequences, kv_heads, positions]")
-    s = _struct(MkbsSelect)
-    s.layers, s.sequences, s.kv_heads, s.positions = weights.shape
-    s.weights = _check("weights", weights, torch.float32, inner=1)
+    _refuse_host("weights", weights)
+    load_library()
+    s, where = _struct(MkbsSelect), _Where(stream)
+    device = where.device
+    layers, sequences, kv_heads, positions = weights.shape
+    s.layers, s.sequences, s.kv_heads, s.positions = layers, sequences, kv_heads, positions
+    s.weights = _check("weights", weights, torch.float32, device, inner=1)
     s.w_layer, s.w_sequence, s.w_head = weights.stride()[:3]
     s.keep, s.sinks, s.recent = keep, sinks, recent
-    lengths = _lengths(s, lengths, s.sequences, s.positions)
+    lengths = _set_lengths(s, lengths, device, sequences, positions)
     if kept is not None:
-        s.kept = _check("kept", kept, torch.float32, weights.shape, inner=1)
+        s.kept = _check("kept", kept, torch.float32, device, weights.shape, inner=1)
         if kept.stride() != weights.stride():
             raise ValueError("kept must have the strides of weights")
-    where = _stream(stream, weights.device)
-    with torch.cuda.stream(where):
-        rows = torch.empty(s.layers, s.sequences, s.kv_heads, max(keep, 0), dtype=torch.int32, device=weights.device)
+    rows = where.empty(layers, sequences, kv_heads, max(keep, 1), dtype=torch.int32)  # (the library refuses less)
     s.rows = rows.data_ptr()
-    _call("select_rows", s, where)
-    _keep_alive(where, weights, lengths, kept)
+    where.launch("mkb_select_rows", s, weights, lengths, kept)
     return rows
 
 
 def move_rows(keys: Tensor, values: Tensor | None, rows: Tensor, lengths: Tensor | int, *, stream=None) -> None:
     """Row r of every key/value head <- its row ``rows[..., r]``, in place, in caches ``[layers, sequences, positions,
     kv_heads, dim]`` of one shape; ``rows`` as :func:`select_rows` returns them, ``lengths`` as it was given there."""
-    s = _struct(MkbsMove)
     if not all(isinstance(t, Tensor) for t in (keys, rows)) or keys.ndim != 5 or rows.ndim != 4:
         raise ValueError("caches must be [layers, sequences, positions, kv_heads, dim], rows [layers, sequences, kv_heads, keep]")
-    s.layers, s.sequences, s.positions, s.kv_heads, dim = keys.shape
-    s.caches[0] = _check("keys", keys, keys.dtype, inner=3)
+    _refuse_host("keys", keys)
+    load_library()
+    s, where = _struct(MkbsMove), _Where(stream)
+    device = where.device
+    layers, sequences, positions, kv_heads, dim = keys.shape
+    s.layers, s.sequences, s.positions, s.kv_heads = layers, sequences, positions, kv_heads
+    s.caches[0] = _check("keys", keys, keys.dtype, device, inner=3)
     if values is not None:
-        s.caches[1] = _check("values", values, keys.dtype, keys.shape, inner=3)
+        s.caches[1] = _check("values", values, keys.dtype, device, keys.shape, inner=3)
         if values.stride() != keys.stride():
             raise ValueError("keys and values must have the same strides")
     size = keys.element_size()
     s.head_bytes, s.c_layer, s.c_sequence = dim * size, keys.stride(0) * size, keys.stride(1) * size
     s.keep = rows.shape[3]
-    s.rows = _check("rows", rows, torch.int32, (s.layers, s.sequences, s.kv_heads, s.keep))
-    lengths = _lengths(s, lengths, s.sequences, s.positions)
-    where = _stream(stream, keys.device)
-    _call("move_rows", s, where)
-    _keep_alive(where, keys, values, rows, lengths)
+    s.rows = _check("rows", rows, torch.int32, device, (layers, sequences, kv_heads, s.keep))
+    lengths = _set_lengths(s, lengths, device, sequences, positions)
+    where.launch("mkb_move_rows", s, keys, values, rows, lengths)
