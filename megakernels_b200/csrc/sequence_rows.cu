@@ -6,9 +6,12 @@ namespace mkbs {
 namespace {
 
 // ---- x[slot] <- x[parents[slot]] ---------------------------------------------------------- //
-// A block takes one run of bytes of all slots at once: it reads what other slots take into shared memory, each source once
-// however many take it, and writes it when all of it is there.  Runs do not overlap, so no slot loses what another still needs.
-constexpr int kReorderThreads = 512, kReorderBytes = 96 * 1024;
+// A block takes one run of bytes of all slots that depend on each other at once: it reads what other slots take into shared
+// memory, each source once however many take it, and writes it when all of it is there.  Runs do not overlap, so no slot loses
+// what another still needs.  Slots that depend on each other are the components of the graph of parents (a beam search's
+// groups): the fewer sources a run has, the longer its copies are.
+constexpr int kReorderThreads = 256, kReorderBytes = 96 * 1024;  // (bytes: of the plain kernel)
+constexpr int kStages = 4, kStageBytes = 52 * 1024, kShortRun = 2048;
 
 struct ReorderArgs {
     int slots, num_regions, first;
@@ -16,6 +19,191 @@ struct ReorderArgs {
     MkbsRegion regions[MKBS_MAX_REGIONS];
 };
 
+struct Components {
+    int parent[MKBS_MAX_SLOTS], length[MKBS_MAX_SLOTS], label[MKBS_MAX_SLOTS], place[MKBS_MAX_SLOTS];
+    int source[MKBS_MAX_SLOTS], target[MKBS_MAX_SLOTS];  // sources, and slots that take one, by component
+    int source_begin[MKBS_MAX_SLOTS + 1], target_begin[MKBS_MAX_SLOTS + 1], run[MKBS_MAX_SLOTS], longest[MKBS_MAX_SLOTS];
+    int count, changed;
+    unsigned long long bytes;  // that all sources hold
+
+    __device__ __forceinline__ bool moves(int s, int first) const { return parent[s] != s && length[parent[s]] > first; }
+
+    // By all threads of a block of kReorderThreads.
+    __device__ void find(const ReorderArgs& a) {
+        const int s = threadIdx.x, n = a.slots;
+        static_assert(kReorderThreads == MKBS_MAX_SLOTS, "a thread per slot");
+        if (s < n) {
+            const int p = a.parents[s];
+            parent[s] = p >= 0 && p < n ? p : s;
+            length[s] = a.lengths != nullptr ? max(a.lengths[s], 0) : 1 << 30;
+            label[s] = s;
+            place[s] = 0;
+        }
+        if (s == 0) count = 0, bytes = 0;
+        __syncthreads();
+        const bool taken = s < n && moves(s, a.first);
+        if (taken) place[parent[s]] = 1;
+        do {  // every slot learns the lowest slot that it is connected with
+            __syncthreads();
+            if (s == 0) changed = 0;
+            __syncthreads();
+            if (taken) {
+                const int mine = label[s], its = label[parent[s]], low = min(mine, its);
+                if (mine > low) atomicMin(&label[s], low), changed = 1;
+                if (its > low) atomicMin(&label[parent[s]], low), changed = 1;
+            }
+            __syncthreads();
+        } while (changed);
+        // sources and targets in the order of their components, components in the order of their lowest slots
+        const bool source_here = s < n && place[s];
+        int sources = 0, targets = 0, before = 0, own_sources = 0, own_targets = 0, most = 0;
+        if (s < n) {
+            for (int i = 0; i < n; ++i) {
+                const bool first_of = label[i] < label[s] || (label[i] == label[s] && i < s), takes = moves(i, a.first);
+                sources += place[i] && first_of;
+                targets += takes && first_of;
+                if (label[i] == s) {
+                    own_sources += place[i];
+                    own_targets += takes;
+                    if (place[i]) most = max(most, length[i]);
+                }
+            }
+            run[s] = own_sources > 0;  // a component's lowest slot
+        }
+        __syncthreads();
+        if (s < n) {
+            for (int i = 0; i < s; ++i) before += run[i];
+            if (source_here) source[sources] = s, place[s] = sources;
+            if (taken) target[targets] = s;
+            if (own_sources > 0) {
+                longest[before] = most;
+                source_begin[before + 1] = own_sources;
+                target_begin[before + 1] = own_targets;
+                atomicMax(&count, before + 1);
+            }
+        }
+        __syncthreads();
+        if (s == 0) {
+            source_begin[0] = target_begin[0] = 0;
+            for (int c = 0; c < count; ++c) {
+                source_begin[c + 1] += source_begin[c];
+                target_begin[c + 1] += target_begin[c];
+            }
+        }
+        __syncthreads();
+        if (s < count) {
+            unsigned long long all = 0;
+            for (int r = 0; r < a.num_regions; ++r) all += (unsigned long long)(max(min(longest[s], a.regions[r].rows) - a.first, 0) * a.regions[r].row_bytes) * a.regions[r].outer;
+            atomicAdd(&bytes, all * (source_begin[s + 1] - source_begin[s]));
+        }
+        __syncthreads();
+        if (s < count) {
+            // four steps and more for every block, as far as copies do not get short
+            const int sources_here = source_begin[s + 1] - source_begin[s], longest_run = kStageBytes / sources_here / 128 * 128;
+            const int64_t share = (int64_t)(bytes / (4 * kSms) / sources_here + 127) / 128 * 128;
+            run[s] = (int)min((int64_t)longest_run, max((int64_t)kShortRun, share));
+        }
+        __syncthreads();
+    }
+};
+
+// A step: one run of the bytes of a component's slots, in one layer of one region.
+struct Step {
+    int c, r;
+    int64_t at, runs;  // step of this component and region, and how many runs a layer has there
+    __device__ __forceinline__ void count(const ReorderArgs& a, const Components& k) {
+        const MkbsRegion& g = a.regions[r];
+        const int64_t bytes = (min(k.longest[c], g.rows) - a.first) * g.row_bytes;
+        runs = bytes > 0 ? (bytes + k.run[c] - 1) / k.run[c] : 0;
+    }
+    __device__ __forceinline__ bool settle(const ReorderArgs& a, const Components& k) {  // false: there are no more
+        while (c < k.count && at >= runs * a.regions[r].outer) {
+            at -= runs * a.regions[r].outer;
+            if (++r == a.num_regions) r = 0, ++c;
+            if (c < k.count) count(a, k);
+        }
+        return c < k.count;
+    }
+    __device__ __forceinline__ Step(const ReorderArgs& a, const Components& k) : c(0), r(0), at(blockIdx.x), runs(0) {
+        if (k.count > 0) count(a, k);
+    }
+    __device__ __forceinline__ int64_t begin(const ReorderArgs& a, const Components& k) const { return a.first * a.regions[r].row_bytes + at % runs * k.run[c]; }
+    __device__ __forceinline__ char* base(const ReorderArgs& a) const { return static_cast<char*>(a.regions[r].base) + at / runs * a.regions[r].outer_stride; }
+    // bytes of the run that a slot holds
+    __device__ __forceinline__ int held(const ReorderArgs& a, const Components& k, int slot) const {
+        const MkbsRegion& g = a.regions[r];
+        return (int)max((int64_t)0, min((int64_t)k.run[c], min(k.length[slot], g.rows) * g.row_bytes - begin(a, k)));
+    }
+};
+
+// Everything a multiple of 16 bytes: one warp keeps bulk copies under way, a lane per slot.
+__global__ void __launch_bounds__(kReorderThreads, 1) reorder_bulk_kernel(const __grid_constant__ ReorderArgs a) {
+    extern __shared__ uint4 raw[];
+    __shared__ Components k;
+    __shared__ uint64_t bars[kStages];
+    k.find(a);
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    const uint32_t bar0 = mkb::smem_u32(bars), data = (mkb::smem_u32(raw) + 127u) & ~127u;
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mkb::mbar_init(bar0 + i * 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    Step load(a, k), store = load;
+    int issued = 0;
+    auto issue = [&]() {
+        const int st = issued % kStages, from = k.source_begin[load.c], to = k.source_begin[load.c + 1], run = k.run[load.c];
+        int bytes = 0;
+        for (int i = from + lane; i < to; i += 32) bytes += load.held(a, k, k.source[i]);
+        bytes = __reduce_add_sync(0xffffffffu, bytes);
+        if (lane == 0) mkb::mbar_expect_tx(bar0 + st * 8, bytes);
+        __syncwarp();
+        const char* const base = load.base(a) + load.begin(a, k);
+        for (int i = from + lane; i < to; i += 32) {
+            const int n = load.held(a, k, k.source[i]);
+            if (n > 0)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(data + st * kStageBytes + (i - from) * run),
+                             "l"(base + k.source[i] * a.regions[load.r].slot_stride), "r"(n), "r"(bar0 + st * 8)
+                             : "memory");
+        }
+        ++issued;
+        load.at += gridDim.x;
+    };
+    while (issued < kStages && load.settle(a, k)) issue();
+    for (int done = 0; store.settle(a, k); ++done, store.at += gridDim.x) {
+        const int st = done % kStages, source0 = k.source_begin[store.c], run = k.run[store.c];
+        unsigned long long began = 0;
+        bool there = true;
+        while (!mkb::mbar_try_wait(bar0 + st * 8, (uint32_t)(done / kStages) & 1u)) {  // (every lane reads what has arrived)
+            const unsigned long long now = mkb::globaltimer_ns();
+            if (began == 0) began = now;
+            if (now - began > 2000000000ull) {
+                there = false;
+                break;
+            }
+        }
+        if (!__all_sync(0xffffffffu, there)) break;
+        char* const base = store.base(a) + store.begin(a, k);
+        for (int i = k.target_begin[store.c] + lane; i < k.target_begin[store.c + 1]; i += 32) {
+            const int s = k.target[i], p = k.parent[s], n = store.held(a, k, p);
+            if (n > 0)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + s * a.regions[store.r].slot_stride),
+                             "r"(data + st * kStageBytes + (k.place[p] - source0) * run), "r"(n)
+                             : "memory");
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        if (done > 0 && load.settle(a, k)) {  // the stage before this one is free when its copies have been read
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            __syncwarp();
+            issue();
+        }
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// Any sizes and alignments.
 template <typename V>
 __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderArgs a) {
     extern __shared__ uint4 raw[];
@@ -77,124 +265,180 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 
 // ---- which rows stay ------------------------------------------------------------------------ //
 // A block per layer, sequence and head.  The weight of the last row that stays is found digit by digit (11, 11 and 10 bits
-// of its order) by counting; rows of that very weight stay in the order of their places.
-constexpr int kSelectThreads = 1024, kDigits = 2048;
+// of its order) by counting; rows of that very weight stay in the order of their places.  The weights are read from memory
+// once: their orders lie in shared memory, as far as they fit, for the passes that follow.  Then each warp has a run of rows:
+// it counts those that stay, and with the counts of the warps before it writes them.
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kDigits = 2048, kSelectAhead = 8;
+constexpr int kMostOrders = (227 * 1024 - kStaticShared) / 4;
 
-
-__device__ __forceinline__ int block_scan(int v, int* warps, int* total) {  // exclusive; kSelectThreads threads
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int sum = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int n = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += n;
-    }
-    if (lane == 31) warps[warp] = sum;
-    __syncthreads();
-    if (warp == 0) {
-        int w = warps[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int n = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += n;
-        }
-        warps[lane] = w;
-    }
-    __syncthreads();
-    *total = warps[31];
-    const int before = (warp ? warps[warp - 1] : 0) + sum - v;
-    __syncthreads();
-    return before;
-}
-
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const MkbsSelect s) {
-    __shared__ int count[kDigits], warps[32], found[2];
-    const int t = threadIdx.x, head = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(const MkbsSelect s, const int fit) {
+    extern __shared__ uint32_t orders[];
+    __shared__ int count[kDigits], sums[2][kSelectWarps], found[2];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, head = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
     const int n = length_of(s.lengths, s.length, s.positions, b), kept = min(n, s.keep);
     const int64_t at = layer * s.w_layer + b * s.w_sequence + head * s.w_head;
     const float* const w = s.weights + at;
-    float* const kept_w = s.kept != nullptr ? s.kept + at : nullptr;
     int32_t* const rows = s.rows + (((int64_t)layer * s.sequences + b) * s.kv_heads + head) * s.keep;
     for (int r = kept + t; r < s.keep; r += kSelectThreads) rows[r] = -1;
-    // not a number: the order of minus infinity
-    auto order = [&](int j) { return order_of(fmaxf(w[j], -INFINITY)); };
-    const int lo = n > s.keep ? s.sinks : n, hi = n > s.keep ? n - s.recent : n;  // rows that compete
-    int need = s.keep - s.sinks - s.recent;
+    if (n <= s.keep) {
+        for (int r = t; r < n; r += kSelectThreads) rows[r] = r;
+        float* const out = s.kept != nullptr ? s.kept + at : nullptr;
+        if (out != nullptr && out != w)
+            for (int r = t; r < n; r += kSelectThreads) out[r] = w[r];
+        return;
+    }
+    const int lo = s.sinks, hi = n - s.recent;  // rows that compete
+    int need = s.keep - s.sinks - s.recent;     // of them stay
+    // order_of, not a number as minus infinity
+    auto from_memory = [&](int j) { return order_of(fmaxf(w[j], -INFINITY)); };
+    // rows lo .. hi - 1 by `step`, some of whose loads are under way together
+    auto each = [&](int from, int to, int step, auto get, auto use) {
+        for (int j0 = from; j0 < to; j0 += kSelectAhead * step) {
+            uint32_t o[kSelectAhead];
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) o[u] = j0 + u * step < to ? get(j0 + u * step) : 0u;
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u)
+                if (j0 + u * step < to) use(j0 + u * step, o[u]);
+        }
+    };
+    auto order = [&](int j) { return j < fit ? orders[j] : from_memory(j); };
     uint32_t limit = 0;
     int shift = 32;
-    if (n > s.keep && need > 0) {
-        for (const int bits : {11, 11, 10}) {
-            shift -= bits;
-            for (int d = t; d < kDigits; d += kSelectThreads) count[d] = 0;
-            __syncthreads();
-            const uint32_t above = shift + bits == 32 ? 0 : limit >> (shift + bits);
-            for (int j = lo + t; j < hi; j += kSelectThreads) {
-                const uint32_t o = order(j);
-                if (shift + bits == 32 || o >> (shift + bits) == above) atomicAdd(&count[o >> shift & ((1 << bits) - 1)], 1);
-            }
-            __syncthreads();
-            // digits from the largest down: two per thread
-            const int d = kDigits - 1 - 2 * t, c0 = count[d], c1 = count[d - 1];
-            int total;
-            const int before = block_scan(c0 + c1, warps, &total);
-            if (before < need && need <= before + c0) found[0] = d, found[1] = before;
-            if (before + c0 < need && need <= before + c0 + c1) found[0] = d - 1, found[1] = before + c0;
-            __syncthreads();
+    for (const int bits : {11, 11, 10}) {
+        shift -= bits;
+        for (int d = t; d < kDigits; d += kSelectThreads) count[d] = 0;
+        __syncthreads();
+        if (shift + bits == 32) {
+            each(lo + t, hi, kSelectThreads, from_memory, [&](int j, uint32_t o) {
+                if (j < fit) orders[j] = o;
+                atomicAdd(&count[o >> shift], 1);
+            });
+        } else {
+            each(lo + t, hi, kSelectThreads, order, [&](int, uint32_t o) {
+                if (o >> (shift + bits) == limit >> (shift + bits)) atomicAdd(&count[o >> shift & ((1 << bits) - 1)], 1);
+            });
+        }
+        __syncthreads();
+        // digits from the largest down, two per thread: how many rows lie above a digit
+        const int d = kDigits - 1 - 2 * t, c0 = count[d], c1 = count[d - 1];
+        int before = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int m = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += m;
+        }
+        if (lane == 31) sums[0][warp] = before;
+        __syncthreads();
+        before -= c0 + c1;
+        for (int i = 0; i < warp; ++i) before += sums[0][i];
+        if (before < need && need <= before + c0) found[0] = d, found[1] = before;
+        if (before + c0 < need && need <= before + c0 + c1) found[0] = d - 1, found[1] = before + c0;
+        __syncthreads();
+        if (need > 0) {
             limit |= (uint32_t)found[0] << shift;
-            need -= found[1];  // of this weight's digits so far
-            __syncthreads();
+            need -= found[1];
         }
     }
-    // rows above the limit, and the first `need` rows at it
-    int out = 0, ties = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + t;
-        const bool there = j < n, competes = j >= lo && j < hi;
-        const float x = there ? w[j] : 0.f;
-        const uint32_t o = order_of(fmaxf(x, -INFINITY));
-        const bool tie = there && competes && o == limit;
-        int tied, total;
-        const int tie_rank = ties + block_scan(tie, warps, &tied);
-        const bool stays = there && (!competes || (need > 0 && (o > limit || (tie && tie_rank < need))));
-        const int to = out + block_scan(stays, warps, &total);  // (all of this step's weights have been read)
-        if (stays) {
-            rows[to] = j;
-            if (kept_w != nullptr) kept_w[to] = x;
-        }
-        out += total;
-        ties += tied;
+    // Rows above the limit stay, and the first `need` at it
+    const int run = (hi - lo + kSelectThreads - 1) / kSelectThreads * 32, from = lo + warp * run, to = min(from + run, hi);
+    const bool some = s.keep > s.sinks + s.recent;
+    int above = 0, ties = 0;
+    each(from + lane, to, 32, order, [&](int, uint32_t o) {
+        above += o > limit;
+        ties += o == limit;
+    });
+    above = __reduce_add_sync(0xffffffffu, above);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) sums[0][warp] = above, sums[1][warp] = ties;
+    __syncthreads();
+    int out = s.sinks, tied = 0;
+    for (int i = 0; i < warp; ++i) {
+        out += sums[0][i];
+        tied += sums[1][i];
+    }
+    out += min(tied, need);
+    for (int j0 = from; j0 < to && some; j0 += 32) {
+        const int j = j0 + lane;
+        const uint32_t o = j < to ? order(j) : 0u, less = (1u << lane) - 1;
+        const uint32_t tie = __ballot_sync(0xffffffffu, j < to && o == limit);
+        const bool stays = j < to && (o > limit || (o == limit && tied + __popc(tie & less) < need));
+        const uint32_t all = __ballot_sync(0xffffffffu, stays);
+        if (stays) rows[out + __popc(all & less)] = j;
+        out += __popc(all);
+        tied += __popc(tie);
+    }
+    for (int r = t; r < s.sinks; r += kSelectThreads) rows[r] = r;
+    for (int r = t; r < s.recent; r += kSelectThreads) rows[s.keep - s.recent + r] = hi + r;
+    if (s.kept == nullptr) return;
+    // In their order: weights to come lie behind those that have been written
+    float* const put = s.kept + at;
+    for (int r0 = 0; r0 < s.keep; r0 += kSelectThreads) {
+        const int r = r0 + t;
+        __syncthreads();
+        const float x = r < s.keep ? w[rows[r]] : 0.f;
+        __syncthreads();
+        if (r < s.keep) put[r] = x;
     }
 }
 
 // ---- rows that stay, to the front ------------------------------------------------------------ //
-// A block takes one head's rows of one cache in their order, some at a time: all of them are in registers before the first is
-// written, and later rows come from behind what has been written.
-constexpr int kMoveThreads = 256, kMoveAhead = 4;
+// A block takes one head's rows of one cache, or a part of their columns, in their order, some at a time: all of them have been
+// read before the first is written.  Later rows come from behind what is written, so the next ones are on their way meanwhile:
+// copies into shared memory, of which each thread writes what it has fetched itself.
+constexpr int kMoveThreads = 256, kMoveRows = 4, kMoveStages = 4, kMoveBytes = kMoveStages * kMoveRows * kMoveThreads * 16;
 
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const MkbsMove m) {
-    const int lanes = m.head_bytes / 16, head = blockIdx.x / 2, which = blockIdx.x & 1, b = blockIdx.y, layer = blockIdx.z;
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const MkbsMove m, const int parts) {
+    extern __shared__ uint4 fetched[];  // [stage][row][thread]
+    const int lanes = m.head_bytes / 16 / parts, part = blockIdx.x % parts, which = blockIdx.x / parts % 2, head = blockIdx.x / parts / 2;
+    const int b = blockIdx.y, layer = blockIdx.z;
     if (m.caches[which] == nullptr) return;
     const int n = length_of(m.lengths, m.length, m.positions, b), kept = min(n, m.keep);
     const int32_t* const rows = m.rows + (((int64_t)layer * m.sequences + b) * m.kv_heads + head) * m.keep;
-    const int per = kMoveThreads / lanes, mine = threadIdx.x / lanes, u = threadIdx.x - mine * lanes;
+    const int per = kMoveThreads / lanes, mine = threadIdx.x / lanes, u = threadIdx.x - mine * lanes, step = per * kMoveRows;
     const int64_t row_bytes = (int64_t)m.kv_heads * m.head_bytes;
-    char* const base = static_cast<char*>(m.caches[which]) + layer * m.c_layer + b * m.c_sequence + (int64_t)head * m.head_bytes + u * 16;
-    for (int r0 = 0; r0 < kept; r0 += per * kMoveAhead) {
-        uint4 x[kMoveAhead];
-        bool moves[kMoveAhead];
+    char* const base = static_cast<char*>(m.caches[which]) + layer * m.c_layer + b * m.c_sequence + (int64_t)head * m.head_bytes + (part * lanes + u) * 16;
+    int from[kMoveRows];  // where the rows of the step to be fetched next come from; -1: they stay
+    auto find = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < kMoveAhead; ++i) {
-            const int r = r0 + i * per + mine, from = mine < per && r < kept ? rows[r] : -1;
-            moves[i] = from >= 0 && from < n && from != r;
-            if (moves[i]) x[i] = *reinterpret_cast<const uint4*>(base + from * row_bytes);
+        for (int k = 0; k < kMoveRows; ++k) {
+            const int r = i * step + k * per + mine;
+            from[k] = mine < per && r < kept ? __ldg(rows + r) : -1;
+            if (from[k] >= n || from[k] == r) from[k] = -1;
         }
-        __syncthreads();
+    };
+    uint32_t moving = 0;  // four bits a step, the one fetched last lowest
+    auto fetch = [&](int i) {
+        moving <<= kMoveRows;
 #pragma unroll
-        for (int i = 0; i < kMoveAhead; ++i)
-            if (moves[i]) *reinterpret_cast<uint4*>(base + (r0 + i * per + mine) * row_bytes) = x[i];
-        __syncthreads();
+        for (int k = 0; k < kMoveRows; ++k) {
+            if (from[k] < 0) continue;
+            moving |= 1u << k;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mkb::smem_u32(fetched + (i % kMoveStages * kMoveRows + k) * kMoveThreads + threadIdx.x)),
+                         "l"(base + from[k] * row_bytes)
+                         : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    find(0);
+    for (int i = 0; i < kMoveStages - 1; ++i) {
+        fetch(i);
+        find(i + 1);
     }
+    for (int i = 0; i * step < kept; ++i) {
+        fetch(i + kMoveStages - 1);
+        find(i + kMoveStages);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMoveStages - 1) : "memory");
+        __syncthreads();  // everybody has fetched step i
+        const uint32_t moves = moving >> kMoveRows * (kMoveStages - 1);
+#pragma unroll
+        for (int k = 0; k < kMoveRows; ++k)
+            if (moves >> k & 1)
+                *reinterpret_cast<uint4*>(base + (int64_t)(i * step + k * per + mine) * row_bytes) = fetched[(i % kMoveStages * kMoveRows + k) * kMoveThreads + threadIdx.x];
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
+static_assert(kMoveRows * kMoveStages <= 32, "bits of `moving`");
 
 template <typename V>
 cudaError_t reorder(const ReorderArgs& a, cudaStream_t s) {
@@ -212,16 +456,25 @@ cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
         const MkbsRegion& g = a.regions[i] = r.regions[i];
         bits |= reinterpret_cast<uintptr_t>(g.base) | (uintptr_t)g.outer_stride | (uintptr_t)g.slot_stride | (uintptr_t)g.row_bytes;
     }
-    return bits % 16 == 0 ? reorder<uint4>(a, s) : bits % 4 == 0 ? reorder<uint32_t>(a, s) : reorder<uint8_t>(a, s);
+    if (bits % 16 != 0) return bits % 4 == 0 ? reorder<uint32_t>(a, s) : reorder<uint8_t>(a, s);
+    if (const cudaError_t e = allow_shared_memory<reorder_bulk_kernel>(); e != cudaSuccess) return e;
+    reorder_bulk_kernel<<<kSms, kReorderThreads, kStages * kStageBytes + 128, s>>>(a);
+    return cudaGetLastError();
 }
 
 cudaError_t select_launch(const MkbsSelect& a, cudaStream_t s) {
-    select_kernel<<<dim3(a.kv_heads, a.sequences, a.layers), kSelectThreads, 0, s>>>(a);
+    if (const cudaError_t e = allow_shared_memory<select_kernel>(); e != cudaSuccess) return e;
+    const int longest = a.lengths != nullptr ? a.positions : a.length, fit = longest <= a.keep ? 0 : longest < kMostOrders ? longest : kMostOrders;
+    select_kernel<<<dim3(a.kv_heads, a.sequences, a.layers), kSelectThreads, fit * 4, s>>>(a, fit);
     return cudaGetLastError();
 }
 
 cudaError_t move_launch(const MkbsMove& m, cudaStream_t s) {
-    move_kernel<<<dim3(2 * m.kv_heads, m.sequences, m.layers), kMoveThreads, 0, s>>>(m);
+    // Two blocks and more for every SM, none with less than 32 bytes of a row (a sector)
+    int parts = 1;
+    while (m.kv_heads * 2 * m.sequences * m.layers * parts < 2 * kSms && m.head_bytes % (64 * parts) == 0) parts *= 2;
+    if (const cudaError_t e = allow_shared_memory<move_kernel>(); e != cudaSuccess) return e;
+    move_kernel<<<dim3(2 * m.kv_heads * parts, m.sequences, m.layers), kMoveThreads, kMoveBytes, s>>>(m, parts);
     return cudaGetLastError();
 }
 
