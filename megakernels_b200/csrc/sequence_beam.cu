@@ -3,13 +3,16 @@
 // The score of continuation (b, v) is c_b + (l_bv - top_b) - log sum_v exp(l_bv - top_b); within a beam it grows with
 // the logit.  So the order of whole segments of a beam's vocabulary by their largest logit says which of them can hold
 // one of the k best: a segment behind k others has k better continuations before it.  That gives two launches:
-//   scan   reads every logit once: the maximum of every segment, and per warp the maximum and sum of exponentials of a
+//   scan   reads every logit once: the maximum of every segment, and per block the maximum and sum of exponentials of a
 //          run of segments;
 //   merge  a block per group: the log sums, the k best segments of all beams, and of their elements (still in L2)
 //          the k best.
-// Both selections are knock-outs: candidates fall into a few hundred groups by thread, the groups' best ones are ranked by
-// counting, the members of the k best groups go into the next round.  A candidate is a 64-bit key and its index, which are
-// never equal (what is no candidate has the key 0 and comes last), so every round is exact, ties included.
+// Both selections go through the candidates' scores in fp32 first: a lower bound of the k-th best is the k-th best of the maxima
+// over groups of threads, and what may lie above it is listed, mostly little more than k.  The listed ones' 64-bit scores are
+// ranked by counting.  Where the list is too short for what may lie above (equal logits, fewer than k finite scores), the selection is
+// a knock-out: candidates fall into groups by thread, the groups' best ones are ranked by counting, the members of the k best
+// groups go into the next round.  A candidate is a 64-bit key and its index, which are never equal (what is no candidate has the
+// key 0 and comes last), so both are exact, ties included.
 #include "hybrid_common.cuh"
 #include "sequence_kernels.h"
 
@@ -17,14 +20,14 @@ namespace mkbs {
 namespace {
 
 constexpr int kBlockElems = 256;  // elements that a warp reads at a time
-constexpr int kScanWarps = 8;
-constexpr int kMergeThreads = 1024;
+constexpr int kScanWarps = 8, kAhead = 4;  // (kAhead: blocks whose loads are under way together)
+constexpr int kMergeThreads = 512, kStaged = 8192, kListed = kMergeThreads;  // (kStaged: candidates whose logits lie in shared memory)
+constexpr int kCandidateBytes = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamPlan {
-    int rows, segment, segments, per_warp, parts;  // elements per segment; segments, segments per warp and warps of a row
-    int level1, level2;                            // candidates: all segments, the elements of k of them
-    int groups_ranked, list_a, list_b;             // groups per round, entries of the two lists
+    int rows, segment, segments, per_warp, parts;  // elements per segment; segments of a row and of a warp, blocks of a row
+    int groups, list_a, list_b, staged;            // of the merge: groups per round, entries of the two lists, logits in shared memory
     size_t part_offset, bytes;
     explicit BeamPlan(const MkbsBeams& b) {
         rows = b.groups * b.beams;
@@ -33,28 +36,27 @@ struct BeamPlan {
         for (segment = kBlockElems; (int64_t)b.beams * ((span + segment - 1) / segment) > 2 * (int64_t)b.k * segment; segment *= 2) {
         }
         segments = (int)((span + segment - 1) / segment);
-        // two blocks' worth of warps per SM before a warp takes a second segment
-        per_warp = (int)(((int64_t)rows * segments + kSms * 16 - 1) / (kSms * 16));
-        parts = (segments + per_warp - 1) / per_warp;
-        level1 = b.beams * segments;
-        level2 = (level1 < b.k ? level1 : b.k) * segment;
-        for (groups_ranked = 64; groups_ranked < 4 * b.k; groups_ranked *= 2) {
-        }
-        const int most = level1 > level2 ? level1 : level2;
-        list_a = next(most, b.k);
-        list_b = next(list_a, b.k);
+        // four blocks and more per SM before a warp takes a second segment
+        per_warp = (int)(((int64_t)rows * segments + 4 * kSms * kScanWarps - 1) / (4 * kSms * kScanWarps));
+        parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps);
+        groups = b.k <= 32 ? 128 : kMergeThreads;
+        // candidates: all segments, then the elements of k of them
+        const int level1 = b.beams * segments, level2 = (level1 < b.k ? level1 : b.k) * segment, most = level1 > level2 ? level1 : level2;
+        list_a = next(most, b.k) < kListed ? kListed : (next(most, b.k) + 3) / 4 * 4;  // (16-byte numbers follow)
+        list_b = (next(list_a, b.k) + 3) / 4 * 4;
+        staged = most < kStaged ? most : kStaged;
         part_offset = ((size_t)rows * segments * 4 + 255) / 256 * 256;
         bytes = part_offset + (size_t)rows * parts * 8;
     }
     int next(int m, int k) const {  // entries of the next round
-        if (m <= groups_ranked) return 0;
-        return k * (m <= kMergeThreads ? (m + groups_ranked - 1) / groups_ranked : (m + kMergeThreads - 1) / kMergeThreads * (kMergeThreads / groups_ranked));
+        if (m <= groups) return 0;
+        return k * (m <= kMergeThreads ? (m + groups - 1) / groups : (m + kMergeThreads - 1) / kMergeThreads * (kMergeThreads / groups));
     }
-    size_t merge_smem() const { return (size_t)(list_a + list_b + groups_ranked) * 12 + (size_t)groups_ranked * 4 + MKBS_MAX_BEST * 4 + MKBS_MAX_BEAMS * 24 + 16; }
+    size_t merge_smem() const { return (size_t)(list_a + list_b + groups) * kCandidateBytes + (size_t)(groups + staged) * 4 + MKBS_MAX_BEST * 8 + MKBS_MAX_BEAMS * 28; }
 };
 
 struct BeamArgs {
-    int beams, vocab, k, segment, segments, per_warp, parts, groups_ranked, list_a, list_b;
+    int beams, vocab, k, segment, segments, per_warp, parts, groups, list_a, list_b, staged;
     int64_t row_stride;
     const void* logits;
     const float* scores;
@@ -73,17 +75,50 @@ __device__ __forceinline__ int shift_of(const T* row) { return (int)((reinterpre
 
 __device__ __forceinline__ bool is_live(float c) { return c > -INFINITY && c < INFINITY; }
 
-// The lane's elements of a block: a lane holds 8 bf16 or twice 4 floats next to each other.  Not a number and what lies
-// outside the row is minus infinity.
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16 bytes of a row from element `at` on; what lies outside the row is minus infinity.  (Out of line: a launch fetches its code
+// anew, and few vectors lie at a row's ends.)
 template <typename T>
-__device__ __forceinline__ void load_elems(const T* base, int p, int shift, int end, float (&x)[8]) {
-    constexpr int n = 16 / sizeof(T);
+__device__ __noinline__ uint4 edge_vector(const T* base, int at, int shift, int end) {
+    uint32_t words[4];
 #pragma unroll
-    for (int v = 0; v < 8 / n; ++v) {
-        const int at = p + v * kBlockElems / 2;
-        if (at >= shift && at + n <= end) {
-            const uint4 w = mkb::ld_nc_v4(base + at);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            words[i] = at + i >= shift && at + i < end ? __float_as_uint(base[at + i]) : 0xff800000u;
+        } else {
+            const uint16_t* const bits = reinterpret_cast<const uint16_t*>(base);
+            const int k = at + 2 * i;
+            const uint32_t low = k >= shift && k < end ? bits[k] : 0xff80u, high = k + 1 >= shift && k + 1 < end ? bits[k + 1] : 0xff80u;
+            words[i] = low | high << 16;
+        }
+    }
+    return make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+// The lane's elements of a block: a lane holds 8 bf16 or twice 4 floats next to each other.
+template <typename T>
+struct Elems {
+    static constexpr int kVector = 16 / sizeof(T), kVectors = 8 / kVector;
+    uint4 w[kVectors];
+    __device__ __forceinline__ void load(const T* base, int block, int lane, int shift, int end) {
+        const int p = block * kBlockElems + lane * kVector;
+        const bool inside = block * kBlockElems >= shift && (block + 1) * kBlockElems <= end;  // (for the whole warp)
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int at = p + v * kBlockElems / 2;
+            w[v] = inside ? mkb::ld_nc_v4(base + at) : edge_vector(base, at, shift, end);
+        }
+    }
+    // as floats; not a number is minus infinity
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const uint32_t words[4] = {w[v].x, w[v].y, w[v].z, w[v].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (sizeof(T) == 2) {
@@ -93,37 +128,43 @@ __device__ __forceinline__ void load_elems(const T* base, int p, int shift, int 
                     x[4 * v + i] = __uint_as_float(words[i]);
                 }
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < n; ++i) x[n * v + i] = at + i >= shift && at + i < end ? mkbh::to_f<T>(base[at + i]) : -INFINITY;
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], -INFINITY);
-}
+        for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], -INFINITY);
+    }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamArgs a) {
+    __shared__ float2 shared[kScanWarps];
     mkbh::let_next();
-    constexpr int kAhead = 4;  // blocks whose loads are under way together
-    const int lane = threadIdx.x & 31, row = blockIdx.y, part = blockIdx.x * kScanWarps + (threadIdx.x >> 5);
-    if (part >= a.parts) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
     // beams whose continuations' scores do not depend on their logits
     if ((a.done != nullptr && a.done[row]) || (a.scores != nullptr && !is_live(a.scores[row]))) return;
     const T* const begin = static_cast<const T*>(a.logits) + row * a.row_stride;
     const int shift = shift_of(begin), end = shift + a.vocab, blocks = a.segment / kBlockElems;
     const T* const base = begin - shift;
-    const int first = part * a.per_warp * blocks, last = min(first + a.per_warp * blocks, a.segments * blocks);
-    constexpr int n = 16 / sizeof(T);
+    const int first = (blockIdx.x * kScanWarps + warp) * a.per_warp * blocks, last = min(first + a.per_warp * blocks, a.segments * blocks);
     float top = -INFINITY, sum = 0.f, best = -INFINITY;
+    Elems<T> ahead[kAhead];
+    auto load = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (at + u < last) ahead[u].load(base, at + u, lane, shift, end);
+    };
+    load(first);
     for (int at = first; at < last; at += kAhead) {
-        float x[kAhead][8], high[kAhead];
+        float x[kAhead][8], high[kAhead], most = top;
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int p = at + u < last ? (at + u) * kBlockElems + lane * n : end;
-            load_elems(base, p, shift, end, x[u]);
+            if (at + u < last) {
+                ahead[u].floats(x[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u][i] = -INFINITY;
+            }
         }
-        float most = top;
+        load(at + kAhead);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             high[u] = x[u][0];
@@ -138,12 +179,12 @@ __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamAr
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum += x[u][i] == INFINITY ? 1.f : 0.f;
         } else if (most > -INFINITY) {
-            sum *= exp2f((top - most) * kLog2e);  // (0 from minus infinity)
+            sum *= fast_exp2((top - most) * kLog2e);  // (0 from minus infinity)
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 float part_sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) part_sum += exp2f((x[u][i] - most) * kLog2e);
+                for (int i = 0; i < 8; ++i) part_sum += fast_exp2((x[u][i] - most) * kLog2e);
                 sum += part_sum;
             }
         }
@@ -159,10 +200,20 @@ __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamAr
             }
         }
     }
+    // the lanes' and the warps' sums; a part without a finite logit has the sum 0
+    auto scaled = [](float2 part, float most) { return part.x == most ? part.y : part.x > -INFINITY ? part.y * fast_exp2((part.x - most) * kLog2e) : 0.f; };
     const float most = value_of(__reduce_max_sync(0xffffffffu, order_of(top)));
-    const float factor = top == most ? 1.f : exp2f((top - most) * kLog2e);
-    sum = mkbh::warp_sum(top > -INFINITY ? sum * factor : 0.f);
-    if (lane == 0) a.sums[(size_t)row * a.parts + part] = make_float2(most, sum);
+    sum = mkbh::warp_sum(scaled(make_float2(top, sum), most));
+    if (lane == 0) shared[warp] = make_float2(most, sum);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float high = shared[0].x, all = 0.f;
+#pragma unroll
+        for (int i = 1; i < kScanWarps; ++i) high = fmaxf(high, shared[i].x);
+#pragma unroll
+        for (int i = 0; i < kScanWarps; ++i) all += scaled(shared[i], high);
+        a.sums[(size_t)row * a.parts + blockIdx.x] = make_float2(high, all);
+    }
 }
 
 __device__ __forceinline__ uint64_t order64(double x) {
@@ -180,153 +231,278 @@ struct Candidate {
 struct MergeSmem {
     uint64_t *key_a, *key_b, *group_key;
     double *log_sum, *start;
-    uint32_t *at_a, *at_b, *group_at;
-    int *rank, *chosen;
-    float* top;
-    __device__ MergeSmem(void* raw, int list_a, int list_b, int groups) {
+    uint32_t *at_a, *at_b, *group_at, *staged;
+    int *rank, *chosen_beam, *chosen_segment, *kind;
+    float *top, *offset;
+    __device__ MergeSmem(void* raw, const BeamArgs& a) {
         key_a = static_cast<uint64_t*>(raw);
-        key_b = key_a + list_a;
-        group_key = key_b + list_b;
-        log_sum = reinterpret_cast<double*>(group_key + groups);
+        key_b = key_a + a.list_a;
+        group_key = key_b + a.list_b;
+        log_sum = reinterpret_cast<double*>(group_key + a.groups);
         start = log_sum + MKBS_MAX_BEAMS;
         at_a = reinterpret_cast<uint32_t*>(start + MKBS_MAX_BEAMS);
-        at_b = at_a + list_a;
-        group_at = at_b + list_b;
-        rank = reinterpret_cast<int*>(group_at + groups);
-        chosen = rank + groups;
-        top = reinterpret_cast<float*>(chosen + MKBS_MAX_BEST);
+        at_b = at_a + a.list_a;
+        group_at = at_b + a.list_b;
+        rank = reinterpret_cast<int*>(group_at + a.groups);
+        chosen_beam = rank + a.groups;
+        chosen_segment = chosen_beam + MKBS_MAX_BEST;
+        kind = chosen_segment + MKBS_MAX_BEST;
+        top = reinterpret_cast<float*>(kind + MKBS_MAX_BEAMS);
+        offset = top + MKBS_MAX_BEAMS;
+        staged = reinterpret_cast<uint32_t*>(offset + MKBS_MAX_BEAMS);
     }
 };
 
-// The k first of candidates 0 .. count - 1; `take(rank, candidate)` is called for each of them by some thread.
-template <typename Get, typename Take>
-__device__ __forceinline__ void knock_out(const MergeSmem& sm, int count, int k, int groups, Get get, Take take) {
-    const int t = threadIdx.x, lanes = kMergeThreads / groups, group = t / lanes;
-    auto rank_groups = [&]() {  // (group_key, group_at) -> rank
-        for (int g = t; g < groups; g += kMergeThreads) sm.rank[g] = 0;
-        __syncthreads();
-        const int mine = t % groups, share = groups / lanes, from = t / groups * share;
-        const Candidate own{sm.group_key[mine], sm.group_at[mine]};
-        int before = 0;
-#pragma unroll 4
-        for (int j = from; j < from + share; ++j) before += Candidate{sm.group_key[j], sm.group_at[j]}.before(own);
-        if (before) atomicAdd(&sm.rank[mine], before);
-        __syncthreads();
-    };
-    bool in_a = false, listed = false;
-    auto candidate = [&](int i) {
-        if (!listed) return get(i);
-        return in_a ? Candidate{sm.key_a[i], sm.at_a[i]} : Candidate{sm.key_b[i], sm.at_b[i]};
-    };
-    while (count > groups) {
-        // Candidates of a thread: t, t + 1024, ...; of few candidates one that leaves no group empty
-        const bool few = count <= kMergeThreads;
-        const int turns = few ? 1 : (count + kMergeThreads - 1) / kMergeThreads, members = few ? (count + groups - 1) / groups : turns * lanes;
-        const int first = few ? t % lanes * groups + group : t;
-        Candidate best{0, 0x80000000u};
-        for (int i = first; i < count; i += kMergeThreads) {
-            const Candidate c = candidate(i);
-            if (c.before(best)) best = c;
-        }
-        for (int o = lanes / 2; o; o >>= 1) {
-            const Candidate c{__shfl_xor_sync(0xffffffffu, best.key, o), __shfl_xor_sync(0xffffffffu, best.at, o)};
-            if (c.before(best)) best = c;
-        }
-        if (t % lanes == 0) sm.group_key[group] = best.key, sm.group_at[group] = best.key ? best.at : 0x80000000u + group;
-        __syncthreads();
-        rank_groups();
-        const int place = sm.rank[group];
-        uint64_t* const key = in_a ? sm.key_b : sm.key_a;
-        uint32_t* const at = in_a ? sm.at_b : sm.at_a;
-        if (place < k) {
-            for (int n = 0; n < turns; ++n) {
-                const int i = first + n * kMergeThreads, member = n * lanes + t % lanes;
-                if (member >= members) continue;
-                const Candidate c = i < count ? candidate(i) : Candidate{0, 0};
-                key[place * members + member] = c.key;
-                at[place * members + member] = c.at;
-            }
-        }
-        count = k * members;
-        in_a = !in_a;
-        listed = true;
-        __syncthreads();
-    }
-    if (t < groups) {
-        const Candidate c = t < count ? candidate(t) : Candidate{0, 0x80000000u + t};
-        sm.group_key[t] = c.key;
-        sm.group_at[t] = c.key ? c.at : 0x80000000u + t;  // (what is none is behind all others, and no two alike)
-    }
-    __syncthreads();
-    rank_groups();
-    if (t < groups && sm.rank[t] < k) take(sm.rank[t], Candidate{sm.group_key[t], sm.group_at[t]});
-    __syncthreads();
-}
-
 enum Kind { kLive = 0, kDone = 1, kDead = 2 };  // kDead: every continuation has score minus infinity
 
+// Segments, then elements, go through the same code, loops are hardly unrolled, and there are not more threads than there is work
+// for: a block runs through this once, fetching and issuing instructions is what takes the time.
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArgs a) {
-    extern __shared__ uint64_t raw[];
-    const MergeSmem sm(raw, a.list_a, a.list_b, a.groups_ranked);
-    __shared__ int kind[MKBS_MAX_BEAMS];
-    const int group = blockIdx.x, row0 = group * a.beams, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    mkbh::after_previous();
-    for (int b = warp; b < a.beams; b += kMergeThreads / 32) {
-        const int row = row0 + b;
-        const float c = a.scores != nullptr ? a.scores[row] : 0.f;
-        int what = !is_live(c) ? kDead : a.done != nullptr && a.done[row] ? kDone : kLive;
-        if (what == kLive) {
-            const float2* const sums = a.sums + (size_t)row * a.parts;
-            float top = -INFINITY;
-            for (int i = lane; i < a.parts; i += 32) top = fmaxf(top, sums[i].x);
-            top = mkbh::warp_max(top);
-            double sum = 0.0;
-            for (int i = lane; i < a.parts; i += 32) {
-                const float2 part = sums[i];
-                if (part.x == top) sum += part.y;
-                else if (part.x > -INFINITY) sum += part.y * exp((double)part.x - (double)top);
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (top == -INFINITY) what = kDead;
-            if (lane == 0) sm.top[b] = top, sm.log_sum[b] = log(sum);
-        }
-        if (lane == 0) kind[b] = what, sm.start[b] = c;
-    }
-    __syncthreads();
+    extern __shared__ __align__(16) uint64_t raw[];
+    const MergeSmem sm(raw, a);
+    __shared__ int listed;
+    __shared__ uint32_t bound;
+    const int t = threadIdx.x, group_of = blockIdx.x, row0 = group_of * a.beams, warp = t >> 5, lane = t & 31;
+    const int segments = a.segments, groups = a.groups, k = a.k, shift_segment = __ffs(a.segment) - 1;
+    constexpr int threads = kMergeThreads;
+    const int lanes = threads / groups, group = t / lanes;
+    const float per_segments = 1.f / segments;  // (exact quotients: candidates are fewer than 2^17)
+    const uint32_t* const tops = a.tops + (size_t)row0 * segments;
     const uint64_t lowest = order64(-(double)INFINITY);
-    auto key_of = [&](int b, float x) {
-        const double d = x == sm.top[b] ? 0.0 : (double)x - (double)sm.top[b];
-        return x == -INFINITY ? lowest : order64(sm.start[b] + (d - sm.log_sum[b]));
-    };
     auto row_of = [&](int b) { return static_cast<const T*>(a.logits) + (row0 + b) * a.row_stride; };
-    const int segments = a.segments, count = a.beams * segments;
-    knock_out(sm, count, a.k, a.groups_ranked, [&](int i) {
-        const int b = i / segments, s = i - b * segments, shift = shift_of(row_of(b));
-        if (s * a.segment >= shift + a.vocab) return Candidate{0, (uint32_t)i};
-        if (kind[b] == kLive) return Candidate{key_of(b, value_of(a.tops[(size_t)(row0 + b) * segments + s])), (uint32_t)i};
-        const bool ends = kind[b] == kDone && (a.eos + shift) / a.segment == s;
-        return Candidate{ends ? order64(sm.start[b]) : lowest, (uint32_t)i};
-    }, [&](int rank, const Candidate& c) { sm.chosen[rank] = c.key ? (int)c.at : -1; });
-    const int chosen = min(a.k, count);
-    knock_out(sm, chosen * a.segment, a.k, a.groups_ranked, [&](int i) {
-        const int at = sm.chosen[i / a.segment];
-        if (at < 0) return Candidate{0, 0};
-        const int b = at / segments, s = at - b * segments;
-        const T* const row = row_of(b);
-        const int v = s * a.segment + i % a.segment - shift_of(row);
-        if (v < 0 || v >= a.vocab) return Candidate{0, 0};
-        const uint32_t flat = (uint32_t)b * a.vocab + v;
-        if (kind[b] == kLive) return Candidate{key_of(b, fmaxf(mkbh::to_f<T>(row[v]), -INFINITY)), flat};
-        return Candidate{kind[b] == kDone && v == a.eos ? order64(sm.start[b]) : lowest, flat};
-    }, [&](int rank, const Candidate& c) {
-        const int b = c.at / a.vocab, v = c.at - b * a.vocab, to = group * a.k + rank;
-        a.out_scores[to] = (float)value64(c.key);
-        a.out_parents[to] = row0 + b;
-        a.out_tokens[to] = v;
-        if (a.out_done != nullptr) a.out_done[to] = v == a.eos || (a.done != nullptr && a.done[row0 + b]);
-    });
+    auto beam_of = [&](int i) { return (int)((i + 0.5f) * per_segments); };
+    mkbh::after_previous();
+    int chosen = 0, infinite = 0;  // (infinite: some logit is; the bounds below hold for finite ones)
+#pragma unroll 1
+    for (int stage = 0; stage < 2; ++stage) {
+        int count = stage == 0 ? a.beams * segments : chosen << shift_segment;
+        // element i: of which beam, and where in its row; -1: none
+        auto place = [&](int i, int& v) {
+            const int b = sm.chosen_beam[i >> shift_segment];
+            if (b < 0) return -1;
+            v = (sm.chosen_segment[i >> shift_segment] << shift_segment) + (i & (a.segment - 1)) - shift_of(row_of(b));
+            return v >= 0 && v < a.vocab ? b : -1;
+        };
+        // a segment's largest logit, or an element, as order_of; 0: there is none (not set for a beam that has none, or has ended)
+        auto fetch = [&](int i) {
+            if (stage == 0) return tops[i];
+            int v = 0;
+            const int b = place(i, v);
+            return b >= 0 && sm.kind[b] == kLive ? order_of(fmaxf(mkbh::to_f<T>(row_of(b)[v]), -INFINITY)) : 0u;
+        };
+        const bool staged = count <= a.staged;
+        if (staged) {
+#pragma unroll 4
+            for (int i = t; i < count; i += threads) sm.staged[i] = fetch(i);
+        }
+        if (stage == 0) {
+#pragma unroll 1
+            for (int b = warp; b < a.beams; b += threads / 32) {  // the beams' sums
+                const int row = row0 + b;
+                const float c = a.scores != nullptr ? a.scores[row] : 0.f;
+                const float2* const sums = a.sums + (size_t)row * a.parts;
+                int what = !is_live(c) ? kDead : a.done != nullptr && a.done[row] ? kDone : kLive;
+                float top = -INFINITY;
+                double sum = 0.0;
+                if (what == kLive) {
+                    for (int i = lane; i < a.parts; i += 32) top = fmaxf(top, sums[i].x);
+                    top = mkbh::warp_max(top);
+                    for (int i = lane; i < a.parts; i += 32) {
+                        const float2 part = sums[i];
+                        sum += part.x == top ? part.y : part.x > -INFINITY ? part.y * fast_exp2((part.x - top) * kLog2e) : 0.f;
+                    }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (top == -INFINITY) what = kDead;
+                    infinite |= top == INFINITY;
+                }
+                if (lane == 0) {
+                    const double log_sum = log(sum);
+                    sm.kind[b] = what;
+                    sm.start[b] = c;
+                    sm.top[b] = top;
+                    sm.log_sum[b] = log_sum;
+                    sm.offset[b] = what == kLive ? (float)((double)c - (double)top - log_sum) : -INFINITY;
+                }
+            }
+        }
+        if (t == 0) listed = 0;
+        infinite = __syncthreads_or(infinite);
+        auto candidate = [&](int i) {
+            const uint32_t order = staged ? sm.staged[i] : fetch(i);
+            int b, v = 0;
+            bool there, ends;
+            uint32_t at = i;
+            if (stage == 0) {
+                b = beam_of(i);
+                const int s = i - b * segments, shift = shift_of(row_of(b));
+                there = (s << shift_segment) < shift + a.vocab;
+                ends = (a.eos + shift) >> shift_segment == s;
+            } else {
+                b = place(i, v);
+                there = b >= 0;
+                b = max(b, 0);
+                ends = v == a.eos;
+                at = (uint32_t)b * a.vocab + v;
+            }
+            if (!there) return Candidate{0, at};
+            uint64_t key = lowest;
+            if (sm.kind[b] == kLive) {
+                const float x = value_of(order), top = sm.top[b];
+                if (x > -INFINITY) key = order64(sm.start[b] + ((x == top ? 0.0 : (double)x - (double)top) - sm.log_sum[b]));
+            } else if (sm.kind[b] == kDone && ends) {
+                key = order64(sm.start[b]);
+            }
+            return Candidate{key, at};
+        };
+        auto take = [&](int rank, const Candidate& c) {
+            if (stage == 0) {
+                const int b = c.key ? beam_of(c.at) : -1;
+                sm.chosen_beam[rank] = b;
+                sm.chosen_segment[rank] = c.at - b * segments;
+            } else {
+                const int b = c.at / a.vocab, v = c.at - b * a.vocab, to = group_of * k + rank;
+                a.out_scores[to] = (float)value64(c.key);
+                a.out_parents[to] = row0 + b;
+                a.out_tokens[to] = v;
+                if (a.out_done != nullptr) a.out_done[to] = v == a.eos || (a.done != nullptr && a.done[row0 + b]);
+            }
+        };
+        // A score in fp32, and by how much it may be off
+        auto score = [&](int i, float& off) {
+            const int b = stage == 0 ? beam_of(i) : max(sm.chosen_beam[i >> shift_segment], 0);
+            const uint32_t order = staged ? sm.staged[i] : fetch(i);
+            const float x = order ? value_of(order) : -INFINITY, y = sm.offset[b];
+            off = (fabsf(x) + fabsf(y)) * 0x1p-21f;  // (infinite with the score; then the bounds are not numbers, and pass no comparison)
+            return x + y;
+        };
+        float best_score = -INFINITY;
+#pragma unroll 2
+        for (int i = t; i < count; i += threads) {
+            float off;
+            const float x = score(i, off);
+            best_score = fmaxf(best_score, x - off);
+        }
+        for (int o = lanes / 2; o; o >>= 1) best_score = fmaxf(best_score, __shfl_xor_sync(0xffffffffu, best_score, o));
+        if (t % lanes == 0) {
+            sm.group_at[group] = order_of(best_score);
+            sm.rank[group] = 0;
+        }
+        __syncthreads();
+        // ranks of the groups' maxima: a thread compares one of them with a share of the others
+        const int mine = t % groups, share = groups / lanes, first = t / groups * share;
+        {
+            const uint32_t own = sm.group_at[mine];
+            int before = 0;
+#pragma unroll 4
+            for (int j = first; j < first + share; j += 4) {
+                const uint4 o = *reinterpret_cast<const uint4*>(sm.group_at + j);
+                before += (o.x > own || (o.x == own && j < mine)) + (o.y > own || (o.y == own && j + 1 < mine)) + (o.z > own || (o.z == own && j + 2 < mine)) +
+                          (o.w > own || (o.w == own && j + 3 < mine));
+            }
+            if (before) atomicAdd(&sm.rank[mine], before);
+        }
+        __syncthreads();
+        if (t % lanes == 0 && sm.rank[group] == k - 1) bound = order_of(best_score);
+        __syncthreads();
+        const float least = value_of(bound);
+        auto list = [&](int i) {
+            const int n = atomicAdd(&listed, 1);
+            if (n < kListed) sm.at_a[n] = i;
+        };
+        if (least > -INFINITY && !infinite) {
+#pragma unroll 2
+            for (int i = t; i < count; i += threads) {
+                float off;
+                const float x = score(i, off);
+                if (x + off >= least) list(i);
+            }
+            // beams that have ended: their one continuation
+            if (a.done != nullptr && t < (stage == 0 ? a.beams : chosen)) {
+                const int b = stage == 0 ? t : sm.chosen_beam[t];
+                if (b >= 0 && sm.kind[b] == kDone) {
+                    const int at = a.eos + shift_of(row_of(b)), s = at >> shift_segment;
+                    if (stage == 0) list(b * segments + s);
+                    else if (s == sm.chosen_segment[t]) list((t << shift_segment) + (at & (a.segment - 1)));
+                }
+            }
+        }
+        __syncthreads();
+        const int some = listed;
+        if (some >= k && some <= kListed) {
+            Candidate own{0, 0};
+            if (t < some) own = candidate(sm.at_a[t]);
+            __syncthreads();
+            sm.key_a[t] = own.key;
+            sm.at_a[t] = own.at;
+            __syncthreads();
+            if (t < some) {
+                int rank = 0;
+#pragma unroll 4
+                for (int j = 0; j < some; ++j) rank += Candidate{sm.key_a[j], sm.at_a[j]}.before(own);
+                if (rank < k) take(rank, own);
+            }
+        } else {
+            // Rounds: into groups by thread, the groups' best ranked, the members of the first k into a list
+            int from_list = 0;  // 0: candidate(i), 1: list a, 2: list b
+            auto get = [&](int i) {
+                if (from_list == 0) return candidate(i);
+                return from_list == 1 ? Candidate{sm.key_a[i], sm.at_a[i]} : Candidate{sm.key_b[i], sm.at_b[i]};
+            };
+#pragma unroll 1
+            for (bool last = false;;) {
+                last = count <= groups;
+                // Candidates of a thread: t, t + threads, ...; of few candidates one that leaves no group empty; in the end a group is a candidate
+                const bool few = count <= threads;
+                const int turns = few ? 1 : (count + threads - 1) / threads, members = few ? (count + groups - 1) / groups : turns * lanes;
+                const int from = last ? (t % lanes ? count : group) : few ? t % lanes * groups + group : t;
+                Candidate best{0, 0};
+#pragma unroll 1
+                for (int i = from; i < count; i += threads) {
+                    const Candidate c = get(i);
+                    if (c.before(best)) best = c;
+                }
+                for (int o = lanes / 2; o; o >>= 1) {
+                    const Candidate c{__shfl_xor_sync(0xffffffffu, best.key, o), __shfl_xor_sync(0xffffffffu, best.at, o)};
+                    if (c.before(best)) best = c;
+                }
+                if (t % lanes == 0) {
+                    sm.group_key[group] = best.key;
+                    sm.group_at[group] = best.key ? best.at : 0x80000000u + group;  // (what is none is behind all others, and no two alike)
+                    sm.rank[group] = 0;
+                }
+                __syncthreads();
+                const Candidate own{sm.group_key[mine], sm.group_at[mine]};
+                int before = 0;
+                for (int j = first; j < first + share; ++j) before += Candidate{sm.group_key[j], sm.group_at[j]}.before(own);
+                if (before) atomicAdd(&sm.rank[mine], before);
+                __syncthreads();
+                const int rank = sm.rank[group];
+                if (last) {
+                    if (t % lanes == 0 && rank < k) take(rank, best);
+                    break;
+                }
+                uint64_t* const key = from_list == 1 ? sm.key_b : sm.key_a;
+                uint32_t* const at = from_list == 1 ? sm.at_b : sm.at_a;
+                if (rank < k) {
+#pragma unroll 1
+                    for (int n = 0; n < turns; ++n) {
+                        const int i = from + n * threads, member = n * lanes + t % lanes;
+                        if (member >= members) continue;
+                        const Candidate c = i < count ? get(i) : Candidate{0, 0};
+                        key[rank * members + member] = c.key;
+                        at[rank * members + member] = c.at;
+                    }
+                }
+                count = k * members;
+                from_list = from_list == 1 ? 2 : 1;
+                __syncthreads();
+            }
+        }
+        chosen = min(k, a.beams * segments);
+        __syncthreads();
+    }
 }
 
 template <typename T>
@@ -336,7 +512,7 @@ cudaError_t launch(const BeamPlan& p, const MkbsBeams& b, const BeamArgs& a, cud
         const cudaError_t e = allow_shared_memory<beam_merge_kernel<T>>();
         if (e != cudaSuccess) return e;
     }
-    beam_scan_kernel<T><<<dim3((p.parts + kScanWarps - 1) / kScanWarps, p.rows), 32 * kScanWarps, 0, s>>>(a);
+    beam_scan_kernel<T><<<dim3(p.parts, p.rows), 32 * kScanWarps, 0, s>>>(a);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(b.groups);
@@ -356,7 +532,7 @@ size_t beam_bytes(const MkbsBeams& b) { return BeamPlan(b).bytes; }
 cudaError_t beam_launch(const MkbsBeams& b, cudaStream_t s) {
     const BeamPlan p(b);
     char* const work = static_cast<char*>(b.workspace);
-    const BeamArgs a{b.beams, b.vocab, b.k, p.segment, p.segments, p.per_warp, p.parts, p.groups_ranked, p.list_a, p.list_b, b.row_stride, b.logits, b.scores,
+    const BeamArgs a{b.beams, b.vocab, b.k, p.segment, p.segments, p.per_warp, p.parts, p.groups, p.list_a, p.list_b, p.staged, b.row_stride, b.logits, b.scores,
                      b.done, b.eos, reinterpret_cast<uint32_t*>(work), reinterpret_cast<float2*>(work + p.part_offset), b.out_scores, b.out_parents,
                      b.out_tokens, b.out_done};
     return b.dtype == MKBS_F32 ? launch<float>(p, b, a, s) : launch<bf16>(p, b, a, s);

@@ -10,7 +10,7 @@ namespace {
 // memory, each source once however many take it, and writes it when all of it is there.  Runs do not overlap, so no slot loses
 // what another still needs.  Slots that depend on each other are the components of the graph of parents (a beam search's
 // groups): the fewer sources a run has, the longer its copies are.
-constexpr int kReorderThreads = 256, kReorderBytes = 96 * 1024;  // (bytes: of the plain kernel)
+constexpr int kReorderThreads = MKBS_MAX_SLOTS, kReorderBytes = 96 * 1024;  // (bytes: of the plain kernel)
 constexpr int kStages = 4, kStageBytes = 52 * 1024, kShortRun = 2048;
 
 struct ReorderArgs {
@@ -28,10 +28,9 @@ struct Components {
 
     __device__ __forceinline__ bool moves(int s, int first) const { return parent[s] != s && length[parent[s]] > first; }
 
-    // By all threads of a block of kReorderThreads.
+    // By all threads of a block, of which there is one per slot.
     __device__ void find(const ReorderArgs& a) {
         const int s = threadIdx.x, n = a.slots;
-        static_assert(kReorderThreads == MKBS_MAX_SLOTS, "a thread per slot");
         if (s < n) {
             const int p = a.parents[s];
             parent[s] = p >= 0 && p < n ? p : s;
@@ -98,9 +97,10 @@ struct Components {
         }
         __syncthreads();
         if (s < count) {
-            // four steps and more for every block, as far as copies do not get short
+            // two steps and more for every block, as far as copies do not get short (a step costs the warp nearly a microsecond: six states
+            // of 5 MB with 1, 2, 3, 4, 8 steps 14.9, 14.9, 15.9, 16.0, 20.5 us)
             const int sources_here = source_begin[s + 1] - source_begin[s], longest_run = kStageBytes / sources_here / 128 * 128;
-            const int64_t share = (int64_t)(bytes / (4 * kSms) / sources_here + 127) / 128 * 128;
+            const int64_t share = (int64_t)(bytes / (2 * kSms) / sources_here + 127) / 128 * 128;
             run[s] = (int)min((int64_t)longest_run, max((int64_t)kShortRun, share));
         }
         __syncthreads();
@@ -110,11 +110,13 @@ struct Components {
 // A step: one run of the bytes of a component's slots, in one layer of one region.
 struct Step {
     int c, r;
-    int64_t at, runs;  // step of this component and region, and how many runs a layer has there
+    int at, runs;   // step of this component and region, and how many runs a layer has there (memory ends before 2^31 runs)
+    int64_t begin;  // of the run, from a slot's first byte on
+    char* base;     // of the run in slot 0
     __device__ __forceinline__ void count(const ReorderArgs& a, const Components& k) {
         const MkbsRegion& g = a.regions[r];
         const int64_t bytes = (min(k.longest[c], g.rows) - a.first) * g.row_bytes;
-        runs = bytes > 0 ? (bytes + k.run[c] - 1) / k.run[c] : 0;
+        runs = bytes > 0 ? (int)((bytes + k.run[c] - 1) / k.run[c]) : 0;
     }
     __device__ __forceinline__ bool settle(const ReorderArgs& a, const Components& k) {  // false: there are no more
         while (c < k.count && at >= runs * a.regions[r].outer) {
@@ -122,17 +124,19 @@ struct Step {
             if (++r == a.num_regions) r = 0, ++c;
             if (c < k.count) count(a, k);
         }
-        return c < k.count;
+        if (c >= k.count) return false;
+        const int layer = at / runs;
+        begin = a.first * a.regions[r].row_bytes + (int64_t)(at - layer * runs) * k.run[c];
+        base = static_cast<char*>(a.regions[r].base) + layer * a.regions[r].outer_stride + begin;
+        return true;
     }
     __device__ __forceinline__ Step(const ReorderArgs& a, const Components& k) : c(0), r(0), at(blockIdx.x), runs(0) {
         if (k.count > 0) count(a, k);
     }
-    __device__ __forceinline__ int64_t begin(const ReorderArgs& a, const Components& k) const { return a.first * a.regions[r].row_bytes + at % runs * k.run[c]; }
-    __device__ __forceinline__ char* base(const ReorderArgs& a) const { return static_cast<char*>(a.regions[r].base) + at / runs * a.regions[r].outer_stride; }
     // bytes of the run that a slot holds
     __device__ __forceinline__ int held(const ReorderArgs& a, const Components& k, int slot) const {
         const MkbsRegion& g = a.regions[r];
-        return (int)max((int64_t)0, min((int64_t)k.run[c], min(k.length[slot], g.rows) * g.row_bytes - begin(a, k)));
+        return (int)max((int64_t)0, min((int64_t)k.run[c], min(k.length[slot], g.rows) * g.row_bytes - begin));
     }
 };
 
@@ -160,12 +164,11 @@ __global__ void __launch_bounds__(kReorderThreads, 1) reorder_bulk_kernel(const 
         bytes = __reduce_add_sync(0xffffffffu, bytes);
         if (lane == 0) mkb::mbar_expect_tx(bar0 + st * 8, bytes);
         __syncwarp();
-        const char* const base = load.base(a) + load.begin(a, k);
         for (int i = from + lane; i < to; i += 32) {
             const int n = load.held(a, k, k.source[i]);
             if (n > 0)
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(data + st * kStageBytes + (i - from) * run),
-                             "l"(base + k.source[i] * a.regions[load.r].slot_stride), "r"(n), "r"(bar0 + st * 8)
+                             "l"(load.base + k.source[i] * a.regions[load.r].slot_stride), "r"(n), "r"(bar0 + st * 8)
                              : "memory");
         }
         ++issued;
@@ -185,11 +188,10 @@ __global__ void __launch_bounds__(kReorderThreads, 1) reorder_bulk_kernel(const 
             }
         }
         if (!__all_sync(0xffffffffu, there)) break;
-        char* const base = store.base(a) + store.begin(a, k);
         for (int i = k.target_begin[store.c] + lane; i < k.target_begin[store.c + 1]; i += 32) {
             const int s = k.target[i], p = k.parent[s], n = store.held(a, k, p);
             if (n > 0)
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + s * a.regions[store.r].slot_stride),
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(store.base + s * a.regions[store.r].slot_stride),
                              "r"(data + st * kStageBytes + (k.place[p] - source0) * run), "r"(n)
                              : "memory");
         }
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const MkbsSelect
                 }
             }
         } else {
-            auto look = [&](uint32_t o) {  // (what does not begin with the digits so far is beyond the last one)
+            auto look = [&](uint32_t o) {  // (what does not begin with the digits so far is beyond the last one: orders end at 0xff800000)
                 const uint32_t digit = (o - limit) >> shift;
                 if (digit < 1u << bits) atomicAdd(&count[digit], 1);
             };
@@ -498,7 +500,7 @@ cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
     }
     if (bits % 16 != 0) return bits % 4 == 0 ? reorder<uint32_t>(a, s) : reorder<uint8_t>(a, s);
     if (const cudaError_t e = allow_shared_memory<reorder_bulk_kernel>(); e != cudaSuccess) return e;
-    reorder_bulk_kernel<<<kSms, kReorderThreads, kStages * kStageBytes + 128, s>>>(a);
+    reorder_bulk_kernel<<<kSms, r.slots <= 32 ? 32 : kReorderThreads, kStages * kStageBytes + 128, s>>>(a);
     return cudaGetLastError();
 }
 
