@@ -36,9 +36,9 @@ struct BeamPlan {
         for (segment = kBlockElems; (int64_t)b.beams * ((span + segment - 1) / segment) > 2 * (int64_t)b.k * segment; segment *= 2) {
         }
         segments = (int)((span + segment - 1) / segment);
-        // four blocks and more per SM before a warp takes a second segment
-        per_warp = (int)(((int64_t)rows * segments + 4 * kSms * kScanWarps - 1) / (4 * kSms * kScanWarps));
-        parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps);
+        // as few segments per warp as let all blocks run at once, three on an SM (64 rows of 128256: 576 blocks 10.5 us, 384 8.5)
+        for (per_warp = 1; parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps), parts > 1 && (int64_t)rows * parts > 3 * kSms; ++per_warp) {
+        }
         groups = b.k <= 32 ? 128 : kMergeThreads;
         // candidates: all segments, then the elements of k of them
         const int level1 = b.beams * segments, level2 = (level1 < b.k ? level1 : b.k) * segment, most = level1 > level2 ? level1 : level2;
@@ -114,7 +114,6 @@ struct Elems {
             w[v] = inside ? mkb::ld_nc_v4(base + at) : edge_vector(base, at, shift, end);
         }
     }
-    // as floats; not a number is minus infinity
     __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
@@ -129,10 +128,37 @@ struct Elems {
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], -INFINITY);
+    }
+    // the largest; not a number is minus infinity
+    __device__ __forceinline__ float most() const {
+        if constexpr (sizeof(T) == 2) {
+            auto pair = [](uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+            const __nv_bfloat162 m = __hmax2(__hmax2(pair(w[0].x), pair(w[0].y)), __hmax2(pair(w[0].z), pair(w[0].w)));
+            return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
+        } else {
+            float x[8];
+            floats(x);
+            return fmaxf(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))), -INFINITY);
+        }
     }
 };
+
+// A sum of exponentials goes with the largest logit `top` of what it sums: it is that of exp(l - top), so that the largest term is
+// exactly 1, and a beam with one continuation gives it the whole probability.  What such a sum is multiplied with to go with
+// `high`, which is not less:
+__device__ __forceinline__ float to_top(float top, float high) { return top == high ? 1.f : fast_exp2((top - high) * kLog2e); }
+
+// A lane's sum of elements first .. last - 1 in the general way, for logits that are infinite or no numbers.
+template <typename T>
+__device__ __noinline__ float general_sum(const T* base, int first, int last, int lane, float top) {
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = first + lane; i < last; i += 32) {
+        const float x = fmaxf(mkbh::to_f<T>(base[i]), -INFINITY);
+        sum += x == -INFINITY ? 0.f : to_top(x, top);
+    }
+    return sum;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamArgs a) {
@@ -154,65 +180,50 @@ __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamAr
     };
     load(first);
     for (int at = first; at < last; at += kAhead) {
-        float x[kAhead][8], high[kAhead], most = top;
+        Elems<T> now[kAhead];
+        float most = top;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (at + u < last) {
-                ahead[u].floats(x[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[u][i] = -INFINITY;
-            }
-        }
+        for (int u = 0; u < kAhead; ++u) now[u] = ahead[u];
         load(at + kAhead);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            high[u] = x[u][0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) high[u] = fmaxf(high[u], x[u][i]);
-            most = fmaxf(most, high[u]);
-        }
-        if (most == INFINITY) {  // infinite logits count, the others are nothing beside them
-            if (top < INFINITY) sum = 0.f;
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += x[u][i] == INFINITY ? 1.f : 0.f;
-        } else if (most > -INFINITY) {
-            sum *= fast_exp2((top - most) * kLog2e);  // (0 from minus infinity)
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                float part_sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) part_sum += fast_exp2((x[u][i] - most) * kLog2e);
-                sum += part_sum;
-            }
-        }
-        top = most;
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
             if (at + u >= last) break;
-            best = fmaxf(best, high[u]);
+            const float high = now[u].most();
+            most = fmaxf(most, high);
+            best = fmaxf(best, high);
             if ((at + u + 1) % blocks == 0) {
                 const uint32_t order = __reduce_max_sync(0xffffffffu, order_of(best));
                 if (lane == 0) a.tops[(size_t)row * a.segments + (at + u) / blocks] = order;
                 best = -INFINITY;
             }
         }
+        const float off = most == -INFINITY ? 0.f : most;
+        sum *= fast_exp2((top - off) * kLog2e);  // (0 from minus infinity)
+        top = most;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (at + u >= last) break;
+            float x[8], y[2] = {0.f, 0.f};
+            now[u].floats(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i & 1] += fast_exp2((x[i] - off) * kLog2e);
+            sum += y[0] + y[1];
+        }
     }
     // the lanes' and the warps' sums; a part without a finite logit has the sum 0
-    auto scaled = [](float2 part, float most) { return part.x == most ? part.y : part.x > -INFINITY ? part.y * fast_exp2((part.x - most) * kLog2e) : 0.f; };
-    const float most = value_of(__reduce_max_sync(0xffffffffu, order_of(top)));
-    sum = mkbh::warp_sum(scaled(make_float2(top, sum), most));
-    if (lane == 0) shared[warp] = make_float2(most, sum);
+    const float high = value_of(__reduce_max_sync(0xffffffffu, order_of(top)));
+    if (__any_sync(0xffffffffu, !(sum < INFINITY))) sum = general_sum(base, max(first * kBlockElems, shift), min(last * kBlockElems, end), lane, high);
+    else if (sum > 0.f) sum *= to_top(top, high);
+    sum = mkbh::warp_sum(sum);
+    if (lane == 0) shared[warp] = make_float2(high, sum);
     __syncthreads();
     if (threadIdx.x == 0) {
-        float high = shared[0].x, all = 0.f;
+        float most = shared[0].x, all = 0.f;
 #pragma unroll
-        for (int i = 1; i < kScanWarps; ++i) high = fmaxf(high, shared[i].x);
-#pragma unroll
-        for (int i = 0; i < kScanWarps; ++i) all += scaled(shared[i], high);
-        a.sums[(size_t)row * a.parts + blockIdx.x] = make_float2(high, all);
+        for (int i = 1; i < kScanWarps; ++i) most = fmaxf(most, shared[i].x);
+#pragma unroll 1
+        for (int i = 0; i < kScanWarps; ++i) all += shared[i].y > 0.f ? shared[i].y * to_top(shared[i].x, most) : 0.f;
+        a.sums[(size_t)row * a.parts + blockIdx.x] = make_float2(most, all);
     }
 }
 
@@ -272,6 +283,13 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     const uint64_t lowest = order64(-(double)INFINITY);
     auto row_of = [&](int b) { return static_cast<const T*>(a.logits) + (row0 + b) * a.row_stride; };
     auto beam_of = [&](int i) { return (int)((i + 0.5f) * per_segments); };
+    for (int b = t; b < a.beams; b += threads) {
+        const float c = a.scores != nullptr ? a.scores[row0 + b] : 0.f;
+        const bool over = a.done != nullptr && a.done[row0 + b];
+        sm.start[b] = c;
+        sm.kind[b] = !is_live(c) ? kDead : over ? kDone : kLive;
+    }
+    __syncthreads();
     mkbh::after_previous();
     int chosen = 0, infinite = 0;  // (infinite: some logit is; the bounds below hold for finite ones)
 #pragma unroll 1
@@ -293,38 +311,38 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
         };
         const bool staged = count <= a.staged;
         if (staged) {
-#pragma unroll 4
+#pragma unroll 8
             for (int i = t; i < count; i += threads) sm.staged[i] = fetch(i);
         }
         if (stage == 0) {
 #pragma unroll 1
             for (int b = warp; b < a.beams; b += threads / 32) {  // the beams' sums
-                const int row = row0 + b;
-                const float c = a.scores != nullptr ? a.scores[row] : 0.f;
-                const float2* const sums = a.sums + (size_t)row * a.parts;
-                int what = !is_live(c) ? kDead : a.done != nullptr && a.done[row] ? kDone : kLive;
                 float top = -INFINITY;
                 double sum = 0.0;
-                if (what == kLive) {
-                    for (int i = lane; i < a.parts; i += 32) top = fmaxf(top, sums[i].x);
-                    top = mkbh::warp_max(top);
+                if (sm.kind[b] == kLive) {
+                    const float2* const sums = a.sums + (size_t)(row0 + b) * a.parts;
+                    float2 part = make_float2(-INFINITY, 0.f);  // of the lane's parts together, the first 32 at once
                     for (int i = lane; i < a.parts; i += 32) {
-                        const float2 part = sums[i];
-                        sum += part.x == top ? part.y : part.x > -INFINITY ? part.y * fast_exp2((part.x - top) * kLog2e) : 0.f;
+                        const float2 next = sums[i];
+                        const float high = fmaxf(part.x, next.x);
+                        part.y = (part.y > 0.f ? part.y * to_top(part.x, high) : 0.f) + (next.y > 0.f ? next.y * to_top(next.x, high) : 0.f);
+                        part.x = high;
                     }
+                    top = mkbh::warp_max(part.x);
+                    if (part.y > 0.f) sum = part.y * to_top(part.x, top);
 #pragma unroll
                     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (top == -INFINITY) what = kDead;
                     infinite |= top == INFINITY;
                 }
-                if (lane == 0) {
+                if (lane == 0 && sm.kind[b] == kLive) {
                     const double log_sum = log(sum);
-                    sm.kind[b] = what;
-                    sm.start[b] = c;
                     sm.top[b] = top;
                     sm.log_sum[b] = log_sum;
-                    sm.offset[b] = what == kLive ? (float)((double)c - (double)top - log_sum) : -INFINITY;
+                    sm.offset[b] = (float)(sm.start[b] - (double)top - log_sum);
+                    if (top == -INFINITY) sm.kind[b] = kDead;
                 }
+                __syncwarp();
+                if (lane == 0 && sm.kind[b] != kLive) sm.offset[b] = -INFINITY;
             }
         }
         if (t == 0) listed = 0;

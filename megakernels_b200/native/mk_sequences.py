@@ -146,8 +146,8 @@ class _Where:
     """The stream of a call, and the tensors that it allocates there: given back when the call returns they go to
     that stream alone, whose later work runs after the kernels."""
 
-    def __init__(self, stream):
-        self.device = torch.cuda.current_device()
+    def __init__(self, stream, of: Tensor):
+        self.device, self.where = torch.cuda.current_device(), of.device
         if stream is None:
             self.other, self.handle = None, torch.cuda.current_stream(self.device).cuda_stream
         elif isinstance(stream, int):  # (an external stream of handle 0 would be another one from torch's pool)
@@ -156,11 +156,11 @@ class _Where:
         else:
             self.other, self.handle = stream, stream.cuda_stream
 
-    def empty(self, *shape, dtype) -> Tensor:
-        if self.other is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+    def empty(self, shape: tuple[int, ...], strides: tuple[int, ...], dtype) -> Tensor:
+        if self.other is None:  # (with its strides given a tensor takes 1.5 us, without them 2.4)
+            return torch.empty_strided(shape, strides, dtype=dtype, device=self.where)
         with torch.cuda.stream(self.other):
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return torch.empty_strided(shape, strides, dtype=dtype, device=self.where)
 
     def launch(self, name: str, struct, *used) -> None:
         """``used``: tensors that are not given out again before this stream has used them."""
@@ -207,7 +207,7 @@ def beam_select(logits: Tensor, scores: Tensor | None = None, *, beams: int, k: 
     if beams < 1 or rows < 1 or rows % beams:
         raise ValueError(f"{rows} rows of logits are no groups of {beams}")
     _refuse_host("logits", logits)
-    lib, where, groups = load_library(), _Where(stream), rows // beams
+    lib, where, groups = load_library(), _Where(stream, logits), rows // beams
     s, device = _struct(MkbsBeams), where.device
     s.groups, s.beams, s.vocab, s.k, s.dtype = groups, beams, vocab, k, int(logits.dtype is torch.float32)
     s.row_stride = logits.stride(0) if rows > 1 else vocab
@@ -220,8 +220,8 @@ def beam_select(logits: Tensor, scores: Tensor | None = None, *, beams: int, k: 
     size = lib.mkb_beam_bytes(s)
     if not size:
         where.launch("mkb_beam_select", s)  # (says what is wrong)
-    out = [where.empty(groups, k, dtype=t) for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
-    workspace = where.empty(size, dtype=torch.uint8)
+    out = [where.empty((groups, k), (k, 1), t) for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+    workspace = where.empty((size,), (1,), torch.uint8)
     s.out_scores, s.out_parents, s.out_tokens, s.out_done = (t.data_ptr() for t in out)
     s.workspace, s.workspace_bytes = workspace.data_ptr(), size
     where.launch("mkb_beam_select", s, logits, scores, done)
@@ -246,7 +246,7 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
         raise ValueError("parents must be int32 [slots]")
     _refuse_host("parents", parents)
     load_library()
-    slots, where = parents.shape[0], _Where(stream)
+    slots, where = parents.shape[0], _Where(stream, parents)
     base, device = _struct(MkbsReorder), where.device
     base.slots, base.first = slots, first
     base.parents = _check("parents", parents, torch.int32, device)
@@ -287,7 +287,7 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
     if not all(isinstance(t, Tensor) for t in (q, keys, weights)) or q.ndim != 5 or keys.ndim != 5:
         raise ValueError("q must be [layers, sequences, queries, heads, dim], keys [layers, sequences, positions, kv_heads, dim]")
     _refuse_host("q", q)
-    lib, where, bf16 = load_library(), _Where(stream), torch.bfloat16
+    lib, where, bf16 = load_library(), _Where(stream, q), torch.bfloat16
     s, device = _struct(MkbsKeyWeights), where.device
     layers, sequences, s.queries, s.heads, dim = q.shape
     positions, kv_heads = keys.shape[2:4]
@@ -307,7 +307,7 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
     size = lib.mkb_key_weights_bytes(s)
     if not size:
         where.launch("mkb_key_weights", s)  # (says what is wrong)
-    workspace = where.empty(size, dtype=torch.uint8)
+    workspace = where.empty((size,), (1,), torch.uint8)
     s.workspace, s.workspace_bytes = workspace.data_ptr(), size
     where.launch("mkb_key_weights", s, q, keys, weights, lengths, status)
 
@@ -324,7 +324,7 @@ def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int
         raise ValueError("weights must be [layers, sequences, kv_heads, positions]")
     _refuse_host("weights", weights)
     load_library()
-    s, where = _struct(MkbsSelect), _Where(stream)
+    s, where = _struct(MkbsSelect), _Where(stream, weights)
     device = where.device
     layers, sequences, kv_heads, positions = weights.shape
     s.layers, s.sequences, s.kv_heads, s.positions = layers, sequences, kv_heads, positions
@@ -336,7 +336,8 @@ def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int
         s.kept = _check("kept", kept, torch.float32, device, weights.shape, inner=1)
         if kept.stride() != weights.stride():
             raise ValueError("kept must have the strides of weights")
-    rows = where.empty(layers, sequences, kv_heads, max(keep, 1), dtype=torch.int32)  # (the library refuses less)
+    n = max(keep, 1)  # (the library refuses less)
+    rows = where.empty((layers, sequences, kv_heads, n), (sequences * kv_heads * n, kv_heads * n, n, 1), torch.int32)
     s.rows = rows.data_ptr()
     where.launch("mkb_select_rows", s, weights, lengths, kept)
     return rows
@@ -349,7 +350,7 @@ def move_rows(keys: Tensor, values: Tensor | None, rows: Tensor, lengths: Tensor
         raise ValueError("caches must be [layers, sequences, positions, kv_heads, dim], rows [layers, sequences, kv_heads, keep]")
     _refuse_host("keys", keys)
     load_library()
-    s, where = _struct(MkbsMove), _Where(stream)
+    s, where = _struct(MkbsMove), _Where(stream, keys)
     device = where.device
     layers, sequences, positions, kv_heads, dim = keys.shape
     s.layers, s.sequences, s.positions, s.kv_heads = layers, sequences, positions, kv_heads

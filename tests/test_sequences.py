@@ -301,6 +301,17 @@ def test_beam_select_far_apart_and_large_logits():
     x[0, 4321], x[1, 7] = 3e38, -3e38
     check_beams(x, beams=2, k=5)
     check_beams(draw(3, 4, 3333) * 1e4, draw(4, 1, 4) * 100, beams=4, k=40)
+    for low in (torch.finfo(F32).min, -2e6, -1.2e6, 0.9e6, 1.1e6, 3e37):  # rows whose logits are all of that size
+        x = torch.full((3, 3000), low)
+        x[0, 5::7] += abs(low) * 2**-20
+        x[1, 1000:] = torch.finfo(F32).min
+        x[2, 3::2] = -math.inf
+        check_beams(x.cuda(), beams=3, k=20)
+        x[:, 7] = math.nan
+        check_beams(x.cuda(), torch.tensor([[0.0, 1.0, -2.0]]).cuda(), beams=3, k=20)
+    near = torch.full((2, 9000), -1e6) + torch.arange(9000) % 100 / 4 - 10  # on both sides of where sums change their reference
+    check_beams(near.cuda(), beams=1, k=7)
+    check_beams(-near.cuda(), beams=2, k=7)
 
 
 # ---- reordering ----------------------------------------------------------------------------------- #
