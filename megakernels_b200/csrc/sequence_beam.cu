@@ -21,30 +21,32 @@ namespace {
 
 constexpr int kBlockElems = 256;  // elements that a warp reads at a time
 constexpr int kScanWarps = 8, kAhead = 4;  // (kAhead: blocks whose loads are under way together)
-constexpr int kMergeThreads = 512, kStaged = 8192, kListed = kMergeThreads;  // (kStaged: candidates whose logits lie in shared memory)
+constexpr int kMergeThreads = 512, kStaged = 8192, kListed = kMergeThreads;  // (kStaged: candidates whose bounds lie in shared memory)
 constexpr int kCandidateBytes = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamPlan {
     int rows, segment, segments, per_warp, parts;  // elements per segment; segments of a row and of a warp, blocks of a row
-    int groups, list_a, list_b, staged;            // of the merge: groups per round, entries of the two lists, logits in shared memory
+    int groups, list_a, list_b, staged;            // of the merge: groups per round, entries of the two lists, bounds in shared memory
+    int chosen;                                    // segments whose elements are candidates, at most
     size_t part_offset, bytes;
     explicit BeamPlan(const MkbsBeams& b) {
         rows = b.groups * b.beams;
         const int64_t span = b.vocab + 15;  // (a row may start anywhere in 16 bytes)
-        // as many segments as the chosen ones have elements, at least 256
-        for (segment = kBlockElems; (int64_t)b.beams * ((span + segment - 1) / segment) > 2 * (int64_t)b.k * segment; segment *= 2) {
+        // about as many segments as the chosen ones have elements, of 256 at least
+        chosen = most_chosen(b.k);
+        for (segment = kBlockElems; (int64_t)b.beams * ((span + segment - 1) / segment) > 2 * (int64_t)chosen * segment; segment *= 2) {
         }
         segments = (int)((span + segment - 1) / segment);
         // as few segments per warp as let all blocks run at once, three on an SM (64 rows of 128256: 576 blocks 10.5 us, 384 8.5)
         for (per_warp = 1; parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps), parts > 1 && (int64_t)rows * parts > 3 * kSms; ++per_warp) {
         }
-        groups = b.k <= 32 ? 128 : kMergeThreads;
-        // candidates: all segments, then the elements of k of them
-        const int level1 = b.beams * segments, level2 = (level1 < b.k ? level1 : b.k) * segment, most = level1 > level2 ? level1 : level2;
+        groups = b.k <= 16 ? 128 : b.k <= 32 ? 256 : kMergeThreads;
+        // candidates: all segments, then the elements of k of them, or of those that may be among the k
+        const int level1 = b.beams * segments, level2 = (level1 < chosen ? level1 : chosen) * segment, most = level1 > level2 ? level1 : level2;
         list_a = next(most, b.k) < kListed ? kListed : (next(most, b.k) + 3) / 4 * 4;  // (16-byte numbers follow)
         list_b = (next(list_a, b.k) + 3) / 4 * 4;
-        staged = most < kStaged ? most : kStaged;
+        staged = most < kStaged ? (most + 1) / 2 * 2 : kStaged;
         part_offset = ((size_t)rows * segments * 4 + 255) / 256 * 256;
         bytes = part_offset + (size_t)rows * parts * 8;
     }
@@ -52,11 +54,15 @@ struct BeamPlan {
         if (m <= groups) return 0;
         return k * (m <= kMergeThreads ? (m + groups - 1) / groups : (m + kMergeThreads - 1) / kMergeThreads * (kMergeThreads / groups));
     }
-    size_t merge_smem() const { return (size_t)(list_a + list_b + groups) * kCandidateBytes + (size_t)(groups + staged) * 4 + MKBS_MAX_BEST * 8 + MKBS_MAX_BEAMS * 28; }
+    static constexpr int most_chosen(int k) { return k + k / 4 + 8; }
+    size_t merge_smem() const {  // (bounds and lists take turns)
+        const size_t lists = (size_t)(list_a + list_b) * kCandidateBytes, bounds = (size_t)staged * 4;
+        return (lists > bounds ? lists : bounds) + (size_t)groups * (kCandidateBytes + 4) + (size_t)chosen * 16 + MKBS_MAX_BEAMS * 28 + kListed * 4;
+    }
 };
 
 struct BeamArgs {
-    int beams, vocab, k, segment, segments, per_warp, parts, groups, list_a, list_b, staged;
+    int beams, vocab, k, segment, segments, per_warp, parts, groups, list_a, list_b, staged, chosen;
     int64_t row_stride;
     const void* logits;
     const float* scores;
@@ -242,25 +248,29 @@ struct Candidate {
 struct MergeSmem {
     uint64_t *key_a, *key_b, *group_key;
     double *log_sum, *start;
-    uint32_t *at_a, *at_b, *group_at, *staged;
-    int *rank, *chosen_beam, *chosen_segment, *kind;
+    const void** chosen_at;
+    uint32_t *at_a, *at_b, *group_at, *staged, *listed;
+    int *rank, *chosen_beam, *chosen_first, *kind;  // chosen_first: what the segment's first element continues its beam with
     float *top, *offset;
     __device__ MergeSmem(void* raw, const BeamArgs& a) {
-        key_a = static_cast<uint64_t*>(raw);
+        group_at = static_cast<uint32_t*>(raw);  // (read 16 bytes at a time)
+        listed = group_at + a.groups;
+        staged = listed + kListed;
+        key_a = reinterpret_cast<uint64_t*>(staged);
         key_b = key_a + a.list_a;
-        group_key = key_b + a.list_b;
-        log_sum = reinterpret_cast<double*>(group_key + a.groups);
-        start = log_sum + MKBS_MAX_BEAMS;
-        at_a = reinterpret_cast<uint32_t*>(start + MKBS_MAX_BEAMS);
+        at_a = reinterpret_cast<uint32_t*>(key_b + a.list_b);
         at_b = at_a + a.list_a;
-        group_at = at_b + a.list_b;
-        rank = reinterpret_cast<int*>(group_at + a.groups);
+        uint32_t *const lists_end = at_b + a.list_b, *const bounds_end = staged + a.staged;
+        group_key = reinterpret_cast<uint64_t*>(lists_end > bounds_end ? lists_end : bounds_end);
+        chosen_at = reinterpret_cast<const void**>(group_key + a.groups);
+        log_sum = reinterpret_cast<double*>(chosen_at + a.chosen);
+        start = log_sum + MKBS_MAX_BEAMS;
+        rank = reinterpret_cast<int*>(start + MKBS_MAX_BEAMS);
         chosen_beam = rank + a.groups;
-        chosen_segment = chosen_beam + MKBS_MAX_BEST;
-        kind = chosen_segment + MKBS_MAX_BEST;
+        chosen_first = chosen_beam + a.chosen;
+        kind = chosen_first + a.chosen;
         top = reinterpret_cast<float*>(kind + MKBS_MAX_BEAMS);
         offset = top + MKBS_MAX_BEAMS;
-        staged = reinterpret_cast<uint32_t*>(offset + MKBS_MAX_BEAMS);
     }
 };
 
@@ -297,17 +307,22 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
         int count = stage == 0 ? a.beams * segments : chosen << shift_segment;
         // element i: of which beam, and where in its row; -1: none
         auto place = [&](int i, int& v) {
-            const int b = sm.chosen_beam[i >> shift_segment];
-            if (b < 0) return -1;
-            v = (sm.chosen_segment[i >> shift_segment] << shift_segment) + (i & (a.segment - 1)) - shift_of(row_of(b));
-            return v >= 0 && v < a.vocab ? b : -1;
+            v = sm.chosen_first[i >> shift_segment] + (i & (a.segment - 1));
+            return v >= 0 && v < a.vocab ? sm.chosen_beam[i >> shift_segment] : -1;
         };
         // a segment's largest logit, or an element, as order_of; 0: there is none (not set for a beam that has none, or has ended)
         auto fetch = [&](int i) {
             if (stage == 0) return tops[i];
             int v = 0;
             const int b = place(i, v);
-            return b >= 0 && sm.kind[b] == kLive ? order_of(fmaxf(mkbh::to_f<T>(row_of(b)[v]), -INFINITY)) : 0u;
+            const T* const at = static_cast<const T*>(sm.chosen_at[i >> shift_segment]) + (i & (a.segment - 1));
+            return b >= 0 && sm.kind[b] == kLive ? order_of(fmaxf(mkbh::to_f<T>(*at), -INFINITY)) : 0u;
+        };
+        auto choose = [&](int n, int b, int s) {  // segment s of beam b, as the n-th; b below 0: none
+            const T* const row = row_of(max(b, 0));
+            sm.chosen_beam[n] = b;
+            sm.chosen_first[n] = (s << shift_segment) - shift_of(row);
+            sm.chosen_at[n] = row + ((s << shift_segment) - shift_of(row));
         };
         const bool staged = count <= a.staged;
         if (staged) {
@@ -348,7 +363,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
         if (t == 0) listed = 0;
         infinite = __syncthreads_or(infinite);
         auto candidate = [&](int i) {
-            const uint32_t order = staged ? sm.staged[i] : fetch(i);
+            const uint32_t order = fetch(i);
             int b, v = 0;
             bool there, ends;
             uint32_t at = i;
@@ -377,8 +392,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
         auto take = [&](int rank, const Candidate& c) {
             if (stage == 0) {
                 const int b = c.key ? beam_of(c.at) : -1;
-                sm.chosen_beam[rank] = b;
-                sm.chosen_segment[rank] = c.at - b * segments;
+                choose(rank, b, c.at - b * segments);
             } else {
                 const int b = c.at / a.vocab, v = c.at - b * a.vocab, to = group_of * k + rank;
                 a.out_scores[to] = (float)value64(c.key);
@@ -388,9 +402,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             }
         };
         // A score in fp32, and by how much it may be off
-        auto score = [&](int i, float& off) {
+        auto score = [&](int i, uint32_t order, float& off) {
             const int b = stage == 0 ? beam_of(i) : max(sm.chosen_beam[i >> shift_segment], 0);
-            const uint32_t order = staged ? sm.staged[i] : fetch(i);
             const float x = order ? value_of(order) : -INFINITY, y = sm.offset[b];
             off = (fabsf(x) + fabsf(y)) * 0x1p-21f;  // (infinite with the score; then the bounds are not numbers, and pass no comparison)
             return x + y;
@@ -399,8 +412,9 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
 #pragma unroll 2
         for (int i = t; i < count; i += threads) {
             float off;
-            const float x = score(i, off);
+            const float x = score(i, staged ? sm.staged[i] : fetch(i), off);
             best_score = fmaxf(best_score, x - off);
+            if (staged) sm.staged[i] = __float_as_uint(x + off);
         }
         for (int o = lanes / 2; o; o >>= 1) best_score = fmaxf(best_score, __shfl_xor_sync(0xffffffffu, best_score, o));
         if (t % lanes == 0) {
@@ -425,33 +439,45 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
         if (t % lanes == 0 && sm.rank[group] == k - 1) bound = order_of(best_score);
         __syncthreads();
         const float least = value_of(bound);
-        auto list = [&](int i) {
+        // What may be among the k best: of the segments all are chosen, in any order, of the elements the k best
+        const int most = stage == 0 ? a.chosen : kListed;
+        auto list = [&](int i, int b, int segment_of) {
             const int n = atomicAdd(&listed, 1);
-            if (n < kListed) sm.at_a[n] = i;
+            if (n >= most) return;
+            if (stage == 0) choose(n, b, segment_of);
+            else sm.listed[n] = i;
         };
         if (least > -INFINITY && !infinite) {
-#pragma unroll 2
+#pragma unroll 4
             for (int i = t; i < count; i += threads) {
-                float off;
-                const float x = score(i, off);
-                if (x + off >= least) list(i);
+                float high;
+                if (staged) {
+                    high = __uint_as_float(sm.staged[i]);
+                } else {
+                    float off;
+                    high = score(i, fetch(i), off);
+                    high += off;
+                }
+                if (high >= least) list(i, stage == 0 ? beam_of(i) : 0, stage == 0 ? i - beam_of(i) * segments : 0);
             }
             // beams that have ended: their one continuation
             if (a.done != nullptr && t < (stage == 0 ? a.beams : chosen)) {
                 const int b = stage == 0 ? t : sm.chosen_beam[t];
                 if (b >= 0 && sm.kind[b] == kDone) {
-                    const int at = a.eos + shift_of(row_of(b)), s = at >> shift_segment;
-                    if (stage == 0) list(b * segments + s);
-                    else if (s == sm.chosen_segment[t]) list((t << shift_segment) + (at & (a.segment - 1)));
+                    const int at = stage == 0 ? 0 : a.eos - sm.chosen_first[t];
+                    if (stage == 0) list(0, b, (a.eos + shift_of(row_of(b))) >> shift_segment);
+                    else if (at >= 0 && at < a.segment) list((t << shift_segment) + at, 0, 0);
                 }
             }
         }
         __syncthreads();
         const int some = listed;
-        if (some >= k && some <= kListed) {
+        const bool few_listed = some >= min(k, count) && some <= most && least > -INFINITY;
+        if (stage == 0 && few_listed) {
+            chosen = some;
+        } else if (few_listed) {
             Candidate own{0, 0};
-            if (t < some) own = candidate(sm.at_a[t]);
-            __syncthreads();
+            if (t < some) own = candidate(sm.listed[t]);
             sm.key_a[t] = own.key;
             sm.at_a[t] = own.at;
             __syncthreads();
@@ -518,7 +544,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
                 __syncthreads();
             }
         }
-        chosen = min(k, a.beams * segments);
+        if (stage == 0 && !few_listed) chosen = min(k, a.beams * segments);
         __syncthreads();
     }
 }
@@ -545,12 +571,15 @@ cudaError_t launch(const BeamPlan& p, const MkbsBeams& b, const BeamArgs& a, cud
 
 }  // namespace
 
-size_t beam_bytes(const MkbsBeams& b) { return BeamPlan(b).bytes; }
+size_t beam_bytes(const MkbsBeams& b) {
+    const BeamPlan p(b);
+    return p.merge_smem() <= 227 * 1024 - kStaticShared ? p.bytes : 0;
+}
 
 cudaError_t beam_launch(const MkbsBeams& b, cudaStream_t s) {
     const BeamPlan p(b);
     char* const work = static_cast<char*>(b.workspace);
-    const BeamArgs a{b.beams, b.vocab, b.k, p.segment, p.segments, p.per_warp, p.parts, p.groups, p.list_a, p.list_b, p.staged, b.row_stride, b.logits, b.scores,
+    const BeamArgs a{b.beams, b.vocab, b.k, p.segment, p.segments, p.per_warp, p.parts, p.groups, p.list_a, p.list_b, p.staged, p.chosen, b.row_stride, b.logits, b.scores,
                      b.done, b.eos, reinterpret_cast<uint32_t*>(work), reinterpret_cast<float2*>(work + p.part_offset), b.out_scores, b.out_parents,
                      b.out_tokens, b.out_done};
     return b.dtype == MKBS_F32 ? launch<float>(p, b, a, s) : launch<bf16>(p, b, a, s);

@@ -46,6 +46,7 @@ int check_shape(const MkbsBeams* b) {
     if ((int64_t)b->beams * b->vocab > MKBS_MAX_BEAM_WORK / b->k)
         return fail(MKBS_ERR_UNSUPPORTED, "beams: beams * vocab * k above %d", MKBS_MAX_BEAM_WORK);
     if (b->k > (int64_t)b->beams * b->vocab) return invalid("beams: k is more than there are continuations");
+    if (mkbs::beam_bytes(*b) == 0) return fail(MKBS_ERR_UNSUPPORTED, "beams: more candidates than shared memory holds");
     return MKBS_OK;
 }
 int check(const MkbsBeams* b) {

@@ -156,6 +156,17 @@ def test_only_the_device_is_missing_in_the_calls_that_the_refusals_start_from(na
     assert getattr(lib, f"mkb_{name}")(None, None) == 1
 
 
+def test_beam_selection_takes_all_it_says_it_takes():
+    """Every shape at the limits has a plan that fits shared memory."""
+    lib = ops.load_library()
+    for k in range(1, 129):
+        for beams in (1, 2, 3, 5, 8, 13, 16, 32, 63, 64):
+            vocab = (1 << 30) // (beams * k)
+            for v in {vocab, vocab // 2, vocab // 3, 128256}:
+                if v * beams * k <= 1 << 30:
+                    assert lib.mkb_beam_bytes(ctypes.byref(beams_struct(groups=1, beams=beams, vocab=v, k=k))) > 0, (k, beams, v)
+
+
 def test_workspace_sizes_of_wrong_shapes_are_zero():
     lib = ops.load_library()
     assert lib.mkb_beam_bytes(ctypes.byref(beams_struct())) > 0 and lib.mkb_beam_bytes(ctypes.byref(beams_struct(k=0))) == 0
@@ -188,27 +199,27 @@ def test_the_shim_refuses_what_is_not_on_the_device():
 # ---- beam selection ------------------------------------------------------------------------------ #
 def beam_reference(logits, scores, beams, k, done, eos):
     rows, vocab = logits.shape
-    x = logits.cpu().double()
+    x = logits.double()
     x[x.isnan()] = -math.inf
     top = x.max(dim=1, keepdim=True).values
     from_top = torch.where(x == top, torch.zeros_like(x), x - top)  # (infinite logits share everything)
     log_p = from_top - from_top.exp().sum(dim=1, keepdim=True).log()
-    c = (scores.cpu().double() if scores is not None else torch.zeros(rows // beams, beams).double()).reshape(-1, 1)
+    c = (scores.double() if scores is not None else x.new_zeros(rows // beams, beams)).reshape(-1, 1)
     total = torch.where(x == -math.inf, torch.full_like(x, -math.inf), c + log_p)
     if done is not None:
-        over = done.cpu().reshape(-1) != 0
+        over = done.reshape(-1) != 0
         total[over] = -math.inf
         total[over, eos] = c[over, 0]
     total[~c.isfinite().reshape(-1)] = -math.inf
     flat = total.view(rows // beams, beams * vocab)
     best, at = torch.sort(flat, dim=1, descending=True, stable=True)
     best, at = best[:, :k], at[:, :k]
-    parents = at // vocab + torch.arange(rows // beams).unsqueeze(1) * beams
+    parents = at // vocab + torch.arange(rows // beams, device=x.device).unsqueeze(1) * beams
     tokens = at % vocab
     ended = tokens == (-1 if eos is None else eos)
     if done is not None:
-        ended |= done.cpu().reshape(-1)[parents] != 0
-    return best, parents, tokens, ended
+        ended |= done.reshape(-1)[parents] != 0
+    return best.cpu(), parents.cpu(), tokens.cpu(), ended.cpu()
 
 
 def check_beams(logits, scores=None, *, beams, k, done=None, eos=None, stream=None):
@@ -238,7 +249,7 @@ BF16, F32 = torch.bfloat16, torch.float32
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("groups,beams,vocab,k", [
     (1, 1, 1, 1), (2, 1, 7, 7), (3, 2, 5, 10), (1, 4, 255, 4), (2, 3, 256, 6), (1, 5, 257, 128), (5, 2, 4099, 16), (1, 64, 1000, 128), (1, 64, 128256, 64),
-    (1, 4, 128256, 4), (8, 8, 128256, 16), (64, 1, 32003, 3), (1, 16, 32003, 33), (2, 1, 262144, 128),
+    (1, 4, 128256, 4), (8, 8, 128256, 16), (64, 1, 32003, 3), (1, 16, 32003, 33), (2, 1, 262144, 128), (1, 64, 131072, 128), (1, 64, 262144, 32), (1, 2, 500_000, 1),
 ])
 def test_beam_select(groups, beams, vocab, k, dtype):
     rows = groups * beams
