@@ -23,6 +23,7 @@ constexpr int kBlockElems = 256;  // elements that a warp reads at a time
 constexpr int kScanWarps = 8, kAhead = 4;  // (kAhead: blocks whose loads are under way together)
 constexpr int kMergeThreads = 512, kStaged = 8192, kListed = kMergeThreads;  // (kStaged: candidates whose bounds lie in shared memory)
 constexpr int kCandidateBytes = 12;
+constexpr size_t kMostShared = 227 * 1024 - kStaticShared;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamPlan {
@@ -41,12 +42,15 @@ struct BeamPlan {
         // as few segments per warp as let all blocks run at once, three on an SM (64 rows of 128256: 576 blocks 10.5 us, 384 8.5)
         for (per_warp = 1; parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps), parts > 1 && (int64_t)rows * parts > 3 * kSms; ++per_warp) {
         }
-        groups = b.k <= 16 ? 128 : b.k <= 32 ? 256 : kMergeThreads;
         // candidates: all segments, then the elements of k of them, or of those that may be among the k
         const int level1 = b.beams * segments, level2 = (level1 < chosen ? level1 : chosen) * segment, most = level1 > level2 ? level1 : level2;
-        list_a = next(most, b.k) < kListed ? kListed : (next(most, b.k) + 3) / 4 * 4;  // (16-byte numbers follow)
-        list_b = (next(list_a, b.k) + 3) / 4 * 4;
         staged = most < kStaged ? (most + 1) / 2 * 2 : kStaged;
+        // (the more groups, the shorter the lists, and the longer a round's ranking)
+        for (groups = 64;; groups *= 2) {
+            list_a = next(most, b.k) < kListed ? kListed : (next(most, b.k) + 3) / 4 * 4;  // (16-byte numbers follow)
+            list_b = (next(list_a, b.k) + 3) / 4 * 4;
+            if (groups >= kMergeThreads || (groups >= 4 * b.k && merge_smem() <= kMostShared)) break;
+        }
         part_offset = ((size_t)rows * segments * 4 + 255) / 256 * 256;
         bytes = part_offset + (size_t)rows * parts * 8;
     }
@@ -248,7 +252,7 @@ struct Candidate {
 struct MergeSmem {
     uint64_t *key_a, *key_b, *group_key;
     double *log_sum, *start;
-    const void** chosen_at;
+    const void** chosen_row;
     uint32_t *at_a, *at_b, *group_at, *staged, *listed;
     int *rank, *chosen_beam, *chosen_first, *kind;  // chosen_first: what the segment's first element continues its beam with
     float *top, *offset;
@@ -262,8 +266,8 @@ struct MergeSmem {
         at_b = at_a + a.list_a;
         uint32_t *const lists_end = at_b + a.list_b, *const bounds_end = staged + a.staged;
         group_key = reinterpret_cast<uint64_t*>(lists_end > bounds_end ? lists_end : bounds_end);
-        chosen_at = reinterpret_cast<const void**>(group_key + a.groups);
-        log_sum = reinterpret_cast<double*>(chosen_at + a.chosen);
+        chosen_row = reinterpret_cast<const void**>(group_key + a.groups);
+        log_sum = reinterpret_cast<double*>(chosen_row + a.chosen);
         start = log_sum + MKBS_MAX_BEAMS;
         rank = reinterpret_cast<int*>(start + MKBS_MAX_BEAMS);
         chosen_beam = rank + a.groups;
@@ -314,15 +318,15 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
         auto fetch = [&](int i) {
             if (stage == 0) return tops[i];
             int v = 0;
-            const int b = place(i, v);
-            const T* const at = static_cast<const T*>(sm.chosen_at[i >> shift_segment]) + (i & (a.segment - 1));
-            return b >= 0 && sm.kind[b] == kLive ? order_of(fmaxf(mkbh::to_f<T>(*at), -INFINITY)) : 0u;
+            const int b = place(i, v);  // (read in any case, so that reads do not wait for one another)
+            const float x = mkbh::to_f<T>(static_cast<const T*>(sm.chosen_row[i >> shift_segment])[min(max(v, 0), a.vocab - 1)]);
+            return b >= 0 && sm.kind[b] == kLive ? order_of(fmaxf(x, -INFINITY)) : 0u;
         };
         auto choose = [&](int n, int b, int s) {  // segment s of beam b, as the n-th; b below 0: none
             const T* const row = row_of(max(b, 0));
             sm.chosen_beam[n] = b;
             sm.chosen_first[n] = (s << shift_segment) - shift_of(row);
-            sm.chosen_at[n] = row + ((s << shift_segment) - shift_of(row));
+            sm.chosen_row[n] = row;
         };
         const bool staged = count <= a.staged;
         if (staged) {
@@ -481,11 +485,12 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             sm.key_a[t] = own.key;
             sm.at_a[t] = own.at;
             __syncthreads();
-            if (t < some) {
+#pragma unroll 1
+            for (int c = warp; c < some; c += threads / 32) {  // (a warp ranks a candidate)
+                const Candidate it{sm.key_a[c], sm.at_a[c]};
                 int rank = 0;
-#pragma unroll 4
-                for (int j = 0; j < some; ++j) rank += Candidate{sm.key_a[j], sm.at_a[j]}.before(own);
-                if (rank < k) take(rank, own);
+                for (int j = lane; j - lane < some; j += 32) rank += __popc(__ballot_sync(0xffffffffu, j < some && Candidate{sm.key_a[j], sm.at_a[j]}.before(it)));
+                if (lane == 0 && rank < k) take(rank, it);
             }
         } else {
             // Rounds: into groups by thread, the groups' best ranked, the members of the first k into a list
@@ -573,7 +578,7 @@ cudaError_t launch(const BeamPlan& p, const MkbsBeams& b, const BeamArgs& a, cud
 
 size_t beam_bytes(const MkbsBeams& b) {
     const BeamPlan p(b);
-    return p.merge_smem() <= 227 * 1024 - kStaticShared ? p.bytes : 0;
+    return p.merge_smem() <= kMostShared ? p.bytes : 0;
 }
 
 cudaError_t beam_launch(const MkbsBeams& b, cudaStream_t s) {
