@@ -322,6 +322,8 @@ int mkb_launch(const MkbGlobals *g, void *cuda_stream);
  * (`wait_timeout_ms` holds for every wait of these kernels too); batch and tensor-parallel launches, residual_scale > 1,
  * MKB_FLAG_RECORD_TIMINGS and a head_dim other than 64 or 128 are MKB_ERR_UNSUPPORTED.  Instructions, barriers and the
  * activation vectors of `g` are not touched.  `workspace`: mkb_prompt_bytes(g, tokens) bytes, 256-byte aligned.
+ * With `key_weights` the softmax weight that the last `observed` of these tokens' queries give each cached key is added
+ * there, summed over the query heads that share it (mkb_key_weights of mkb200_sequences.h).
  */
 typedef struct MkbPrompt {
     uint32_t struct_bytes;
@@ -331,8 +333,17 @@ typedef struct MkbPrompt {
     const void *hidden;   /* bf16 [tokens, hidden_size], 16-byte aligned */
     void *workspace;
     size_t workspace_bytes;
+    /* From here on optional: struct_bytes may end before (MKB_PROMPT_BYTES_PLAIN), or all of it be zero. */
+    float *key_weights;   /* [num_layers, num_kv_heads, kv_max_len] with the strides below, or NULL */
+    int64_t weights_layer, weights_head; /* in elements */
+    int32_t observed;     /* 1..tokens */
+    int32_t reserved;
+    void *weights_workspace; /* mkb_prompt_weights_bytes(g, tokens, pos0, observed) bytes, 256-byte aligned */
+    size_t weights_workspace_bytes;
 } MkbPrompt;
+#define MKB_PROMPT_BYTES_PLAIN 40
 size_t mkb_prompt_bytes(const MkbGlobals *g, int32_t tokens);
+size_t mkb_prompt_weights_bytes(const MkbGlobals *g, int32_t tokens, int32_t pos0, int32_t observed); /* 0: not valid */
 int mkb_prompt(const MkbGlobals *g, const MkbPrompt *p, void *cuda_stream);
 
 /*

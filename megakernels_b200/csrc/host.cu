@@ -3,6 +3,7 @@
 // glue of the reference (demos/low-latency-llama/llama.cu:26-53), which builds
 // its descriptors on every call inside ThunderKittens' bind_kernel.
 #include <cstdarg>
+#include <cstddef>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -11,6 +12,7 @@
 
 #include "llama_prompt.h"
 #include "mk_common.cuh"
+#include "sequence_kernels.h"
 
 namespace mkb {
 __global__ void megakernel(const __grid_constant__ KParams p);
@@ -553,8 +555,21 @@ int mkb_launch(const MkbGlobals* g, void* cuda_stream) {
 
 size_t mkb_prompt_bytes(const MkbGlobals* g, int32_t tokens) { return g && tokens > 0 ? mkb::PromptBuffers(*g, tokens, nullptr).total : 0; }
 
-int mkb_prompt(const MkbGlobals* g, const MkbPrompt* p, void* cuda_stream) {
-    if (!p || p->struct_bytes != sizeof(MkbPrompt)) return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: NULL or another struct size");
+static_assert(offsetof(MkbPrompt, key_weights) == MKB_PROMPT_BYTES_PLAIN, "the fields that every caller knows");
+
+size_t mkb_prompt_weights_bytes(const MkbGlobals* g, int32_t tokens, int32_t pos0, int32_t observed) {
+    if (!g || tokens < 1 || pos0 < 0 || observed < 1 || observed > tokens || (int64_t)pos0 + tokens > g->kv_max_len || g->num_kv_heads < 1 ||
+        g->num_attention_heads < g->num_kv_heads || g->num_attention_heads / g->num_kv_heads > 128)
+        return 0;
+    return mkbs::key_weights_bytes(mkb::prompt_weights(*g, tokens, pos0, observed));
+}
+
+int mkb_prompt(const MkbGlobals* g, const MkbPrompt* caller, void* cuda_stream) {
+    if (!caller || (caller->struct_bytes != sizeof(MkbPrompt) && caller->struct_bytes != MKB_PROMPT_BYTES_PLAIN))
+        return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: NULL or another struct size");
+    MkbPrompt whole = {};
+    memcpy(&whole, caller, caller->struct_bytes);
+    const MkbPrompt* const p = &whole;
     if (g && (g->flags & MKB_FLAG_RECORD_TIMINGS))
         return fail(MKB_ERR_UNSUPPORTED, "prompt: no instructions run, so there are no timings to record");
     int* status = nullptr;
@@ -572,6 +587,14 @@ int mkb_prompt(const MkbGlobals* g, const MkbPrompt* p, void* cuda_stream) {
     if (!p->hidden || !aligned16(p->hidden) || !p->workspace || ((uintptr_t)p->workspace & 255) ||
         p->workspace_bytes < mkb_prompt_bytes(g, p->tokens))
         return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: hidden or workspace missing, unaligned or too small");
+    if (p->key_weights) {
+        if (p->observed < 1 || p->observed > p->tokens) return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: %d of %d tokens observed", p->observed, p->tokens);
+        if (((uintptr_t)p->key_weights & 3) || p->weights_head < g->kv_max_len || p->weights_layer < g->kv_max_len)
+            return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: key weights unaligned, or heads or layers of them overlap");
+        if (!p->weights_workspace || ((uintptr_t)p->weights_workspace & 255) ||
+            p->weights_workspace_bytes < mkb_prompt_weights_bytes(g, p->tokens, p->pos0, p->observed))
+            return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: workspace of the key weights missing, unaligned or too small");
+    }
     MKB_CUDA(mkb::prompt_launch(*g, *p, status, (cudaStream_t)cuda_stream));
     return MKB_OK;
 }

@@ -7,6 +7,7 @@
 #include "llama_prompt.h"
 
 #include "hybrid_kernels.h"
+#include "sequence_kernels.h"
 
 namespace mkb {
 namespace {
@@ -94,6 +95,16 @@ cudaError_t prompt_launch(const MkbGlobals& g, const MkbPrompt& p, int* status, 
         MKB_TRY(gemm(b.act, at(g.qkv_weights, i * (Q + 2 * KV) * H), n, Q + 2 * KV, H,
                      GemmEpilogue::rotate({b.q, k, v, Q, KV, D, p.pos0, static_cast<const float*>(g.rope_cos), static_cast<const float*>(g.rope_sin)})));
         MKB_TRY(mkbh::flash_cache({b.q, k, v, b.act, n, p.pos0, g.num_attention_heads, g.num_kv_heads, D, g.attn_scale, status, wait}, s));
+        if (p.key_weights != nullptr) {
+            MkbsKeyWeights w = prompt_weights(g, n, p.pos0, p.observed);
+            w.q = b.q + (size_t)(n - p.observed) * Q;
+            w.k = k;
+            w.weights = p.key_weights + i * p.weights_layer;
+            w.w_head = p.weights_head;
+            w.workspace = p.weights_workspace;
+            w.status = status;
+            MKB_TRY(mkbs::key_weights_launch(w, s));
+        }
         MKB_TRY(gemm(b.act, at(g.o_proj_weights, i * H * Q), n, H, Q, GemmEpilogue::add_fixed(b.sums, H)));
         MKB_TRY(norm(0, n, false, nullptr, at(g.mlp_ln_weights, i * H)));
         MKB_TRY(gemm(b.act, at(g.gate_proj_weights, i * F * H), n, F, H, GemmEpilogue::silu(b.ffn, F), at(g.up_proj_weights, i * F * H)));

@@ -1,5 +1,6 @@
 // Prompts of llama models: tokens at once (llama_prompt.cu).
 #pragma once
+#include "../../include/mkb200_sequences.h"
 #include "mk_common.cuh"
 
 namespace mkb {
@@ -23,6 +24,23 @@ struct PromptBuffers {
         ffn = reinterpret_cast<__nv_bfloat16*>(take((size_t)g.intermediate_size * 2));
     }
 };
+
+// What the queries of the last `observed` of `tokens` tokens from pos0 on add to the keys' weights in one layer (pointers are
+// left to prompt_launch).
+inline MkbsKeyWeights prompt_weights(const MkbGlobals& g, int tokens, int pos0, int observed) {
+    MkbsKeyWeights w = {};
+    w.struct_bytes = sizeof(w);
+    w.layers = w.sequences = 1;
+    w.queries = observed;
+    w.heads = g.num_attention_heads;
+    w.kv_heads = g.num_kv_heads;
+    w.dim = g.head_dim;
+    w.positions = g.kv_max_len;
+    w.length = pos0 + tokens;
+    w.scale = g.attn_scale;
+    w.wait_timeout_ms = g.wait_timeout_ms;
+    return w;
+}
 
 cudaError_t prompt_launch(const MkbGlobals& g, const MkbPrompt& p, int* status, cudaStream_t stream);
 

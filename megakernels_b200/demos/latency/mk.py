@@ -68,11 +68,15 @@ class LatencyMK_Interpreter(MK_Interpreter):
     def interpret(self, globs: Globals, **kwargs):
         return interpret_with_mk(globs, self.mk_func, **kwargs)
 
-    def prompt(self, globs: Globals, hidden: torch.Tensor, pos0: int, want_logits: bool):
-        """The tokens whose embeddings are ``hidden`` at once, from position ``pos0`` on; no counterpart in the reference."""
+    def prompt(self, globs: Globals, hidden: torch.Tensor, pos0: int, want_logits: bool, observed: int = 0):
+        """The tokens whose embeddings are ``hidden`` at once, from position ``pos0`` on; no counterpart in the reference.
+
+        The attention of the last ``observed`` of them is added to ``globs.key_weights``.
+        """
         globs.pos_id = pos0 + hidden.shape[0] - 1
+        weights = globs.key_weights if observed else None
 
         def call(*args, **kwargs):
-            return self.module.mk_llama_prompt(*args, hidden=hidden, pos0=pos0, want_logits=want_logits, **kwargs)
+            return self.module.mk_llama_prompt(*args, hidden=hidden, pos0=pos0, want_logits=want_logits, key_weights=weights, observed=observed, **kwargs)
 
         return interpret_with_mk(globs, call)

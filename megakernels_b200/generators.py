@@ -12,9 +12,11 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
+from megakernels_b200.beams import BeamResult, beam_search
 from megakernels_b200.demos.latency.mk import LatencyMK_Interpreter
-from megakernels_b200.demos.latency.scheduler import covers_model
-from megakernels_b200.mk import MK_Interpreter
+from megakernels_b200.demos.latency.scheduler import covers_model, make_globals
+from megakernels_b200.llama import build_rope_tables
+from megakernels_b200.mk import MK_Interpreter, get_mk_module
 from megakernels_b200.model_types import BatchState
 from megakernels_b200.scheduler import Schedule
 
@@ -219,8 +221,8 @@ class MK_Generator(Generator):
     # at the 8B widths, are a workspace of this many tokens.
     prompt_portion = 2048
 
-    def _takes_prompts(self, count: int) -> bool:
-        """Whether a prompt of ``count`` tokens goes through the layers at once (``mkb_prompt``).
+    def _takes_prompts(self, count: int, position: int = 0) -> bool:
+        """Whether a prompt of ``count`` tokens from ``position`` on goes through the layers at once (``mkb_prompt``).
 
         Only where that is the same as a step per token: the whole model's instructions (those that were looked at when
         the generator was made, not edited since) on the library's own interpreter, one sequence on one GPU, no part of a
@@ -229,7 +231,7 @@ class MK_Generator(Generator):
         globs, interp = self.schedule.globs, self.interpreter
         own = lambda f, cls, name: getattr(f, "__func__", None) is getattr(cls, name)  # noqa: E731
         return (
-            count >= self.shortest_prompt
+            count >= (1 if globs.key_weights is not None else self.shortest_prompt)
             and self._whole is not None
             and globs.instructions is self._whole[0]
             and _edits(globs.instructions) == self._whole[1]
@@ -239,8 +241,8 @@ class MK_Generator(Generator):
             and globs.residual_scale == 1.0
             and globs.residual_acc is not None
             and globs.hidden_states.is_cuda
-            and count <= globs.k_cache.shape[2]
-            and count <= globs.rope_cos.shape[0]
+            and position + count <= globs.k_cache.shape[2]
+            and position + count <= globs.rope_cos.shape[0]
             and own(self.run, MK_Generator, "run")
             and own(self._step, MK_Generator, "_step")
             and isinstance(interp, LatencyMK_Interpreter)
@@ -253,43 +255,183 @@ class MK_Generator(Generator):
     # take 1,153 us at once and 1,290 us as steps (1B widths, 16 layers), 743 and 1,033 us (8B widths, 4 layers).
     shortest_prompt = 2
 
-    def _prompt(self, ids: Tensor) -> Tensor:
-        globs, count = self.schedule.globs, ids.shape[1]
+    def _prompt(self, ids: Tensor, first: int = 0, globs=None) -> Tensor:
+        """``globs``: those of another schedule over the same model's weights and caches."""
+        globs, count = globs or self.schedule.globs, ids.shape[1]
         if getattr(self, "_graph", None) is not None:  # (a captured step takes any whole numbers, from any device)
             ids = ids.to(self._graph_tok)
+        watched = 0 if globs.key_weights is None else min(self.observed or count, count)  # the last of them
         for a in range(0, count, self.prompt_portion):
             b = min(count, a + self.prompt_portion)
             try:
                 post = self.model.model.embed_tokens(BatchState(input_ids=ids[:, a:b]))
                 hidden = post.hidden_states.reshape(b - a, -1).to(globs.hidden_states)
-                self.last_call = self.interpreter.prompt(globs, hidden, a, b == count)
+                seen = max(0, b - max(a, count - watched)) if watched else 0
+                extra = {"observed": seen} if seen else {}
+                self.last_call = self.interpreter.prompt(globs, hidden, first + a, b == count, **extra)
             except torch.OutOfMemoryError:  # steps need no workspace
-                return self._steps(ids, a)
+                if watched or globs is not self.schedule.globs:
+                    raise
+                return self._steps(ids, a, first)
         globs.hidden_states[:] = hidden[-1]
         if globs.pos_id_device is not None:
-            globs.pos_id_device.fill_(count - 1)
+            globs.pos_id_device.fill_(first + count - 1)
         token = torch.argmax(globs.logits, dim=-1).reshape(1)
         if globs.argmax_out is not None:
             globs.argmax_out.copy_(token)
         return token
 
-    def prefill(self, prompt_ids: Tensor) -> Tensor:
+    def prefill(self, prompt_ids: Tensor, position: int = 0) -> Tensor:
         """Fill the KV cache with a prompt; returns the first generated token ``[1]``.
 
         The reference prefills with its torch model (scripts/generate.py:125-137).  Here the tokens go
         through the layers at once, in portions, or where that does not apply (``_takes_prompts``) or memory
-        for a portion is lacking, through the decode kernel one at a time.
+        for a portion is lacking, through the decode kernel one at a time.  ``position``: of the first token, behind
+        what the cache holds of the sequence (a later turn of a chat); 0 starts a sequence.
         """
         ids = prompt_ids.reshape(1, -1)
-        if self._takes_prompts(ids.shape[1]):
-            return self._prompt(ids)
-        return self._steps(ids, 0)
+        globs = self.schedule.globs
+        if position == 0:
+            self._start_sequence()
+        at_once = self._takes_prompts(ids.shape[1], position)
+        if globs.key_weights is not None and not at_once:
+            raise ValueError("only prompts that go through the layers at once are observed")
+        return self._prompt(ids, position) if at_once else self._steps(ids, 0, position)
 
-    def _steps(self, ids: Tensor, first: int) -> Tensor:
+    def _steps(self, ids: Tensor, done: int, first: int = 0) -> Tensor:
         out = None
-        for pos in range(first, ids.shape[1]):
-            out = self.run(ids[:, pos : pos + 1], pos_id=pos)
+        for i in range(done, ids.shape[1]):
+            out = self.run(ids[:, i : i + 1], pos_id=first + i)
         return out.reshape(-1)
+
+    # -- long caches cut to the keys that are looked at ----------------------- #
+    observed: int | None = None
+    evicted = 0
+
+    def observe(self, window: int | None = None) -> None:
+        """From the next prompt on keep the softmax weight that its last ``window`` tokens (None: all of them) give each
+        cached key, per layer and key/value head (``globs.key_weights``), for :meth:`evict`.  Of decoded tokens none is
+        kept.  Call it before ``enable_cuda_graph``.
+        """
+        globs = self.schedule.globs
+        if globs.batch_size != 1 or globs.tp is not None or self._whole is None or not globs.hidden_states.is_cuda:
+            raise ValueError("the attention of one sequence on one GPU is observed, with the whole model's instructions")
+        if window is not None and window < 1:
+            raise ValueError(f"a window of {window} tokens")
+        if getattr(self, "_graph", None) is not None:
+            raise ValueError("observe before enable_cuda_graph: the captured step reads the rotation tables of this call")
+        if globs.key_weights is None:
+            L, _, T, Hkv, _ = globs.k_cache.shape
+            globs.key_weights = torch.zeros(L, Hkv, T, dtype=torch.float32, device=globs.k_cache.device)
+            # rows and positions part ways with the first eviction: tables by row, of this generator alone
+            globs.rope_cos, globs.rope_sin = globs.rope_cos.clone(), globs.rope_sin.clone()
+        self.observed = window
+
+    def _start_sequence(self) -> None:
+        globs = self.schedule.globs
+        if globs.key_weights is not None:
+            globs.key_weights.zero_()
+            self._turn_to(0)
+
+    def _turn_to(self, evicted: int) -> None:
+        """Rows of the cache from the next one on are ``evicted`` positions further than they say."""
+        globs, model = self.schedule.globs, self.model
+        if evicted == self.evicted:
+            return
+        tables = (model.model.rope_cos, model.model.rope_sin)
+        if evicted:
+            tables = build_rope_tables(model.config, globs.rope_cos.shape[0], model.extra_config.interleave_rope, evicted)
+        globs.rope_cos.copy_(tables[0])
+        globs.rope_sin.copy_(tables[1])
+        self.evicted = evicted
+
+    def evict(self, length: int, keep: int, sinks: int = 4, recent: int = 64) -> int:
+        """Cut a cache of ``length`` rows to ``keep`` in place; returns the rows that it holds then, which is the position to
+        go on from (``prompt_len`` of :meth:`generate`).
+
+        Every layer and key/value head keeps its first ``sinks`` rows, its last ``recent``, and of the others those that the
+        observed prompts (:meth:`observe`) gave the most weight.  Keys stay rotated by the position they had, and tokens to come
+        are rotated by theirs.
+        """
+        globs = self.schedule.globs
+        if globs.key_weights is None:
+            raise ValueError("evict needs observed prompts (observe)")
+        if not 0 <= length <= globs.k_cache.shape[2]:
+            raise ValueError(f"{length} rows of a cache of {globs.k_cache.shape[2]}")
+        if not (keep >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= keep):
+            raise ValueError(f"{sinks} first and {recent} last of {keep} rows")
+        if length <= keep:
+            return length
+        ops = get_mk_module(name="mk_sequences")
+        weights = globs.key_weights.unsqueeze(1)
+        k, v = (c[:, :1] for c in (globs.k_cache, globs.v_cache))
+        rows = ops.select_rows(weights, length, keep=keep, sinks=sinks, recent=recent, kept=weights)
+        ops.move_rows(k, v, rows, length)
+        weights[..., keep:length] = 0
+        self._turn_to(self.evicted + length - keep)
+        return keep
+
+    # -- beam search: the sequences of a batched launch are the beams ----------- #
+    def beam_search(self, prompts, beams: int | None = None, ntok: int = 100, **kw) -> BeamResult:
+        """The best continuations of one prompt, or of several at once, by beam search (``beams.beam_search`` has the
+        arguments).  The schedule's batch is prompts times beams.
+        """
+        return beam_search(self, prompts, beams, ntok, **kw)
+
+    def beam_limits(self) -> tuple[int, int]:
+        """Sequences and positions that there are."""
+        globs = self.schedule.globs
+        if globs.batch_size < 2 or not globs.hidden_states.is_cuda or self.skip_mk or self.skip_rest or getattr(self, "_graph", None) is not None:
+            raise ValueError("beams need a batched schedule (LatencyScheduleOptions(batch_size=...)) whose steps are whole and not captured")
+        return globs.batch_size, min(globs.k_cache.shape[2], globs.rope_cos.shape[0])
+
+    def start_beams(self, prompts: list[Tensor], beams: int) -> Tensor:
+        """Each prompt through the layers once, its cache rows handed to its beams; returns logits ``[prompts, vocab]``."""
+        globs, ops = self.schedule.globs, get_mk_module(name="mk_sequences")
+        device = globs.hidden_states.device
+        single = make_globals(self.model, skip_attn_reduction=True, max_attn_partitions=1)
+        single.instructions = torch.zeros(1, 1, 32, dtype=torch.int32, device=device)  # (a prompt runs none)
+        logits = globs.logits.new_empty(len(prompts), globs.vocab_size)
+        slots = torch.arange(globs.k_cache.shape[1], dtype=torch.int32, device=device)
+        self._positions_before = globs.pos_id_device
+        globs.pos_id_device = torch.zeros(globs.batch_size, dtype=torch.int32, device=device)
+        for p in reversed(range(len(prompts))):  # (prompts go to slot 0: the first one's place)
+            ids = prompts[p]
+            self._prompt(ids.reshape(1, -1).to(device), globs=single)
+            logits[p] = single.logits
+            parents = torch.where(slots // beams == p, 0, slots)
+            ops.reorder_slots([globs.k_cache, globs.v_cache], parents.int(), dim=1, lengths=torch.full_like(slots, ids.numel()))
+        return logits
+
+    def step_beams(self, tokens: Tensor, positions: Tensor) -> Tensor:
+        """One token of every beam at its position (int32); logits ``[beams, vocab]``, there until the next step.
+
+        Sequences of the batch that are no beam decode token 0 at position 0.
+        """
+        globs, n = self.schedule.globs, tokens.numel()
+        ids = torch.zeros(globs.batch_size, dtype=torch.long, device=tokens.device)
+        ids[:n] = tokens
+        post = self.model.model.embed_tokens(BatchState(input_ids=ids.view(-1, 1)))
+        globs.hidden_states[:] = post.hidden_states.reshape(globs.hidden_states.shape)
+        self.fill()
+        globs.pos_id_device[:n] = positions
+        self.last_call = self.interpreter.interpret(globs)
+        return globs.logits[:n]
+
+    def reorder_beams(self, parents: Tensor, first: int, lengths: Tensor) -> None:
+        """Every beam goes on from its parent's rows; rows below ``first`` are alike."""
+        globs, n = self.schedule.globs, parents.numel()
+        slots = globs.k_cache.shape[1]
+        if n < slots:
+            everyone = torch.arange(slots, dtype=torch.int32, device=parents.device)
+            everyone[:n] = parents
+            parents, lengths = everyone, torch.cat([lengths, lengths.new_zeros(slots - n)])
+        get_mk_module(name="mk_sequences").reorder_slots([globs.k_cache, globs.v_cache], parents, dim=1, first=first, lengths=lengths)
+
+    _positions_before = None
+
+    def end_beams(self) -> None:
+        self.schedule.globs.pos_id_device = self._positions_before
 
     def step(self, tokens: list[int], position: int, want: list[int], slot: int = 0) -> Tensor:
         """Feed a sequence's next ``tokens`` (the first one at ``position``) and return fp32 logits
@@ -412,10 +554,65 @@ class Hybrid_Generator(MK_Generator):
         self.check()
         return out
 
-    def prefill(self, prompt_ids: Tensor) -> Tensor:
-        """Run a prompt from position 0; returns the first generated token ``[1]``."""
+    def prefill(self, prompt_ids: Tensor, position: int = 0) -> Tensor:
+        """Run a prompt from ``position`` on (0 starts a sequence); returns the first generated token ``[1]``."""
         n = prompt_ids.numel()
-        return self.feed(prompt_ids, 0, [n - 1]).argmax(dim=-1)
+        return self.feed(prompt_ids, position, [n - 1]).argmax(dim=-1)
+
+    def observe(self, window: int | None = None) -> None:
+        raise NotImplementedError("layer-list models' caches are not cut: their windows, chunks and latents bound them")
+
+    # -- beam search: beams are slots that take turns ---------------------------- #
+    def beam_limits(self) -> tuple[int, int]:
+        if getattr(self, "_graph", None) is not None or self.skip_mk or self.skip_rest:
+            raise ValueError("beams need whole steps that are not captured")
+        return self.model.slots.count - len(self.model.slots), self.model.max_len()
+
+    _beam_slots: list[int] = []
+
+    def start_beams(self, prompts: list[Tensor], beams: int) -> Tensor:
+        """Each prompt once, its state handed to its beams' slots, which are taken from the pool until ``end_beams``."""
+        model, logits = self.model, []
+        self._slot_before, self._beam_slots = self.slot, []
+        for _ in range(len(prompts) * beams):
+            self._beam_slots.append(model.slots.allocate())
+        self._slot_of = torch.tensor(self._beam_slots, dtype=torch.int32, device=model.device)
+        for p, ids in enumerate(prompts):
+            self.slot = self._beam_slots[p * beams]
+            logits.append(self.feed(ids, 0, [ids.numel() - 1])[0])
+        row = torch.arange(len(self._beam_slots), dtype=torch.int32, device=model.device)
+        lengths = torch.tensor([p.numel() for p in prompts], dtype=torch.int32, device=model.device).repeat_interleave(beams)
+        self.reorder_beams(row // beams * beams, 0, lengths)
+        self._beam_logits = torch.empty(row.numel(), model.config.vocab_size, device=model.device)
+        return torch.stack(logits)
+
+    def step_beams(self, tokens: Tensor, positions: Tensor) -> Tensor:
+        globs, before = self.schedule.globs, self.schedule.globs.pos_id_device
+        try:
+            for b, slot in enumerate(self._beam_slots):
+                globs.tokens[:1].copy_(tokens[b : b + 1])
+                globs.slot, globs.pos_id_device = slot, positions[b : b + 1]
+                self.last_call = self.interpreter.interpret(globs)
+                self._beam_logits[b] = globs.logits
+        finally:
+            globs.pos_id_device = before
+        return self._beam_logits
+
+    def reorder_beams(self, parents: Tensor, first: int, lengths: Tensor) -> None:
+        """(A ring may have overwritten rows below ``first`` in one beam and not in another: all rows go.)"""
+        mine = self._slot_of.long()
+        everyone = torch.arange(self.model.slots.count, dtype=torch.int32, device=self.model.device)
+        rows = torch.zeros_like(everyone)
+        everyone[mine] = self._slot_of[parents.long()]
+        rows[mine] = lengths
+        self.model.state.reorder(everyone, rows)
+
+    def end_beams(self) -> None:
+        for slot in self._beam_slots:
+            self.model.slots.free(slot)
+        if self._beam_slots:
+            self.slot = self._slot_before
+        self._beam_slots, self._beam_logits = [], None
 
 
 class TP_MK_Generator(MK_Generator):

@@ -116,6 +116,8 @@ class BaseGlobals:
         self.batch_size: int = 1
         self.pos_ids: list[int] | None = None
         self.normed_states: Tensor | None = None
+        # fp32 [L, Hkv, T]: softmax weight that observed prompts have given sequence 0's cached keys
+        self.key_weights: Tensor | None = None
 
     def residual_stream(self) -> Tensor:
         """The residual stream after a launch as fp32 ``[H]``: embedding + accumulated outputs.

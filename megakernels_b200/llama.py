@@ -149,15 +149,15 @@ def rope_inverse_frequencies(config: LlamaConfig) -> Tensor:
     return torch.where(medium, blended, scaled)
 
 
-def build_rope_tables(config: LlamaConfig, num_positions: int, interleave: bool):
-    """cos/sin tables ``[num_positions, head_dim]`` in fp32.
+def build_rope_tables(config: LlamaConfig, num_positions: int, interleave: bool, first: int = 0):
+    """cos/sin tables ``[num_positions, head_dim]`` in fp32, of positions ``first`` on.
 
     Non-interleaved layout is ``cat(freqs, freqs)``; the interleaved layout
     repeats each frequency on adjacent columns ``(2i, 2i+1)``, which is what
     the column permutation of megakernels/llama.py:453-465 produces.
     """
     inv_freq = rope_inverse_frequencies(config)
-    pos = torch.arange(num_positions, dtype=torch.float32)
+    pos = torch.arange(first, first + num_positions, dtype=torch.float32)
     freqs = (inv_freq[:, None].float() @ pos[None, :].float()).transpose(0, 1)
     emb = torch.cat((freqs, freqs), dim=-1)
     cos, sin = emb.cos(), emb.sin()

@@ -118,6 +118,13 @@ class MkbPrompt(ctypes.Structure):
         ("hidden", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
+        ("key_weights", ctypes.c_void_p),
+        ("weights_layer", ctypes.c_int64),
+        ("weights_head", ctypes.c_int64),
+        ("observed", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("weights_workspace", ctypes.c_void_p),
+        ("weights_workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -162,6 +169,8 @@ def load_library() -> ctypes.CDLL:
     lib.mkb_prompt.restype = ctypes.c_int
     lib.mkb_prompt_bytes.argtypes = [ctypes.POINTER(MkbGlobals), ctypes.c_int32]
     lib.mkb_prompt_bytes.restype = ctypes.c_size_t
+    lib.mkb_prompt_weights_bytes.argtypes = [ctypes.POINTER(MkbGlobals), *[ctypes.c_int32] * 3]
+    lib.mkb_prompt_weights_bytes.restype = ctypes.c_size_t
     lib.mkb_sync_status.argtypes = [
         ctypes.POINTER(MkbGlobals),
         ctypes.c_void_p,
@@ -488,12 +497,13 @@ def mk_llama(
     return g
 
 
-def mk_llama_prompt(*args, hidden, pos0, want_logits, stream=None, **kw):
+def mk_llama_prompt(*args, hidden, pos0, want_logits, key_weights=None, observed=0, stream=None, **kw):
     """Enqueue a prompt's tokens at once (``mkb_prompt``); other arguments as :func:`mk_llama`.
 
     ``hidden`` holds their embeddings ``[tokens, H]``, the first of position ``pos0``; ``pos_id`` is the
     last one's position.  Keys and values go to the caches, the last token's logits and what the layers added to its
-    embedding (``want_logits``) to ``logits`` and ``residual_acc``.
+    embedding (``want_logits``) to ``logits`` and ``residual_acc``.  ``key_weights`` (float32 ``[layers, kv_heads, positions]``)
+    receives, added, the softmax weight that the queries of the last ``observed`` tokens give each key of sequence 0.
     """
     lib = load_library()
     if kw.get("residual_acc") is None and kw.get("tp") is None:
@@ -512,6 +522,18 @@ def mk_llama_prompt(*args, hidden, pos0, want_logits, stream=None, **kw):
     if stream != torch.cuda.current_stream(hidden.device):
         hidden.record_stream(stream)
     p.workspace = workspace.data_ptr()
+    if key_weights is not None and observed:
+        if tuple(key_weights.shape) != (g.num_layers, g.num_kv_heads, g.kv_max_len) or key_weights.stride(2) != 1:
+            raise ValueError(f"key_weights must be [{g.num_layers}, {g.num_kv_heads}, {g.kv_max_len}], its rows contiguous")
+        _check_tensor("key_weights", key_weights[0, 0], torch.float32)
+        p.key_weights, p.observed = key_weights.data_ptr(), int(observed)
+        p.weights_layer, p.weights_head = key_weights.stride(0), key_weights.stride(1)
+        p.weights_workspace_bytes = lib.mkb_prompt_weights_bytes(ctypes.byref(g), p.tokens, pos0, int(observed))
+        with torch.cuda.stream(stream):
+            weights_workspace = torch.empty(max(p.weights_workspace_bytes, 1), dtype=torch.uint8, device=hidden.device)
+        p.weights_workspace = weights_workspace.data_ptr()
+        if stream != torch.cuda.current_stream(hidden.device):
+            key_weights.record_stream(stream)
     rc = lib.mkb_prompt(ctypes.byref(g), ctypes.byref(p), ctypes.c_void_p(_stream_handle(stream)))
     if rc != 0:
         raise MegakernelError(rc, lib.mkb_last_error().decode())

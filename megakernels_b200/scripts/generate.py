@@ -55,6 +55,15 @@ class ScriptConfig:
     attn_partitions: int = 0
     coalesce_o_proj: bool = False
     merge_in_last_partial: bool = False
+    # beam search: this many beams; eos < 0: none
+    beams: int = 1
+    eos: int = -1
+    length_penalty: float = 0.0
+    # > 0: behind the prompt the cache is cut to this many rows, by the attention of the prompt's last `window` tokens
+    keep: int = 0
+    window: int = 64
+    sinks: int = 4
+    recent: int = 64
 
     def finalize(self):
         if self.mode != "mk":
@@ -66,6 +75,10 @@ class ScriptConfig:
         if self.setting not in BUILDER_MAP:
             raise SystemExit(f"unknown setting {self.setting!r}; available: {sorted(BUILDER_MAP)}")
         assert self.batch_size == 1, "the latency megakernel decodes one sequence"
+        if self.beams < 1 or self.keep < 0:
+            raise SystemExit("beams is at least 1, keep at least 0")
+        if self.beams > 1 and (self.keep or self.noops or self.skip_mk or self.skip_rest):
+            raise SystemExit("beams go with neither keep nor skipped work")
 
     def once(self):
         self.num_warmup, self.num_iters = 0, 1
@@ -109,7 +122,7 @@ def main(config: ScriptConfig):
     extra = ExtraModelConfig(
         interleave_rope=config.interleave_rope,
         max_len_override=config.max_len_override,
-        max_batch_size=config.batch_size,
+        max_batch_size=config.batch_size * config.beams,
     )
     dtype = getattr(torch, config.dtype)
     family = family_of_preset(config.model)
@@ -140,11 +153,11 @@ def main(config: ScriptConfig):
     options = None  # the setting's defaults
     if model.setting == "latency":
         n_part = config.attn_partitions or pick_num_attention_partitions(
-            prompt_len, config.ntok, model.device, model.num_kv_heads()
+            min(prompt_len, config.keep or prompt_len), config.ntok, model.device, model.num_kv_heads()
         )
         options = LatencyScheduleOptions(
             num_attention_partitions=n_part, coalesce_o_proj=config.coalesce_o_proj,
-            merge_in_last_partial=config.merge_in_last_partial,
+            merge_in_last_partial=config.merge_in_last_partial, batch_size=config.beams,
         )
     gen = make_generator(
         model,
@@ -156,8 +169,15 @@ def main(config: ScriptConfig):
         skip_mk=config.skip_mk,
         skip_rest=config.skip_rest,
     )
+    if config.beams > 1:
+        return search(gen, prompt, config)
+    if config.keep:
+        gen.observe(config.window)
     first = gen.prefill(prompt)
     gen.check()
+    if config.keep:
+        prompt_len = gen.evict(prompt_len, config.keep, config.sinks, config.recent)
+        print(f"Rows of the cache behind the prompt: {prompt_len}")
     if config.noops:
         gen.replace_with_noops()
 
@@ -187,6 +207,27 @@ def main(config: ScriptConfig):
     print(f"Fwd per second: {fwd_per_second:.2f}")
     print(f"Tokens per second: {config.batch_size * fwd_per_second:.2f}")
     return output_tokens
+
+
+def search(gen, prompt: torch.Tensor, config: ScriptConfig) -> torch.Tensor:
+    """Beam search, timed as a whole: the prompt is part of it."""
+    times = []
+    for _ in range(config.num_warmup + config.num_iters):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        found = gen.beam_search(prompt, config.beams, config.ntok, eos=config.eos if config.eos >= 0 else None, length_penalty=config.length_penalty)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end) / 1000)
+    gen.check()
+    timed = times[config.num_warmup :]
+    elapsed, steps = sum(timed) / len(timed), found.tokens.shape[-1]
+    print(f"Average time: {elapsed * 1000:.2f}ms")
+    if config.tokens:
+        for tokens, length, score in zip(found.tokens[0].cpu(), found.lengths[0].tolist(), found.scores[0].tolist()):
+            print(f"Score {score:.4f}, output ids: ", tokens[:length])
+    print(f"Tokens per second: {steps / elapsed:.2f}")
+    return found.tokens[0]
 
 
 if __name__ == "__main__":

@@ -89,6 +89,7 @@ class HybridState:
         self.input_terms: dict[int, Tensor] = {}  # [slots, 2, width], in turn by the position's parity
         self.projected: dict[int, Tensor] = {}  # the projections' convolution: [slots, taps - 1, rows]
         self.projected_terms: dict[int, Tensor] = {}  # [slots, rows]
+        self.by_head: set[int] = set()  # runs whose keys and values lie [slots, heads, rows, ...], not [slots, rows, ...]
         layers = config.run_layers
         f32 = lambda *shape: torch.zeros(slots, *shape, device=device, dtype=torch.float32)  # noqa: E731
         for i, layer in enumerate(layers):
@@ -103,6 +104,7 @@ class HybridState:
                 elif m.kind == "attention":  # (a head's rows together: its splits are runs of memory)
                     cache = lambda n: torch.zeros(slots, m.kv_heads, rows.total, n, device=device, dtype=dtype)  # noqa: E731
                     self.keys[i], self.values[i] = cache(m.dim), cache(m.vdim)
+                    self.by_head.add(i)
                 else:
                     cache = lambda *shape: torch.zeros(slots, rows.total, m.kv_heads, *shape, device=device, dtype=dtype)  # noqa: E731
                     self.keys[i], self.values[i] = cache(2, m.dim), cache(m.vdim)
@@ -110,6 +112,23 @@ class HybridState:
                 self.inputs[i], self.input_terms[i] = f32(max(layer.canon_taps - 1, 1), config.width), f32(2, config.width)
             if getattr(m, "conv_taps", 0):
                 self.projected[i], self.projected_terms[i] = f32(max(m.conv_taps - 1, 1), m.in_rows), f32(m.in_rows)
+
+    def reorder(self, parents: Tensor, lengths: Tensor) -> None:
+        """Every slot takes its parent's state, all at once and in place: ``parents`` int32 ``[slots]`` on the device (a slot's
+        own number: it stays), ``lengths`` int32 ``[slots]``: positions that a slot's sequence has, all rows of longer rings."""
+        from megakernels_b200.mk import get_mk_module
+
+        ops = get_mk_module(name="mk_sequences")
+        whole = [t for d in (self.matrices, self.inputs, self.input_terms, self.projected, self.projected_terms) for t in d.values()]
+        caches = lambda runs: [t for i in runs for t in (self.keys[i], self.values.get(i)) if t is not None]  # noqa: E731
+        by_head = [t.transpose(0, 1) for t in caches(self.by_head)]
+        by_row = caches(i for i in self.keys if i not in self.by_head)
+        if whole:
+            ops.reorder_slots(whole, parents)
+        if by_row:
+            ops.reorder_slots(by_row, parents, lengths=lengths)
+        if by_head:
+            ops.reorder_slots(by_head, parents, dim=1, lengths=lengths)
 
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size()

@@ -1,0 +1,374 @@
+"""Beam search and the eviction of cache rows, through the generators and the script."""
+
+import importlib
+import math
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from megakernels_b200.beams import beam_search
+from megakernels_b200.demos.latency.scheduler import LatencyScheduleOptions
+from megakernels_b200.dispatch import make_generator
+from megakernels_b200.llama import LlamaConfig, LlamaForCausalLM, build_rope_tables
+from megakernels_b200.model_types import ExtraModelConfig
+from megakernels_b200.scripts.generate import main, parse_cli
+from tests.oracle_utils import seeded_tokens
+
+VOCAB = 4096
+CONFIGS = {
+    "1b": lambda **kw: LlamaConfig.llama_3_2_1b(**{"num_hidden_layers": 2, "vocab_size": VOCAB, **kw}),
+    "8b": lambda **kw: LlamaConfig.llama_3_1_8b(**{"num_hidden_layers": 2, "vocab_size": VOCAB, **kw}),
+}
+
+
+def llama(shape, batch, max_len=300, seed=0, **kw):
+    extra = ExtraModelConfig(interleave_rope=True, max_len_override=max_len, max_batch_size=batch)
+    return LlamaForCausalLM.from_random(CONFIGS[shape](**kw), extra, device="cuda:0", seed=seed, std=0.05, draw_on="device")
+
+
+def prompt(n, seed):
+    return torch.tensor(seeded_tokens(VOCAB, n, seed=seed)).cuda()
+
+
+# ---- on the host ------------------------------------------------------------------------------------ #
+def test_command_line():
+    cfg = parse_cli(["beams=4", "eos=7", "length_penalty=0.5"])
+    assert (cfg.beams, cfg.eos, cfg.length_penalty, cfg.keep) == (4, 7, 0.5, 0)
+    assert parse_cli(["keep=512", "window=32", "recent=9"]).window == 32
+    for wrong in (["beams=0"], ["keep=-1"], ["beams=2", "keep=100"], ["beams=2", "noops=true"]):
+        with pytest.raises(SystemExit):
+            parse_cli(wrong)
+
+
+def test_rope_tables_from_a_position():
+    cfg = CONFIGS["1b"]()
+    for interleave in (True, False):
+        whole = build_rope_tables(cfg, 300, interleave)
+        part = build_rope_tables(cfg, 100, interleave, first=200)
+        assert all(torch.equal(w[200:], p) for w, p in zip(whole, part))
+
+
+class NoGenerator:
+    """A generator that has sequences, and may not be asked to run them."""
+
+    model = SimpleNamespace(config=SimpleNamespace(vocab_size=50))
+
+    def beam_limits(self):
+        return 8, 100
+
+
+@pytest.mark.parametrize("prompts,kw,said", [
+    ([], {}, "prompts"), ([torch.zeros(0)], {}, "prompts"), ([torch.zeros(3)], dict(beams=0), "beams"), ([torch.zeros(3)], dict(beams=9), "beams"),
+    ([torch.zeros(3)] * 3, dict(beams=3), "beams"), ([torch.zeros(3)] * 9, {}, "beams"), (torch.zeros(3), dict(ntok=0), "tokens"), (torch.zeros(3), dict(ntok=99), "positions"),
+    (torch.zeros(3), dict(eos=50, ntok=9), "eos"), (torch.zeros(3), dict(eos=-1, ntok=9), "eos"),
+])
+def test_refused_searches(prompts, kw, said):
+    with pytest.raises(ValueError, match=said):
+        beam_search(NoGenerator(), prompts, **kw)
+
+
+# ---- beam search ------------------------------------------------------------------------------------ #
+class Plain:
+    """A generator's steps with the selection, the tables and the reordering in plain torch."""
+
+    def __init__(self, gen, caches, slot_dim):
+        self.gen, self.caches, self.slot_dim = gen, caches, slot_dim
+
+    def search(self, prompts, beams, ntok, eos):
+        gen, G = self.gen, len(prompts)
+        logits = gen.start_beams(prompts, beams).double()
+        try:
+            p = torch.log_softmax(logits, dim=-1)
+            scores, tokens = torch.sort(p, dim=1, descending=True, stable=True)
+            scores, tokens = scores[:, :beams].float(), tokens[:, :beams]
+            table, done = [[[int(t)] for t in row] for row in tokens], tokens == (-1 if eos is None else eos)
+            at = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device="cuda").repeat_interleave(beams)
+            for _ in range(1, ntok):
+                p = torch.log_softmax(gen.step_beams(tokens.reshape(-1).int(), at).double(), dim=-1).view(G, beams, -1)
+                at = at + 1
+                total = scores.double().unsqueeze(-1) + p
+                if eos is not None:
+                    total[done] = -math.inf
+                    total[..., eos] = torch.where(done, scores.double(), total[..., eos])
+                best, where = torch.sort(total.flatten(1), dim=1, descending=True, stable=True)
+                scores, where = best[:, :beams].float(), where[:, :beams]
+                parents, tokens = where // p.shape[-1], where % p.shape[-1]
+                done = done.gather(1, parents) | (tokens == (-1 if eos is None else eos))
+                table = [[table[g][int(b)] + [int(t)] for b, t in zip(parents[g], tokens[g])] for g in range(G)]
+                rows = (parents + torch.arange(G, device="cuda").unsqueeze(1) * beams).reshape(-1)
+                for c in self.caches():  # (whole slots, also what nobody reads)
+                    mine = c.narrow(self.slot_dim, 0, G * beams)
+                    mine.copy_(mine.index_select(self.slot_dim, rows))
+            return table, scores
+        finally:
+            gen.end_beams()
+
+
+def check_search(gen, plain, prompts, beams, ntok, eos=None, penalty=0.0):
+    want, scores = plain.search(prompts, beams, ntok, eos)
+    found = gen.beam_search(prompts if len(prompts) > 1 else prompts[0], beams, ntok, eos=eos, length_penalty=penalty, check_interval=4)
+    gen.check()
+    n = found.tokens.shape[-1]
+    for g in range(len(prompts)):
+        lengths = [row.index(eos) + 1 if eos in row else ntok for row in want[g]]
+        ranks = [s / length**penalty for s, length in zip(scores[g].tolist(), lengths)]
+        order = sorted(range(beams), key=lambda b: (-ranks[b], b))
+        assert found.lengths[g].tolist() == [lengths[b] for b in order]
+        for b, tokens in zip(order, found.tokens[g].tolist()):
+            assert tokens == want[g][b][:n] and all(t == eos for t in want[g][b][n:])
+        # (a step's log-probabilities are within the selection's own bound of the plain ones, and scores are sums of them)
+        bound = ntok * ((VOCAB / 32 + 48) * 2.0**-24 + scores[g].abs().max().item() * 2.0**-23)
+        assert (found.scores[g].double() - scores[g][order].double()).abs().max() <= bound
+    return found
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,beams,lengths,ntok", [("1b", 4, [30], 20), ("1b", 8, [5], 9), ("1b", 2, [17, 40, 3], 12), ("8b", 4, [20, 9, 33], 10), ("8b", 16, [12], 6)])
+def test_llama_beams_equal_plain_beams(shape, beams, lengths, ntok):
+    """Tokens, lengths and order equal to a search whose selection and moves are plain torch, on the same steps."""
+    batch = beams * len(lengths)
+    model = llama(shape, batch)
+    gen = make_generator(model, LatencyScheduleOptions(num_attention_partitions=2, batch_size=batch, merge_in_last_partial=True))
+    prompts = [prompt(n, seed=n) for n in lengths]
+    plain = Plain(gen, lambda: model.stacked_kv_cache, 1)
+    first = check_search(gen, plain, prompts, beams, ntok)
+    eos = int(first.tokens[0, 0, ntok // 2])  # a token that is taken: some beams end
+    ended = check_search(gen, plain, prompts, beams, ntok, eos=eos)
+    assert (ended.lengths < ntok).any()
+    check_search(gen, plain, prompts, beams, ntok, eos=eos, penalty=1.0)
+    assert gen.schedule.globs.pos_id_device is None
+
+
+@pytest.mark.gpu
+def test_first_beam_of_one_is_greedy_decoding():
+    """More slots than the search uses.  The batched kernel's logits and the single one's are within 2e-2 of the largest of the
+    oracle's each, so what is best to the one is within 4 times that of the best to the other."""
+    model = llama("1b", 5)
+    gen = make_generator(model, LatencyScheduleOptions(num_attention_partitions=2, batch_size=4))
+    ids = prompt(25, 3)
+    found = gen.beam_search(ids, 1, 12)
+    alone = make_generator(llama("1b", 1), LatencyScheduleOptions(num_attention_partitions=2))
+    alone.prefill(ids)
+    for i, token in enumerate(found.tokens[0, 0].tolist()):
+        logits = alone.schedule.globs.logits.float()
+        assert logits.max() - logits[token] <= 4 * 2e-2 * logits.abs().max()
+        alone.run(torch.tensor([[token]]).cuda(), 25 + i)
+    assert found.ranks[0, 0] == found.scores[0, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("family,name", [("torirax", "odd"), ("torirax", "ragged"), ("dumalix", "odd"), ("dumalix", "ragged"), ("dumalix", "groups")])
+def test_layer_list_beams_go_on_as_if_alone(tmp_path, family, name, dtype):
+    """Recurrent states, convolutions' inputs, rings that wrap, latents: a beam's score is that of its tokens fed as one sequence."""
+    utils = importlib.import_module(f"tests.{family}_utils")
+    raw = utils.MODELS[name]
+    path = utils.write_checkpoint(tmp_path / "ckpt", raw, utils.make_weights(raw))
+    gen = utils.load(path, dtype, portion=6, slots=8, max_len=90)
+    slots, vocab = gen.model.slots, raw["vocab"]
+    held = [slots.allocate(), slots.allocate()]  # somebody else's
+    ids = [torch.tensor(utils.tokens_for(raw, n, seed=n)) for n in (31, 9)]
+    mine = gen.step(ids[1].tolist(), 0, [8], slot=held[1])
+    for beams, which, ntok in ((3, ids, 25), (5, ids[1:], 12)):
+        found = gen.beam_search(which, beams, ntok)
+        gen.check()
+        assert len(slots) == 2
+        for g, start in enumerate(which):
+            for b in range(beams):
+                tokens = found.tokens[g, b].cpu()
+                whole = torch.cat([start, tokens])
+                logits = gen.step(whole[:-1].tolist(), 0, list(range(len(start) - 1, len(whole) - 1)), slot=held[0])
+                p = torch.log_softmax(logits.double().cpu(), dim=-1).gather(1, tokens.unsqueeze(1)).sum()
+                # decoding and prompts are each within the tolerance (of the logits' rms) of the plain model; none of some
+                # thousand logits is further off than five times that
+                tol = 2 * 5 * (utils.F32_TOL if dtype == torch.float32 else utils.BF16_TOL) * float(logits.pow(2).mean().sqrt()) * ntok
+                assert abs(float(found.scores[g, b]) - float(p)) <= tol
+        assert (found.scores[:, :-1] >= found.scores[:, 1:]).all()
+        assert len({tuple(t) for t in found.tokens[0].tolist()}) == beams
+    # the other sequence is where it was
+    assert torch.equal(gen.step(ids[1].tolist(), 0, [8], slot=held[0]), mine)
+    assert torch.equal(gen.step([3], 9, [0], slot=held[0]), gen.step([3], 9, [0], slot=held[1]))
+
+
+@pytest.mark.gpu
+def test_layer_list_states_move_as_torch_moves_them(tmp_path):
+    """Every tensor of a model that has all kinds of them, to the bit; rows behind a sequence stay."""
+    from tests import dumalix_utils, torirax_utils
+
+    for utils in (torirax_utils, dumalix_utils):
+        raw = utils.MODELS["odd"]
+        path = utils.write_checkpoint(tmp_path / utils.__name__ / "ckpt", raw, utils.make_weights(raw))
+        state = utils.load(path, torch.bfloat16, portion=6, slots=5, max_len=90).model.state
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        caches = [t for d in (state.keys, state.values) for t in d.values()]
+        others = [t for d in (state.matrices, state.inputs, state.input_terms, state.projected, state.projected_terms) for t in d.values()]
+        for t in caches + others:
+            t.normal_(generator=gen)
+        before = [t.clone() for t in caches + others]
+        parents, lengths = [3, 0, 2, 3, 1], [7, 20, 0, 90, 1]
+        state.reorder(torch.tensor(parents, dtype=torch.int32).cuda(), torch.tensor(lengths, dtype=torch.int32).cuda())
+        heads = {id(d[i]) for d in (state.keys, state.values) for i in state.by_head if i in d}
+        assert heads or utils is torirax_utils
+        for t, old in zip(caches + others, before):
+            want = old.clone()
+            for slot, parent in enumerate(parents):
+                if any(t is c for c in caches):
+                    rows = slice(0, min(lengths[parent], t.shape[2 if id(t) in heads else 1]))
+                    at = (slot, slice(None), rows) if id(t) in heads else (slot, rows)
+                    want[at] = old[(parent, *at[1:])]
+                else:
+                    want[slot] = old[parent]
+            assert torch.equal(t, want)
+
+
+@pytest.mark.gpu
+def test_searches_that_cannot_run():
+    model = llama("1b", 1)
+    gen = make_generator(model, LatencyScheduleOptions(num_attention_partitions=2))
+    with pytest.raises(ValueError, match="batched schedule"):
+        gen.beam_search(prompt(4, 0), 2, 3)
+    batched = make_generator(llama("1b", 2), LatencyScheduleOptions(num_attention_partitions=2, batch_size=2))
+    with pytest.raises(ValueError, match="one sequence"):
+        batched.observe()
+    with pytest.raises(ValueError, match="observed"):
+        gen.evict(10, 5)
+
+
+# ---- eviction ---------------------------------------------------------------------------------------- #
+def observed_generator(shape, max_len, window, portion=2048, **kw):
+    model = llama(shape, 1, max_len)
+    gen = make_generator(model, LatencyScheduleOptions(num_attention_partitions=2, **kw))
+    gen.prompt_portion = portion
+    gen.observe(window)
+    return model, gen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,count,window,portion", [("1b", 200, None, 2048), ("1b", 150, 40, 64), ("8b", 130, 7, 2048), ("1b", 90, 200, 50), ("8b", 33, 1, 2048)])
+def test_observed_prompts(shape, count, window, portion):
+    """Every observed query of every head shares out one; the first layer's weights against 64 bits; logits as without."""
+    model, gen = observed_generator(shape, count + 20, window, portion)
+    globs, ids = gen.schedule.globs, prompt(count, 5)
+    token = gen.prefill(ids)
+    gen.check()
+    seen, per = min(window or count, count), globs.num_attention_heads // globs.num_kv_heads
+    weights = globs.key_weights.clone()
+    assert not weights[..., count:].any()
+    # (each query's weights add up to one within the rounding of its sum)
+    assert (weights.double().sum(dim=-1) - seen * per).abs().max() <= seen * per * (count + 64) * 2.0**-23
+    logits, cache = globs.logits.clone(), globs.k_cache.clone()
+    # the first layer: its queries are rounded to bf16 from sums in another order, which moves a score by 2^-8 of its size
+    x = model.model.embed_tokens.embed_tokens.weight[ids].double()
+    x = x / (x.pow(2).mean(dim=-1, keepdim=True) + globs.rms_norm_eps).sqrt() * globs.attn_ln_weights[0].double()
+    D, Hq, Hkv = globs.head_dim, globs.num_attention_heads, globs.num_kv_heads
+    q = (x.bfloat16().double() @ globs.qkv_proj_weights[0, : Hq * D].double().T).view(count, Hq, D)
+    cos, sin = (t[:count, None].double() for t in (globs.rope_cos, globs.rope_sin))
+    turned = torch.stack([-q[..., 1::2], q[..., ::2]], dim=-1).flatten(-2)
+    q = q * cos + turned * sin
+    z = torch.einsum("thd,jhd->htj", q, globs.k_cache[0, 0, :count].double().repeat_interleave(per, dim=1)) * globs.attn_scale
+    z = z.masked_fill(torch.arange(count, device="cuda") > torch.arange(count, device="cuda").unsqueeze(1), -math.inf)
+    want = torch.softmax(z, dim=-1)[:, count - seen :].sum(dim=1).view(Hkv, per, count).sum(dim=1)
+    off = 2 * 2.0**-8 * float(z[z.isfinite()].abs().max())
+    assert ((weights[0, :, :count].double() - want).abs() <= want * (math.exp(off) - 1) + 1e-6).all()
+    # the same prompt again starts over; without observing nothing else changes
+    assert torch.equal(gen.prefill(ids), token) and torch.equal(globs.key_weights, weights)
+    plain = make_generator(llama(shape, 1, count + 20), LatencyScheduleOptions(num_attention_partitions=2))
+    plain.prompt_portion = portion
+    assert torch.equal(plain.prefill(ids), token)
+    assert torch.equal(plain.schedule.globs.logits, logits) and torch.equal(plain.schedule.globs.k_cache, cache)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,count,keep,sinks,recent,graph", [("1b", 200, 60, 4, 16, False), ("8b", 150, 149, 0, 0, False), ("1b", 120, 20, 4, 16, True), ("1b", 100, 100, 4, 8, False)])
+def test_evicted_cache_goes_on_as_one_laid_out_by_hand(shape, count, keep, sinks, recent, graph):
+    model, gen = observed_generator(shape, count + 20, 30)
+    globs = gen.schedule.globs
+    if graph:
+        gen.enable_cuda_graph()
+    first = token = gen.prefill(prompt(count, 6))
+    weights, k, v = globs.key_weights.clone(), globs.k_cache.clone(), globs.v_cache.clone()
+    rows = gen.evict(count, keep, sinks, recent)
+    assert rows == min(count, keep) and gen.evicted == count - rows
+    gone = count - rows
+    hand_k, hand_v, left = k.clone(), v.clone(), torch.zeros_like(weights)
+    for layer in range(2):
+        for g in range(globs.num_kv_heads):
+            w = weights[layer, g, :count].tolist()
+            middle = sorted(range(sinks, count - recent), key=lambda j: (-w[j], j))[: keep - sinks - recent]
+            stay = sorted([*range(sinks), *middle, *range(count - recent, count)]) if count > keep else list(range(count))
+            hand_k[layer, 0, :rows, g], hand_v[layer, 0, :rows, g] = k[layer, 0, stay, g], v[layer, 0, stay, g]
+            left[layer, g, :rows] = weights[layer, g, stay]
+    assert torch.equal(globs.k_cache, hand_k) and torch.equal(globs.v_cache, hand_v) and torch.equal(globs.key_weights, left)
+    got = []
+    for i in range(6):
+        token = gen.run(token.view(1, 1), rows + i).clone()
+        got.append((int(token), globs.logits.clone()))
+    gen.check()
+    # another generator, its cache filled by hand, its tables those of the true positions
+    other_model = llama(shape, 1, count + 20)
+    other = make_generator(other_model, LatencyScheduleOptions(num_attention_partitions=2))
+    og = other.schedule.globs
+    og.k_cache.copy_(hand_k)
+    og.v_cache.copy_(hand_v)
+    cos, sin = build_rope_tables(other_model.config, count + 20, True, first=gone)
+    og.rope_cos, og.rope_sin = cos.cuda(), sin.cuda()
+    token = first
+    for i in range(6):
+        token = other.run(token.view(1, 1), rows + i).clone()
+        assert int(token) == got[i][0] and torch.equal(og.logits, got[i][1])
+    # a later turn goes on behind it, is observed and evicted again
+    turn = prompt(5, 9)
+    gen.prefill(turn, position=rows + 6)
+    gen.check()
+    again = gen.evict(rows + 11, max(keep - 3, sinks + recent + 1), sinks, recent)
+    assert gen.evicted == count + 11 - again
+    # and a new sequence starts as if there had been none
+    fresh = make_generator(llama(shape, 1, count + 20), LatencyScheduleOptions(num_attention_partitions=2))
+    ids = prompt(40, 12)
+    assert torch.equal(gen.prefill(ids), fresh.prefill(ids)) and gen.evicted == 0
+    assert torch.equal(globs.logits, fresh.schedule.globs.logits)
+
+
+@pytest.mark.gpu
+def test_tokens_observed_one_at_a_time():
+    """A prompt cut into single tokens is weighed as it is at once.  Queries and keys of other products differ by the last bit of bf16 here and
+    there: single weights by a few hundredths, a query's sum only by the rounding of its own terms."""
+    model, gen = observed_generator("1b", 80, None)
+    ids = prompt(40, 2)
+    gen.prefill(ids)
+    whole = gen.schedule.globs.key_weights.clone()
+    gen.prefill(ids[:30])
+    for i in range(30, 40):
+        gen.prefill(ids[i : i + 1], position=i)
+    gen.check()
+    parts = gen.schedule.globs.key_weights
+    assert (parts.double().sum(dim=-1) - whole.double().sum(dim=-1)).abs().max() <= 2 * 40 * 4 * (40 + 64) * 2.0**-23
+    assert (parts - whole).abs().max() <= 0.05 * whole.max()
+
+
+@pytest.mark.gpu
+def test_observing_needs_whole_prompts():
+    model, gen = observed_generator("1b", 64, 8)
+    gen.replace_with_noops()
+    with pytest.raises(ValueError, match="observed"):
+        gen.prefill(prompt(10, 1))
+    model, gen = observed_generator("1b", 64, 8)
+    for length, keep, sinks, recent in ((65, 10, 1, 1), (-1, 10, 1, 1), (50, 0, 0, 0), (50, 5, 4, 2), (50, 5, -1, 2)):
+        with pytest.raises(ValueError):
+            gen.evict(length, keep, sinks, recent)
+    with pytest.raises(ValueError, match="window"):
+        gen.observe(0)
+    gen.enable_cuda_graph()
+    with pytest.raises(ValueError, match="before"):
+        gen.observe(4)
+
+
+@pytest.mark.gpu
+def test_script(capsys):
+    args = ["layers=2", "max_len_override=256", "once", "ntok=6"]
+    tokens = main(parse_cli(["model=llama-1b", "beams=4", "prompt_len=20", "eos=5", *args]))
+    out = capsys.readouterr().out
+    assert tokens.shape == (4, 6) and out.count("Score") == 4
+    tokens = main(parse_cli(["model=llama-1b", "keep=50", "window=16", "recent=20", "prompt_len=120", *args]))
+    assert tokens.shape == (1, 6) and "Rows of the cache behind the prompt: 50" in capsys.readouterr().out
