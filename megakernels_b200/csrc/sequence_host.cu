@@ -93,6 +93,8 @@ int check_shape(const MkbsKeyWeights* w) {
     if (w->queries < 1 || w->heads < w->kv_heads || w->heads % w->kv_heads) return invalid("key weights: queries must be positive, heads a multiple of kv_heads");
     if ((w->dim != 64 && w->dim != 128) || w->heads / w->kv_heads > 128 || (int64_t)w->queries * (w->heads / w->kv_heads) > 1 << 20)
         return fail(MKBS_ERR_UNSUPPORTED, "key weights: dim 64 or 128, at most 128 heads of a key and 2^20 queries times them");
+    if ((int64_t)w->layers * w->sequences * w->kv_heads * ((w->positions + 127) / 128) > 1 << 30)  // (units of work are counted in 32 bits)
+        return fail(MKBS_ERR_UNSUPPORTED, "key weights: more than 2^30 tiles of 128 keys");
     return MKBS_OK;
 }
 int check(const MkbsKeyWeights* w) {

@@ -2,12 +2,17 @@
 //   w[j] += sum_r exp2(z_rj - log2 sum_i exp2 z_ri),  z = scale log2(e) q k,  r = (query, head of the group).
 // Two passes over the scores, since a row's sum has to be known before its share of a key's weight is.
 //
-// More than 16 rows: scores on tcgen05.mma, both passes.
-//   rows   128 rows of queries (M) x 128 keys: a thread has a row and a quarter of its keys, and keeps their running maximum and
-//          sum; keys are split over blocks where there are few rows (then a small launch joins the parts);
-//   keys   128 keys (M) x 128 rows: a thread has a key and a quarter of the rows, so that a key's weight is a sum in registers.  Where
-//          there are few tiles of keys a cluster shares their rows.
-// The exponentials bound both (16 a clock and SM: 0.54 us for 128 x 128 scores at 1.9 GHz, products 0.07 - 0.13).
+// More than 16 rows: scores on tcgen05.mma, both passes, in one kernel of a block per SM that goes from unit to unit of work.
+//   rows   a unit is 128 rows of queries (M) and a run of keys, 128 at a time: a thread has a row and a quarter of its keys, and keeps their
+//          sum; where there are few rows their keys are several units, and a small launch joins the parts;
+//   keys   a unit is 128 keys (M) and a run of rows, 128 at a time: a thread has a key and a quarter of the rows, so that a key's weight is a
+//          sum in registers; where there are few keys their rows are several units, and a small launch adds the parts.
+// The exponentials bound both (16 a clock and SM: 0.54 us for 128 x 128 scores at 1.9 GHz, products 0.07 - 0.13).  Sums of a row refer to a
+// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 44 us for 1501 queries on 1501
+// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 65 us for 64 queries on 32768 keys (32 heads
+// of 128, exponentials 30 us, keys at 0.5 TB/s): what a unit begins and ends with weighs there, since a key's rows are two steps.
+// Twice the columns a thread (half the warps) took 57 and 78 us, a polynomial for every fourth exponential 45 and 70, the next step's
+// scores fetched ahead 62 and 107 (registers).
 // Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the scores go
 // through memory (4 bytes a row where a key has 128 or 256).
 #include "hybrid_kernels.h"
@@ -21,20 +26,23 @@ using namespace mkbh;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128, kSlab = kTile * 128;  // a slab: 128 rows of 64 bf16
-constexpr int kWarps = 16, kCols = kTile / (kWarps / 4), kThreads = 64 + 32 * kWarps;  // softmax warps, columns of a thread
+constexpr int kWarps = 16, kShares = kWarps / 4, kCols = kTile / kShares, kThreads = 64 + 32 * kWarps;  // softmax warps, columns of a thread
 constexpr int kBuffers = 4;                      // of 128 columns of tensor memory
 constexpr int kFew = 16;                         // rows of a fragment
 
 struct WeightArgs {
-    int sequences, queries, heads, kv_heads, positions, length, per, rows, row_tiles, splits, shares;
+    int sequences, queries, heads, kv_heads, positions, length, per, rows;
+    int row_tiles, key_tiles, splits;   // key_tiles: of the longest sequence that there may be; units of a row tile
+    int chunk, parts, items;            // row tiles of a unit, units of a key tile
     float scale;  // to base 2
     const int32_t* lengths;
     const bf16 *q, *k;
     int64_t q_layer, q_sequence, k_layer, k_sequence;
     float* weights;
     int64_t w_layer, w_sequence, w_head;
-    float2* parts;  // [item][row tile][split][128]: maximum and sum;  few rows: [item][split][16]
+    float2* stats;  // [item][row tile][split][128]: maximum and sum;  few rows: [item][split][16]
     float* offs;    // [item][row tile][128]: log2 of a row's sum, infinite where a row sees no key or there is no row
+    float* sums;    // [item][part][key tile][128]: weights, where there are parts
     float* scores;  // few rows: [item][position][row], rows rounded up to 4, 8 or 16
     int* status;
     unsigned long long timeout_ns;
@@ -42,8 +50,15 @@ struct WeightArgs {
 struct Item {
     int g, b, layer, n;
     __device__ __forceinline__ Item(const WeightArgs& a, int item)
-        : g(item % a.kv_heads), b(item / a.kv_heads % a.sequences), layer(item / a.kv_heads / a.sequences),
-          n(length_of(a.lengths, a.length, a.positions, b)) {}
+        : g(item), b(0), layer(0) {
+        if (a.items != a.kv_heads) {
+            b = item / a.kv_heads;
+            g = item - b * a.kv_heads;
+            layer = b / a.sequences;
+            b -= layer * a.sequences;
+        }
+        n = length_of(a.lengths, a.length, a.positions, b);
+    }
     __device__ __forceinline__ float* weights(const WeightArgs& a) const { return a.weights + layer * a.w_layer + b * a.w_sequence + g * a.w_head; }
 };
 
@@ -79,192 +94,276 @@ __device__ __forceinline__ void load_queries(uint32_t dst, const CUtensorMap* ma
                      : "memory");
 }
 
-// Shared memory of both kernels: `held` operands of the outer loop, a ring of `stages` of the inner one's with 512 bytes each.
+// Shared memory: two operands of units, a ring of operands of their steps with 512 bytes each.
 template <int kDim>
 struct Smem {
-    static constexpr int kOperand = kDim / 64 * kSlab, kExtra = 512;
+    static constexpr int kOperand = kDim / 64 * kSlab, kExtra = 512, kHeld = 2;
     static constexpr int stages = kDim == 64 ? 6 : 4;
-    static constexpr int kHeld = 2;  // (rows: one)
-    int ring, extra, cross, bars, ctl, total;
-    __host__ __device__ explicit Smem(bool keys) {
-        ring = (keys ? kHeld : 1) * kOperand;
-        extra = ring + stages * kOperand;
-        cross = extra + stages * kExtra;
-        bars = cross + kWarps / 4 * kTile * 8;
-        ctl = bars + (2 * kHeld + 2 * stages + 2 * kBuffers + 4) * 8;
-        total = ctl + 16;
+    static constexpr int ring = kHeld * kOperand, extra = ring + stages * kOperand, cross = extra + stages * kExtra;
+    static constexpr int bars = cross + 2 * kShares * kTile * 8, ctl = bars + (2 * kHeld + 2 * stages + 2 * kBuffers + 4) * 8, total = ctl + 16 + 1024;
+    static_assert(total <= 227 * 1024 - kStaticShared, "shared memory of a block");
+};
+
+// A unit of work: a tile held, and tiles of the other operand, first .. first + count - 1.
+template <bool kKeys>
+struct Unit {
+    int item, tile, part, first, count;
+    static __host__ __device__ uint32_t all(const WeightArgs& a) { return (uint32_t)a.items * (kKeys ? a.key_tiles * a.parts : a.row_tiles * a.splits); }
+    // A block's `turn`-th unit: the longest come first and are dealt out to and fro; none: the turn is over
+    __device__ __forceinline__ bool find(const WeightArgs& a, uint32_t turn) {
+        uint32_t u = turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (turn * gridDim.x >= all(a)) return false;
+        count = 0, first = -1;  // (no unit)
+        if (u >= all(a)) return true;
+        const uint32_t parts = kKeys ? a.parts : a.splits, rest = u / a.items;
+        item = (int)(u - rest * a.items);
+        tile = parts == 1 ? rest : rest / parts;
+        part = (int)(rest - tile * parts);
+        const int of_tile = kTile / a.per, before = Item(a, item).n - a.queries;  // (query t sees rows 0 .. before + t)
+        if (kKeys) {  // the first tile has the most rows
+            first = part * a.chunk;
+            if (tile * kTile > before) first += (tile * kTile - before) / of_tile;
+            if (tile * kTile < before + a.queries) count = max(min(a.chunk, a.row_tiles - first), 0);
+        } else {  // the last tile has the most keys
+            tile = a.row_tiles - 1 - tile;
+            const int tiles = (max(before + min((tile + 1) * of_tile, a.queries), 0) + kTile - 1) / kTile;
+            first = parts == 1 ? 0 : (int)((uint64_t)tiles * part / parts);
+            count = (parts == 1 ? tiles : (int)((uint64_t)tiles * (part + 1) / parts)) - first;
+        }
+        return true;
     }
 };
-static_assert((6 + 2) * kSlab + 6 * 512 + 4096 + 2048 < 227 * 1024 - kStaticShared && (4 + 2) * 2 * kSlab + 4 * 512 + 4096 + 2048 < 227 * 1024 - kStaticShared, "shared memory of a block");
 
-// What the roles of both kernels share.
 template <int kDim, bool kKeys>
-struct Block {
-    using S = Smem<kDim>;
-    const S sm;
-    uint32_t base, tmem;
-    char* at;
-    volatile int* ctl;  // [0] dead, [1] tensor memory
-    int warp, lane;
-    unsigned long long timeout_ns;
-    int* status;
-    __device__ __forceinline__ uint32_t bar(int i) const { return base + sm.bars + i * 8; }
-    __device__ __forceinline__ uint32_t held_full(int i) const { return bar(i); }
-    __device__ __forceinline__ uint32_t held_empty(int i) const { return bar(2 + i); }
-    __device__ __forceinline__ uint32_t full(int i) const { return bar(4 + i); }
-    __device__ __forceinline__ uint32_t empty(int i) const { return bar(4 + S::stages + i); }
-    __device__ __forceinline__ uint32_t scored(int i) const { return bar(4 + 2 * S::stages + i); }
-    __device__ __forceinline__ uint32_t read(int i) const { return bar(4 + 2 * S::stages + kBuffers + i); }
-    __device__ __forceinline__ uint32_t meeting(int i) const { return bar(4 + 2 * S::stages + 2 * kBuffers + i); }
-    __device__ __forceinline__ uint32_t stage(int i) const { return base + sm.ring + i * S::kOperand; }
-    __device__ __forceinline__ uint32_t held(int i) const { return base + i * S::kOperand; }
-    __device__ __forceinline__ bool wait(uint32_t b, uint32_t parity, int role) const { return tc_wait(b, parity & 1u, ctl, timeout_ns, status, role); }
-    __device__ __forceinline__ bool wait_all(uint32_t b, uint32_t parity) const { return __all_sync(0xffffffffu, wait(b, parity, 2)); }
-
-    __device__ __forceinline__ Block(uint8_t* raw, const WeightArgs& a, bool clear)
-        : sm(kKeys), warp(threadIdx.x >> 5), lane(threadIdx.x & 31), timeout_ns(a.timeout_ns), status(a.status) {
-        const uint32_t raw32 = mkb::smem_u32(raw);
-        base = (raw32 + 1023u) & ~1023u;
-        at = reinterpret_cast<char*>(raw) + (base - raw32);
-        ctl = reinterpret_cast<volatile int*>(at + sm.ctl);
-        if (clear) {  // rows that the copies leave out are finite
-            for (int i = threadIdx.x; i < sm.extra / 16; i += kThreads) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < 2; ++i) mkb::mbar_init(held_full(i), 1), mkb::mbar_init(held_empty(i), 1);
-            for (int i = 0; i < S::stages; ++i) mkb::mbar_init(full(i), 1), mkb::mbar_init(empty(i), kKeys ? 1 + kWarps : 1);
-            for (int i = 0; i < kBuffers; ++i) mkb::mbar_init(scored(i), 1), mkb::mbar_init(read(i), kWarps);
-            for (int i = 0; i < 4; ++i) mkb::mbar_init(meeting(i), kWarps / 4);
-            ctl[0] = 0;
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        if (warp == 1) {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + sm.ctl + 4), "r"(512u) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        }
-        tc_before_sync();
-        __syncthreads();
-        tc_after_sync();
-        tmem = (uint32_t)ctl[1];
-    }
-    // scores of step `t`: a (M) times b (N)
-    __device__ __forceinline__ void multiply(uint32_t a, uint32_t b, int t) const {
-        const uint32_t desc = tc_idesc(kTile, kTile);
-#pragma unroll
-        for (int i = 0; i < kDim / 64; ++i)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                tc_mma(tmem + t % kBuffers * kTile, tc_desc(a + i * kSlab + kk * 32), tc_desc(b + i * kSlab + kk * 32), desc, (uint32_t)((i | kk) != 0));
-    }
-    // the thread's columns of step `t`
-    __device__ __forceinline__ void scores(int t, int quarter, int part, uint32_t (&x)[kCols]) const {
-        static_assert(kCols == 32, "a load of 32 columns");
-        tc_load32(tmem + ((uint32_t)(quarter * 32) << 16) + t % kBuffers * kTile + part * kCols, x);
-        tc_before_sync();
-        __syncwarp();
-        if (lane == 0) mkb::mbar_arrive(read(t % kBuffers));
-    }
-    __device__ __forceinline__ void leave() const {
-        tc_before_sync();
-        __syncthreads();
-        if (*ctl) tc_settle();
-        if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    }
-};
-
-template <int kDim>
-__global__ void __launch_bounds__(kThreads, 1) weights_rows_kernel(const __grid_constant__ WeightMaps maps, const WeightArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_constant__ WeightMaps maps, const WeightArgs a) {
     extern __shared__ uint8_t raw[];
-    let_next();
-    const Item it(a, blockIdx.z);
-    const int tile = a.row_tiles - 1 - (int)blockIdx.y, of_tile = kTile / a.per, query0 = tile * of_tile, r0 = query0 * a.per;  // (the longest first)
-    const int last_query = min(query0 + of_tile, a.queries) - 1, before = it.n - a.queries;  // query t sees rows 0 .. before + t
-    const int tiles = (max(before + last_query + 1, 0) + kTile - 1) / kTile;
-    const int first = (int)((int64_t)tiles * blockIdx.x / a.splits), count = (int)((int64_t)tiles * (blockIdx.x + 1) / a.splits) - first;
     using S = Smem<kDim>;
-    const Block<kDim, false> c(raw, a, kTile % a.per != 0);
-    const int box_bytes = of_tile * a.per * 128;
+    let_next();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t raw32 = mkb::smem_u32(raw), base = (raw32 + 1023u) & ~1023u;
+    char* const at = reinterpret_cast<char*>(raw) + (base - raw32);
+    volatile int* const ctl = reinterpret_cast<volatile int*>(at + S::ctl);  // [0] dead, [1] tensor memory
+    auto bar = [&](int i) { return base + S::bars + i * 8; };
+    auto held_full = [&](int i) { return bar(i & 1); };
+    auto held_empty = [&](int i) { return bar(2 + (i & 1)); };
+    auto full = [&](int t) { return bar(4 + t % S::stages); };
+    auto empty = [&](int t) { return bar(4 + S::stages + t % S::stages); };
+    auto scored = [&](int t) { return bar(4 + 2 * S::stages + t % kBuffers); };
+    auto read = [&](int t) { return bar(4 + 2 * S::stages + kBuffers + t % kBuffers); };
+    auto meeting = [&](int i) { return bar(4 + 2 * S::stages + 2 * kBuffers + i); };
+    auto held = [&](int i) { return base + (i & 1) * S::kOperand; };
+    auto stage = [&](int t) { return base + S::ring + t % S::stages * S::kOperand; };
+    auto wait = [&](uint32_t b, int turn, int role) { return tc_wait(b, (uint32_t)turn & 1u, ctl, a.timeout_ns, a.status, role); };
+    auto wait_all = [&](uint32_t b, int turn) { return __all_sync(0xffffffffu, wait(b, turn, 2)); };
 
-    float2 mine = make_float2(-INFINITY, 0.f);
-    if (c.warp == 0 && c.lane == 0 && count > 0) {
-        mkb::mbar_expect_tx(c.held_full(0), kDim / 64 * box_bytes);
-        load_queries(c.held(0), &maps.q, it, kDim, a.per, query0, c.held_full(0));
+    if (kTile % a.per != 0) {  // rows that the copies leave out are finite
+        for (int i = threadIdx.x; i < S::extra / 16; i += kThreads) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) mkb::mbar_init(held_full(i), 1), mkb::mbar_init(held_empty(i), 1);
+        for (int i = 0; i < S::stages; ++i) mkb::mbar_init(full(i), 1), mkb::mbar_init(empty(i), kKeys ? 1 + kWarps : 1);
+        for (int i = 0; i < kBuffers; ++i) mkb::mbar_init(scored(i), 1), mkb::mbar_init(read(i), kWarps);
+        for (int i = 0; i < 4; ++i) mkb::mbar_init(meeting(i), kShares);
+        ctl[0] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + S::ctl + 4), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    const uint32_t tmem = (uint32_t)ctl[1];
+    if (kKeys) after_previous();  // (the offsets; the rows' launch is an ordinary one)
+
+    const int of_tile = kTile / a.per, box_bytes = kDim / 64 * of_tile * a.per * 128;
+    if (warp == 0 && lane == 0) {
         bool ok = true;
-        int t = 0;
-        for (; t < count; ++t) {
-            const int st = t % S::stages;
-            ok = c.wait(c.empty(st), (uint32_t)(t / S::stages) ^ 1u, 0);
+        int t = 0, u = 0;
+        Unit<kKeys> unit;
+        for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
+            if (unit.count == 0) continue;
+            const Item it(a, unit.item);
+            ok = wait(held_empty(u), (u >> 1) ^ 1, 0);
             if (!ok) break;
-            mkb::mbar_expect_tx(c.full(st), S::kOperand);
-            load_keys(c.stage(st), &maps.k, it, kDim, (first + t) * kTile, c.full(st));
-        }
-        // no copy may be in flight when the block's shared memory goes away
-        tc_wait(c.held_full(0), 0, nullptr, a.timeout_ns, a.status, 0);
-        for (int i = max(t - S::stages, 0); i < t; ++i) tc_wait(c.full(i % S::stages), (uint32_t)(i / S::stages) & 1u, nullptr, a.timeout_ns, a.status, 0);
-    } else if (c.warp == 1 && c.lane == 0 && count > 0) {
-        bool ok = c.wait(c.held_full(0), 0, 1);
-        for (int t = 0; t < count && ok; ++t) {
-            const int st = t % S::stages;
-            ok = c.wait(c.full(st), (uint32_t)(t / S::stages), 1) && c.wait(c.read(t % kBuffers), (uint32_t)(t / kBuffers) ^ 1u, 1);
-            if (!ok) break;
-            tc_after_sync();
-            c.multiply(c.held(0), c.stage(st), t);
-            tc_commit(c.empty(st));
-            tc_commit(c.scored(t % kBuffers));
-        }
-    } else if (c.warp >= 2) {
-        const int quarter = c.warp & 3, part = (c.warp - 2) >> 2;  // (a warp may touch 32 lanes of tensor memory)
-        const int warp_row = quarter * 32, r = warp_row + c.lane, have = min(of_tile * a.per, a.rows - r0);
-        const int last = before + (r0 + r) / a.per, warp_last = before + (r0 + warp_row) / a.per;
-        for (int t = 0; t < count; ++t) {
-            if (!c.wait_all(c.scored(t % kBuffers), (uint32_t)(t / kBuffers))) break;
-            tc_after_sync();
-            uint32_t x[kCols];
-            c.scores(t, quarter, part, x);
-            if (warp_row >= have) continue;
-            const int j0 = (first + t) * kTile + part * kCols;
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, s4[4] = {0.f, 0.f, 0.f, 0.f}, mul = a.scale;
-            if (j0 + kCols - 1 <= warp_last && a.scale > 0.f) {  // every row sees all of these keys
-#pragma unroll
-                for (int i = 0; i < kCols; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(x[i]));
-            } else {
-                mul = 1.f;
-#pragma unroll
-                for (int i = 0; i < kCols; ++i) {
-                    const float z = j0 + i <= last ? __uint_as_float(x[i]) * a.scale : -INFINITY;
-                    m4[i & 3] = fmaxf(m4[i & 3], z);
-                    x[i] = __float_as_uint(z);
+            mkb::mbar_expect_tx(held_full(u), kKeys ? S::kOperand : box_bytes);
+            if (kKeys) load_keys(held(u), &maps.k, it, kDim, unit.tile * kTile, held_full(u));
+            else load_queries(held(u), &maps.q, it, kDim, a.per, unit.tile * of_tile, held_full(u));
+            ++u;
+            for (int n = unit.first; n < unit.first + unit.count; ++n, ++t) {
+                ok = wait(empty(t), t / S::stages ^ 1, 0);
+                if (!ok) break;
+                mkb::mbar_expect_tx(full(t), kKeys ? box_bytes + S::kExtra : S::kOperand);
+                if (kKeys) {
+                    load_queries(stage(t), &maps.q, it, kDim, a.per, n * of_tile, full(t));
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(base + S::extra + t % S::stages * S::kExtra),
+                                 "l"(a.offs + ((int64_t)unit.item * a.row_tiles + n) * kTile), "r"(S::kExtra), "r"(full(t))
+                                 : "memory");
+                } else {
+                    load_keys(stage(t), &maps.k, it, kDim, n * kTile, full(t));
                 }
             }
-            const float top = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul, mine.x);
-            if (top == -INFINITY) continue;
-            const float keep = fast_exp2(mine.x - top);  // (0 from minus infinity)
+        }
+        // no copy may be in flight when the block's shared memory goes away
+        for (int i = max(u - 2, 0); i < u; ++i) tc_wait(held_full(i), (uint32_t)(i >> 1) & 1u, nullptr, a.timeout_ns, a.status, 0);
+        for (int i = max(t - S::stages, 0); i < t; ++i) tc_wait(full(i), (uint32_t)(i / S::stages) & 1u, nullptr, a.timeout_ns, a.status, 0);
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t desc = tc_idesc(kTile, kTile);
+        bool ok = true;
+        int t = 0, u = 0;
+        Unit<kKeys> unit;
+        for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
+            if (unit.count == 0) continue;
+            ok = wait(held_full(u), u >> 1, 1);
+            for (int n = 0; n < unit.count && ok; ++n, ++t) {
+                ok = wait(full(t), t / S::stages, 1) && wait(read(t), t / kBuffers ^ 1, 1);
+                if (!ok) break;
+                tc_after_sync();
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) s4[i & 3] += fast_exp2(fmaf(__uint_as_float(x[i]), mul, -top));
-            mine = make_float2(top, fmaf(mine.y, keep, (s4[0] + s4[1]) + (s4[2] + s4[3])));
+                for (int slab = 0; slab < kDim / 64; ++slab)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc_mma(tmem + t % kBuffers * kTile, tc_desc(held(u) + slab * kSlab + kk * 32), tc_desc(stage(t) + slab * kSlab + kk * 32), desc,
+                               (uint32_t)((slab | kk) != 0));
+                tc_commit(empty(t));
+                if (n == unit.count - 1) tc_commit(held_empty(u));
+                tc_commit(scored(t));
+            }
+            ++u;
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3, share = (warp - 2) >> 2, lanes = quarter * 32 + lane;  // (a warp may touch 32 lanes of tensor memory)
+        bool ok = true;
+        int t = 0, u = 0;
+        auto scores = [&](uint32_t (&x)[kCols]) {  // the thread's, of step t
+            static_assert(kCols == 32, "one load of 32 columns");
+            tc_load32(tmem + ((uint32_t)(quarter * 32) << 16) + t % kBuffers * kTile + share * kCols, x);
+            tc_before_sync();
+            __syncwarp();
+            if (lane == 0) mkb::mbar_arrive(read(t));
+        };
+        Unit<kKeys> unit;
+        for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
+            if (unit.count == 0 && (kKeys || unit.first < 0)) continue;
+            const Item it(a, unit.item);
+            const int before = it.n - a.queries;
+            float2 mine = make_float2(-INFINITY, 0.f);  // rows: maximum and sum; keys: x is not used
+            if constexpr (kKeys) {
+                const int j = unit.tile * kTile + lanes;
+                const int own_row = max(j - before, 0) * a.per, last_row = max(unit.tile * kTile + quarter * 32 + 31 - before, 0) * a.per;  // the first that sees it
+                float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int n = 0; n < unit.count; ++n, ++t) {
+                    const int r0 = (unit.first + n) * of_tile * a.per + share * kCols;
+                    ok = wait_all(scored(t), t / kBuffers) && wait_all(full(t), t / S::stages);
+                    if (!ok) break;
+                    tc_after_sync();
+                    uint32_t x[kCols];
+                    scores(x);
+                    const float4* const off = reinterpret_cast<const float4*>(at + S::extra + t % S::stages * S::kExtra) + share * (kCols / 4);
+                    if (last_row <= r0) {
+#pragma unroll
+                        for (int c = 0; c < kCols / 4; ++c) {
+                            const float4 o = off[c];
+                            s4[0] += fast_exp2(fmaf(__uint_as_float(x[4 * c]), a.scale, -o.x));
+                            s4[1] += fast_exp2(fmaf(__uint_as_float(x[4 * c + 1]), a.scale, -o.y));
+                            s4[2] += fast_exp2(fmaf(__uint_as_float(x[4 * c + 2]), a.scale, -o.z));
+                            s4[3] += fast_exp2(fmaf(__uint_as_float(x[4 * c + 3]), a.scale, -o.w));
+                        }
+                    } else {
+                        const int hidden = own_row - r0;  // columns before that do not see the key
+#pragma unroll
+                        for (int c = 0; c < kCols / 4; ++c) {
+                            const float4 o = off[c];
+                            const float p[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float y = fast_exp2(fmaf(__uint_as_float(x[4 * c + e]), a.scale, -p[e]));
+                                s4[e] += 4 * c + e >= hidden ? y : 0.f;
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mkb::mbar_arrive(empty(t));
+                }
+                mine.y = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            } else {
+                const int r0 = unit.tile * of_tile * a.per, have = min(of_tile * a.per, a.rows - r0), warp_row = quarter * 32;
+                const int last = before + (r0 + lanes) / a.per, warp_last = before + (r0 + warp_row) / a.per;
+                for (int n = 0; n < unit.count; ++n, ++t) {
+                    ok = wait_all(scored(t), t / kBuffers);
+                    if (!ok) break;
+                    tc_after_sync();
+                    uint32_t x[kCols];
+                    scores(x);
+                    if (warp_row >= have) continue;
+                    const int j0 = (unit.first + n) * kTile + share * kCols;
+                    const bool whole = j0 + kCols - 1 <= warp_last;  // every row sees all of these keys
+                    if (whole && __all_sync(0xffffffffu, mine.x > -INFINITY)) {
+                        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) s4[c & 3] += fast_exp2(fmaf(__uint_as_float(x[c]), a.scale, -mine.x));
+                        const float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                        if (__all_sync(0xffffffffu, sum < 0x1p100f)) {
+                            mine.y += sum;
+                            continue;
+                        }
+                    }
+                    float top = mine.x, sum = 0.f;
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        const float z = j0 + c <= last ? __uint_as_float(x[c]) * a.scale : -INFINITY;
+                        top = fmaxf(top, z);
+                        x[c] = __float_as_uint(z);
+                    }
+                    if (top > -INFINITY) {
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) sum += fast_exp2(__uint_as_float(x[c]) - top);
+                        mine = make_float2(top, fmaf(mine.y, fast_exp2(mine.x - top), sum));  // (0 from minus infinity)
+                    }
+                }
+            }
+            if (!ok) break;
+            // the threads of a row or key
+            float2* const cross = reinterpret_cast<float2*>(at + S::cross) + (u & 1) * kShares * kTile + lanes;
+            cross[share * kTile] = mine;
+            __syncwarp();
+            if (lane == 0) mkb::mbar_arrive(meeting(quarter));
+            ok = wait_all(meeting(quarter), u);
+            ++u;
+            if (!ok || share != 0) continue;
+            if constexpr (kKeys) {
+                float sum = cross[0].y;
+#pragma unroll
+                for (int c = 1; c < kShares; ++c) sum += cross[c * kTile].y;
+                const int j = unit.tile * kTile + lanes;
+                if (a.parts > 1) a.sums[(((int64_t)unit.item * a.parts + unit.part) * a.key_tiles + unit.tile) * kTile + lanes] = sum;
+                else if (j < it.n) it.weights(a)[j] += sum;
+            } else {
+                const bool there = lanes < of_tile * a.per && unit.tile * of_tile * a.per + lanes < a.rows;
+                float2 all = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int c = 0; c < kShares; ++c)
+                    if (there) all = join(all, cross[c * kTile]);
+                const int64_t row_tile = (int64_t)unit.item * a.row_tiles + unit.tile;
+                if (a.splits > 1) a.stats[(row_tile * a.splits + unit.part) * kTile + lanes] = all;
+                else a.offs[row_tile * kTile + lanes] = off_of(all.x, all.y);
+            }
         }
     }
-    float2* const cross = reinterpret_cast<float2*>(c.at + c.sm.cross);
-    if (c.warp >= 2) cross[((c.warp - 2) >> 2) * kTile + (c.warp & 3) * 32 + c.lane] = mine;
-    c.leave();
-    if (threadIdx.x < kTile) {
-        const int r = threadIdx.x;
-        float2 all = cross[r];
-        for (int i = 1; i < kWarps / 4; ++i) all = join(all, cross[i * kTile + r]);
-        if (r >= of_tile * a.per || r0 + r >= a.rows) all = make_float2(-INFINITY, 0.f);
-        const int64_t row_tile = (int64_t)blockIdx.z * a.row_tiles + tile;
-        if (a.splits > 1) a.parts[(row_tile * a.splits + blockIdx.x) * kTile + r] = all;
-        else a.offs[row_tile * kTile + r] = off_of(all.x, all.y);
-    }
+    tc_before_sync();
+    __syncthreads();
+    if (*ctl) tc_settle();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // A row's parts to the logarithm of its sum.
 __global__ void __launch_bounds__(kTile) weights_join_kernel(const WeightArgs a) {
     let_next();
     after_previous();
-    const float2* const parts = a.parts + (int64_t)blockIdx.x * a.splits * kTile + threadIdx.x;
+    const float2* const parts = a.stats + (int64_t)blockIdx.x * a.splits * kTile + threadIdx.x;
     float top = -INFINITY, sum = 0.f;
     for (int i = 0; i < a.splits; ++i) top = fmaxf(top, parts[i * kTile].x);
     for (int i = 0; i < a.splits; ++i) {
@@ -274,138 +373,16 @@ __global__ void __launch_bounds__(kTile) weights_join_kernel(const WeightArgs a)
     a.offs[(int64_t)blockIdx.x * kTile + threadIdx.x] = off_of(top, sum);
 }
 
-template <int kDim>
-__global__ void __launch_bounds__(kThreads, 1) weights_keys_kernel(const __grid_constant__ WeightMaps maps, const WeightArgs a, int parts) {
-    extern __shared__ uint8_t raw[];
+// A key's parts to its weight.
+__global__ void __launch_bounds__(kTile) weights_add_kernel(const WeightArgs a) {
     const Item it(a, blockIdx.y);
-    const int share = blockIdx.x / parts, rank = blockIdx.x - share * parts;
-    const int of_tile = kTile / a.per, before = it.n - a.queries, tiles = (it.n + kTile - 1) / kTile;
-    using S = Smem<kDim>;
-    const Block<kDim, true> c(raw, a, kTile % a.per != 0);
-    const int box_bytes = of_tile * a.per * 128;
-    // Steps: tiles of keys share, share + shares, ...; of each the row tiles that see one of its keys, every `parts`-th of them
-    auto first_rows = [&](int kt) { return max(kt * kTile - before, 0) / of_tile + rank; };
-    auto rows_of = [&](int kt) { return max(a.row_tiles - first_rows(kt) + parts - 1, 0) / parts; };
-    float* const cross = reinterpret_cast<float*>(c.at + c.sm.cross);  // [parity][4][128]
-    float* const weights = it.weights(a);
+    const int j = blockIdx.x * kTile + threadIdx.x, of_tile = kTile / a.per;
+    const int first = max((int)blockIdx.x * kTile - (it.n - a.queries), 0) / of_tile, parts = (max(a.row_tiles - first, 0) + a.chunk - 1) / a.chunk;
     after_previous();
-
-    if (c.warp == 0 && c.lane == 0) {
-        bool ok = true;
-        int t = 0, held = 0;
-        for (int kt = share; kt < tiles && ok; kt += a.shares) {
-            const int steps = rows_of(kt);
-            if (steps == 0) continue;
-            ok = c.wait(c.held_empty(held & 1), (uint32_t)(held >> 1) ^ 1u, 0);
-            if (!ok) break;
-            mkb::mbar_expect_tx(c.held_full(held & 1), S::kOperand);
-            load_keys(c.held(held & 1), &maps.k, it, kDim, kt * kTile, c.held_full(held & 1));
-            ++held;
-            for (int i = 0; i < steps && ok; ++i) {
-                const int st = t % S::stages, tile = first_rows(kt) + i * parts;
-                ok = c.wait(c.empty(st), (uint32_t)(t / S::stages) ^ 1u, 0);
-                if (!ok) break;
-                mkb::mbar_expect_tx(c.full(st), kDim / 64 * box_bytes + S::kExtra);
-                load_queries(c.stage(st), &maps.q, it, kDim, a.per, tile * of_tile, c.full(st));
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(c.base + c.sm.extra + st * S::kExtra),
-                             "l"(a.offs + ((int64_t)blockIdx.y * a.row_tiles + tile) * kTile), "r"(S::kExtra), "r"(c.full(st))
-                             : "memory");
-                ++t;
-            }
-        }
-        for (int i = max(held - 2, 0); i < held; ++i) tc_wait(c.held_full(i & 1), (uint32_t)(i >> 1) & 1u, nullptr, a.timeout_ns, a.status, 0);
-        for (int i = max(t - S::stages, 0); i < t; ++i) tc_wait(c.full(i % S::stages), (uint32_t)(i / S::stages) & 1u, nullptr, a.timeout_ns, a.status, 0);
-    } else if (c.warp == 1 && c.lane == 0) {
-        bool ok = true;
-        int t = 0, held = 0;
-        for (int kt = share; kt < tiles && ok; kt += a.shares) {
-            const int steps = rows_of(kt);
-            if (steps == 0) continue;
-            ok = c.wait(c.held_full(held & 1), (uint32_t)(held >> 1), 1);
-            for (int i = 0; i < steps && ok; ++i, ++t) {
-                const int st = t % S::stages;
-                ok = c.wait(c.full(st), (uint32_t)(t / S::stages), 1) && c.wait(c.read(t % kBuffers), (uint32_t)(t / kBuffers) ^ 1u, 1);
-                if (!ok) break;
-                tc_after_sync();
-                c.multiply(c.held(held & 1), c.stage(st), t);
-                tc_commit(c.empty(st));
-                if (i == steps - 1) tc_commit(c.held_empty(held & 1));
-                tc_commit(c.scored(t % kBuffers));
-            }
-            ++held;
-        }
-    } else if (c.warp >= 2) {
-        const int quarter = c.warp & 3, part = (c.warp - 2) >> 2;
-        bool ok = true;
-        int t = 0, turn = 0;
-        for (int kt = share; kt < tiles && ok; kt += a.shares, ++turn) {
-            const int steps = rows_of(kt), j = kt * kTile + quarter * 32 + c.lane;
-            const int own_row = max(j - before, 0) * a.per, last_row = max(kt * kTile + quarter * 32 + 31 - before, 0) * a.per;  // the first that sees it
-            float s4[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int i = 0; i < steps; ++i, ++t) {
-                const int st = t % S::stages, r0 = (first_rows(kt) + i * parts) * of_tile * a.per + part * kCols;
-                ok = c.wait_all(c.scored(t % kBuffers), (uint32_t)(t / kBuffers)) && c.wait_all(c.full(st), (uint32_t)(t / S::stages));
-                if (!ok) break;
-                tc_after_sync();
-                uint32_t x[kCols];
-                c.scores(t, quarter, part, x);
-                const float4* const off = reinterpret_cast<const float4*>(c.at + c.sm.extra + st * S::kExtra) + part * (kCols / 4);
-                if (last_row <= r0) {
-#pragma unroll
-                    for (int n = 0; n < kCols / 4; ++n) {
-                        const float4 o = off[n];
-                        s4[0] += fast_exp2(fmaf(__uint_as_float(x[4 * n]), a.scale, -o.x));
-                        s4[1] += fast_exp2(fmaf(__uint_as_float(x[4 * n + 1]), a.scale, -o.y));
-                        s4[2] += fast_exp2(fmaf(__uint_as_float(x[4 * n + 2]), a.scale, -o.z));
-                        s4[3] += fast_exp2(fmaf(__uint_as_float(x[4 * n + 3]), a.scale, -o.w));
-                    }
-                } else {
-                    const int hidden = own_row - r0;  // columns before that do not see the key
-#pragma unroll
-                    for (int n = 0; n < kCols / 4; ++n) {
-                        const float4 o = off[n];
-                        const float p[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float y = fast_exp2(fmaf(__uint_as_float(x[4 * n + e]), a.scale, -p[e]));
-                            s4[e] += 4 * n + e >= hidden ? y : 0.f;
-                        }
-                    }
-                }
-                __syncwarp();
-                if (c.lane == 0) mkb::mbar_arrive(c.empty(st));
-            }
-            if (!ok) break;
-            // the four threads of a key
-            float* const at = cross + (turn & 1) * kWarps / 4 * kTile + quarter * 32 + c.lane;
-            at[part * kTile] = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            __syncwarp();
-            if (c.lane == 0) mkb::mbar_arrive(c.meeting(quarter));
-            ok = c.wait_all(c.meeting(quarter), (uint32_t)turn);
-            if (ok && part == 0) {
-                float sum = at[0];
-#pragma unroll
-                for (int i = 1; i < kWarps / 4; ++i) sum += at[i * kTile];
-                if (parts > 1) at[0] = sum;  // (one tile of keys per block)
-                else if (j < it.n) weights[j] += sum;
-            }
-        }
-    }
-    c.leave();
-    if (parts > 1) {
-        tc_cluster_sync();
-        const int j = share * kTile + threadIdx.x;
-        if (rank == 0 && threadIdx.x < kTile && j < it.n) {
-            float sum = cross[threadIdx.x];
-            for (int i = 1; i < parts; ++i) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc_peer(mkb::smem_u32(cross + threadIdx.x), i)) : "memory");
-                sum += v;
-            }
-            weights[j] += sum;
-        }
-        tc_cluster_sync();
-    }
+    if (j >= it.n) return;
+    float sum = 0.f;
+    for (int i = 0; i < parts; ++i) sum += a.sums[(((int64_t)blockIdx.y * a.parts + i) * a.key_tiles + blockIdx.x) * kTile + threadIdx.x];
+    it.weights(a)[j] += sum;
 }
 
 // ---- up to 16 rows ------------------------------------------------------------------------------ //
@@ -491,7 +468,7 @@ __global__ void __launch_bounds__(kFewThreads) weights_few_kernel(const WeightAr
     if (threadIdx.x < kFew) {
         float2 all = shared[0][threadIdx.x];
         for (int i = 1; i < kFewWarps; ++i) all = join(all, shared[i][threadIdx.x]);
-        a.parts[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kFew + threadIdx.x] = all;
+        a.stats[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kFew + threadIdx.x] = all;
     }
 }
 
@@ -502,7 +479,7 @@ __global__ void __launch_bounds__(kFewThreads) weights_sum_kernel(const WeightAr
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     after_previous();
     for (int r = warp; r < kRowsPad; r += kFewWarps) {
-        const float2* const parts = a.parts + (int64_t)blockIdx.y * a.splits * kFew + r;
+        const float2* const parts = a.stats + (int64_t)blockIdx.y * a.splits * kFew + r;
         float2 all = make_float2(-INFINITY, 0.f);
         for (int i = lane; i < a.splits; i += 32) all = join(all, parts[i * kFew]);
 #pragma unroll
@@ -526,43 +503,60 @@ __global__ void __launch_bounds__(kFewThreads) weights_sum_kernel(const WeightAr
 // ---- host ------------------------------------------------------------------------------------------ //
 struct Plan {
     WeightArgs a;
-    int items, parts, rows_pad;
+    int rows_pad;
     bool few;
     size_t bytes;
     explicit Plan(const MkbsKeyWeights& w) {
-        const int per = w.heads / w.kv_heads, rows = w.queries * per;
-        items = w.layers * w.sequences * w.kv_heads;
-        const int longest = w.lengths != nullptr ? w.positions : w.length, tiles = longest > kTile ? (longest + kTile - 1) / kTile : 1;
-        few = rows <= kFew;
-        const int row_tiles = (w.queries + kTile / per - 1) / (kTile / per);
-        a = {w.sequences, w.queries, w.heads, w.kv_heads, w.positions, w.length, per, rows, row_tiles, 1, 1, w.scale * kLog2e, w.lengths,
-             static_cast<const bf16*>(w.q), static_cast<const bf16*>(w.k), w.q_layer, w.q_sequence, w.k_layer, w.k_sequence,
-             w.weights, w.w_layer, w.w_sequence, w.w_head, nullptr, nullptr, nullptr, w.status,
-             w.wait_timeout_ms ? w.wait_timeout_ms * 1000000ull : kWaitNs};
         auto up = [](int n, int of) { return (n + of - 1) / of; };
-        char* const base = static_cast<char*>(w.workspace);
+        auto take = [&](size_t n) {  // bytes of the workspace
+            char* const at = static_cast<char*>(w.workspace) + bytes;
+            bytes += (n + 255) / 256 * 256;
+            return at;
+        };
+        bytes = 0;
+        a = {};
+        a.sequences = w.sequences;
+        a.queries = w.queries;
+        a.heads = w.heads;
+        a.kv_heads = w.kv_heads;
+        a.positions = w.positions;
+        a.length = w.length;
+        a.lengths = w.lengths;
+        a.per = w.heads / w.kv_heads;
+        a.rows = w.queries * a.per;
+        a.items = w.layers * w.sequences * w.kv_heads;
+        a.scale = w.scale * kLog2e;
+        a.q = static_cast<const bf16*>(w.q);
+        a.k = static_cast<const bf16*>(w.k);
+        a.q_layer = w.q_layer, a.q_sequence = w.q_sequence, a.k_layer = w.k_layer, a.k_sequence = w.k_sequence;
+        a.weights = w.weights;
+        a.w_layer = w.w_layer, a.w_sequence = w.w_sequence, a.w_head = w.w_head;
+        a.status = w.status;
+        a.timeout_ns = w.wait_timeout_ms ? w.wait_timeout_ms * 1000000ull : kWaitNs;
+        const int longest = w.lengths != nullptr ? w.positions : w.length;
+        few = a.rows <= kFew;
         if (few) {
-            rows_pad = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+            rows_pad = a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : 16;
             // four blocks per SM, none with less than 64 keys a warp
-            a.splits = up(4 * kSms, items);
+            a.splits = up(4 * kSms, a.items);
             if (a.splits > up(longest, 64 * kFewWarps)) a.splits = up(longest, 64 * kFewWarps);
             if (a.splits < 1) a.splits = 1;
-            const size_t scores = ((size_t)items * w.positions * rows_pad * 4 + 255) / 256 * 256;
-            a.scores = reinterpret_cast<float*>(base);
-            a.parts = reinterpret_cast<float2*>(base + scores);
-            bytes = scores + (size_t)items * a.splits * kFew * 8;
+            a.scores = reinterpret_cast<float*>(take((size_t)a.items * w.positions * rows_pad * 4));
+            a.stats = reinterpret_cast<float2*>(take((size_t)a.items * a.splits * kFew * 8));
             return;
         }
-        // rows: a block per SM; keys as well, and where there are not as many tiles, clusters
-        a.splits = kSms / (items * row_tiles);
-        a.splits = a.splits < 1 ? 1 : a.splits > tiles ? tiles : a.splits;
-        a.shares = kSms / items;
-        a.shares = a.shares < 1 ? 1 : a.shares > tiles ? tiles : a.shares;
-        for (parts = 1; a.shares == tiles && parts < 8 && 2 * parts <= row_tiles && items * a.shares * parts < 2 * kSms;) parts *= 2;
-        const size_t offs = (size_t)items * row_tiles * kTile * 4;
-        a.offs = reinterpret_cast<float*>(base);
-        a.parts = reinterpret_cast<float2*>(base + offs);
-        bytes = offs + (a.splits > 1 ? (size_t)items * row_tiles * a.splits * kTile * 8 : 0);
+        a.row_tiles = up(w.queries, kTile / a.per);
+        a.key_tiles = longest > kTile ? up(longest, kTile) : 1;
+        // as many units of rows as SMs
+        a.splits = kSms / (a.items * a.row_tiles);
+        a.splits = a.splits < 1 ? 1 : a.splits > a.key_tiles ? a.key_tiles : a.splits;
+        // four units of keys and more for every SM, none of less than four row tiles
+        a.chunk = a.row_tiles;
+        while (a.chunk > 4 && (int64_t)a.items * a.key_tiles * up(a.row_tiles, a.chunk) < 4 * kSms) a.chunk = up(a.chunk, 2);
+        a.parts = up(a.row_tiles, a.chunk);
+        a.offs = reinterpret_cast<float*>(take((size_t)a.items * a.row_tiles * kTile * 4));
+        if (a.splits > 1) a.stats = reinterpret_cast<float2*>(take((size_t)a.items * a.row_tiles * a.splits * kTile * 8));
+        if (a.parts > 1) a.sums = reinterpret_cast<float*>(take((size_t)a.items * a.parts * a.key_tiles * kTile * 4));
     }
 };
 
@@ -599,31 +593,22 @@ cudaError_t launch(const MkbsKeyWeights& w, const Plan& p, cudaStream_t s) {
     const cuuint64_t k_stride[3] = {k_row, k_sequence, k_layer};
     const cuuint32_t k_box[4] = {64, kTile, 1, 1};
     if ((e = encode(&maps.k, a.k, 4, k_size, k_stride, k_box)) != cudaSuccess) return e;
-    const int rows_smem = Smem<kDim>(false).total + 1024, keys_smem = Smem<kDim>(true).total + 1024;
-    if ((e = allow_shared_memory<weights_rows_kernel<kDim>>()) != cudaSuccess) return e;
-    if ((e = allow_shared_memory<weights_keys_kernel<kDim>>()) != cudaSuccess) return e;
-    weights_rows_kernel<kDim><<<dim3(a.splits, a.row_tiles, p.items), kThreads, rows_smem, s>>>(maps, a);
+    if ((e = allow_shared_memory<weights_kernel<kDim, false>>()) != cudaSuccess) return e;
+    if ((e = allow_shared_memory<weights_kernel<kDim, true>>()) != cudaSuccess) return e;
+    auto blocks = [](uint32_t units) { return dim3(units < kSms ? units : kSms); };
+    weights_kernel<kDim, false><<<blocks(Unit<false>::all(a)), kThreads, Smem<kDim>::total, s>>>(maps, a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    if (a.splits > 1 && (e = launch_early(weights_join_kernel, dim3(p.items * a.row_tiles), dim3(kTile), 0, s, a)) != cudaSuccess) return e;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(a.shares * p.parts, p.items);
-    c.blockDim = dim3(kThreads);
-    c.dynamicSmemBytes = keys_smem;
-    c.stream = s;
-    cudaLaunchAttribute attrs[2] = {may_begin_early()};
-    attrs[1].id = cudaLaunchAttributeClusterDimension;
-    attrs[1].val.clusterDim.x = p.parts;
-    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
-    c.attrs = attrs;
-    c.numAttrs = p.parts > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&c, weights_keys_kernel<kDim>, maps, a, p.parts);
+    if (a.splits > 1 && (e = launch_early(weights_join_kernel, dim3(a.items * a.row_tiles), dim3(kTile), 0, s, a)) != cudaSuccess) return e;
+    e = launch_early(weights_kernel<kDim, true>, blocks(Unit<true>::all(a)), dim3(kThreads), Smem<kDim>::total, s, maps, a);
+    if (e != cudaSuccess || a.parts == 1) return e;
+    return launch_early(weights_add_kernel, dim3(a.key_tiles, a.items), dim3(kTile), 0, s, a);
 }
 
 template <int kDim, int kRowsPad>
 cudaError_t launch_few(const Plan& p, cudaStream_t s) {
-    weights_few_kernel<kDim, kRowsPad><<<dim3(p.a.splits, p.items), kFewThreads, 0, s>>>(p.a);
+    weights_few_kernel<kDim, kRowsPad><<<dim3(p.a.splits, p.a.items), kFewThreads, 0, s>>>(p.a);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-    return launch_early(weights_sum_kernel<kRowsPad>, dim3(p.a.splits, p.items), dim3(kFewThreads), 0, s, p.a);
+    return launch_early(weights_sum_kernel<kRowsPad>, dim3(p.a.splits, p.a.items), dim3(kFewThreads), 0, s, p.a);
 }
 template <int kDim>
 cudaError_t choose(const MkbsKeyWeights& w, const Plan& p, cudaStream_t s) {

@@ -70,7 +70,7 @@ def beams_struct(**kw):
 
 
 def weights_struct(**kw):
-    base = dict(layers=2, sequences=2, queries=3, heads=8, kv_heads=2, dim=64, positions=100, length=50, scale=0.1, q_layer=3072 * 2, q_sequence=3072 // 2,
+    base = dict(layers=2, sequences=2, queries=3, heads=8, kv_heads=2, dim=64, positions=100, length=50, scale=0.1, q_layer=6144, q_sequence=1536,
                 k_layer=25600, k_sequence=12800, w_layer=400, w_sequence=200, w_head=100, workspace_bytes=1 << 30)
     return fill(ops.MkbsKeyWeights, **{**base, **kw})
 
@@ -121,7 +121,7 @@ REFUSED = [
     ("key_weights", weights_struct, [
         (dict(struct_bytes=8), 1, "struct size"), (dict(layers=0), 1, "positive"), (dict(positions=0), 1, "positive"), (dict(queries=0), 1, "queries"), (dict(heads=7), 1, "multiple"),
         (dict(heads=0), 1, "multiple"), (dict(dim=96), 5, "dim"), (dict(heads=258), 5, "128 heads"), (dict(q_layer=1528), 1, "overlap"), (dict(k_layer=12792), 1, "overlap"), (dict(length=101), 1, "length"), (dict(length=-1), 1, "length"), (dict(lengths=FAKE + 2), 1, "length"),
-        (dict(layers=60000), 5, "65535"), (dict(positions=1 << 29), 5, "positions"), (dict(queries=1 << 20), 5, "2^20"), (dict(q=FAKE + 8), 1, "unaligned"), (dict(k=None), 1, "missing"),
+        (dict(layers=60000), 5, "65535"), (dict(positions=1 << 29), 5, "positions"), (dict(queries=1 << 20), 5, "2^20"), (dict(layers=1, kv_heads=8, sequences=1024, positions=1 << 25), 5, "tiles"), (dict(q=FAKE + 8), 1, "unaligned"), (dict(k=None), 1, "missing"),
         (dict(weights=FAKE + 2), 1, "unaligned"), (dict(q_layer=4), 1, "multiples of 8"), (dict(k_sequence=12804), 1, "multiples of 8"), (dict(k_sequence=12792), 1, "overlap"),
         (dict(q_sequence=1528), 1, "overlap"), (dict(w_head=99), 1, "overlap"), (dict(w_sequence=99), 1, "overlap"), (dict(w_layer=99), 1, "overlap"), (dict(scale=math.nan), 1, "finite"),
         (dict(scale=math.inf), 1, "finite"), (dict(workspace=FAKE + 16), 1, "workspace"), (dict(workspace_bytes=16), 1, "workspace"), (dict(status=FAKE + 1), 1, "unaligned"),
