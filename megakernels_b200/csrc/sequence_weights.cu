@@ -14,7 +14,9 @@
 // Twice the columns a thread (half the warps) took 57 and 78 us, a polynomial for every fourth exponential 45 and 70, the next step's
 // scores fetched ahead 62 and 107 (registers).
 // Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the scores go
-// through memory (4 bytes a row where a key has 128 or 256).
+// through memory (4 bytes a row where a key has 128 or 256).  One query on 65001 keys (32 heads of 64, 8 of keys): 21 us, 3.4 TB/s.  Blocks
+// that all fit the SMs at once: 26.6 -> 22.9 us against four per SM, of which three fit; the sum's loads issued together and before the
+// statistics: 21.3; heads of the same keys in neighbouring blocks: 21.0.  Twice the loads of a warp, or two batches in turn: 24.
 #include "hybrid_kernels.h"
 #include "hybrid_tcgen05.cuh"
 #include "sequence_kernels.h"
@@ -387,6 +389,7 @@ __global__ void __launch_bounds__(kTile) weights_add_kernel(const WeightArgs a) 
 
 // ---- up to 16 rows ------------------------------------------------------------------------------ //
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32, kAhead = 4;  // groups of 8 keys whose loads a warp has under way
+constexpr int few_blocks(int dim) { return dim == 64 ? 3 : 2; }  // per SM, by their registers
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -397,15 +400,15 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 // Rows are the M side, 8 keys the N side.  The contraction's order is free: lane (n, c) of a warp, n = lane / 4 and c = lane % 4, holds the
 // neighbours 8 c + 32 i .. + 7 of key n, two products' worth, so a key is read in 16-byte pieces straight into fragments.
 template <int kDim, int kRowsPad>
-__global__ void __launch_bounds__(kFewThreads) weights_few_kernel(const WeightArgs a) {
+__global__ void __launch_bounds__(kFewThreads, few_blocks(kDim)) weights_few_kernel(const WeightArgs a) {
     let_next();
     constexpr int kPieces = kDim / 32;
     __shared__ float2 shared[kFewWarps][kFew];
-    const Item it(a, blockIdx.y);
+    const Item it(a, blockIdx.x);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane / 4, c = lane % 4, before = it.n - a.queries;
     const bf16* const keys = a.k + it.layer * a.k_layer + it.b * a.k_sequence + it.g * kDim + c * 8;
     const int64_t key_row = (int64_t)a.kv_heads * kDim;
-    float* const scores = a.scores + (int64_t)blockIdx.y * a.positions * kRowsPad;
+    float* const scores = a.scores + (int64_t)blockIdx.x * a.positions * kRowsPad;
     uint32_t q[kPieces][2][4];  // rows n and n + 8
     int last[2];
 #pragma unroll
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(kFewThreads) weights_few_kernel(const WeightAr
             q[i][1][2 + h] = w.w;
         }
     }
-    const int groups = (it.n + 7) / 8, total = (int)gridDim.x * kFewWarps, me = (int)blockIdx.x * kFewWarps + warp;
+    const int groups = (it.n + 7) / 8, total = (int)gridDim.y * kFewWarps, me = (int)blockIdx.y * kFewWarps + warp;
     const int first = (int)((int64_t)groups * me / total), end = (int)((int64_t)groups * (me + 1) / total);
     float2 stats[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
     for (int g0 = first; g0 < end; g0 += kAhead) {
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(kFewThreads) weights_few_kernel(const WeightAr
     if (threadIdx.x < kFew) {
         float2 all = shared[0][threadIdx.x];
         for (int i = 1; i < kFewWarps; ++i) all = join(all, shared[i][threadIdx.x]);
-        a.stats[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kFew + threadIdx.x] = all;
+        a.stats[((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * kFew + threadIdx.x] = all;
     }
 }
 
@@ -477,7 +480,24 @@ __global__ void __launch_bounds__(kFewThreads) weights_sum_kernel(const WeightAr
     __shared__ float off[kFew];
     const Item it(a, blockIdx.y);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float* const scores = a.scores + (int64_t)blockIdx.y * a.positions * kRowsPad;
+    float* const weights = it.weights(a);
+    constexpr int kBatch = 4;  // keys of a thread whose loads are under way
+    const int step = gridDim.x * kFewThreads;
+    float4 z[kBatch][kRowsPad / 4];
+    float w[kBatch];
+    auto load = [&](int64_t j) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (j + (int64_t)i * step < it.n) {
+                w[i] = weights[j + i * step];
+#pragma unroll
+                for (int r = 0; r < kRowsPad / 4; ++r) z[i][r] = *reinterpret_cast<const float4*>(scores + (j + i * step) * kRowsPad + 4 * r);
+            }
+    };
+    int64_t j = (int64_t)blockIdx.x * kFewThreads + threadIdx.x;
     after_previous();
+    load(j);
     for (int r = warp; r < kRowsPad; r += kFewWarps) {
         const float2* const parts = a.stats + (int64_t)blockIdx.y * a.splits * kFew + r;
         float2 all = make_float2(-INFINITY, 0.f);
@@ -487,16 +507,20 @@ __global__ void __launch_bounds__(kFewThreads) weights_sum_kernel(const WeightAr
         if (lane == 0) off[r] = off_of(all.x, all.y);
     }
     __syncthreads();
-    const float* const scores = a.scores + (int64_t)blockIdx.y * a.positions * kRowsPad;
-    float* const weights = it.weights(a);
-    for (int j = blockIdx.x * kFewThreads + threadIdx.x; j < it.n; j += gridDim.x * kFewThreads) {
-        float sum = 0.f;
+    while (j < it.n) {
 #pragma unroll
-        for (int r = 0; r < kRowsPad; r += 4) {
-            const float4 z = *reinterpret_cast<const float4*>(scores + (int64_t)j * kRowsPad + r);
-            sum += (fast_exp2(z.x - off[r]) + fast_exp2(z.y - off[r + 1])) + (fast_exp2(z.z - off[r + 2]) + fast_exp2(z.w - off[r + 3]));
-        }
-        weights[j] += sum;
+        for (int i = 0; i < kBatch; ++i)
+            if (j + (int64_t)i * step < it.n) {
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < kRowsPad; r += 4) {
+                    const float4 x = z[i][r / 4];
+                    sum += (fast_exp2(x.x - off[r]) + fast_exp2(x.y - off[r + 1])) + (fast_exp2(x.z - off[r + 2]) + fast_exp2(x.w - off[r + 3]));
+                }
+                weights[j + i * step] = w[i] + sum;
+            }
+        j += (int64_t)kBatch * step;
+        if (j < it.n) load(j);
     }
 }
 
@@ -537,8 +561,8 @@ struct Plan {
         few = a.rows <= kFew;
         if (few) {
             rows_pad = a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : 16;
-            // four blocks per SM, none with less than 64 keys a warp
-            a.splits = up(4 * kSms, a.items);
+            // blocks that fit the SMs at once, none with less than 64 keys a warp
+            a.splits = few_blocks(w.dim) * kSms / a.items;
             if (a.splits > up(longest, 64 * kFewWarps)) a.splits = up(longest, 64 * kFewWarps);
             if (a.splits < 1) a.splits = 1;
             a.scores = reinterpret_cast<float*>(take((size_t)a.items * w.positions * rows_pad * 4));
@@ -606,7 +630,7 @@ cudaError_t launch(const MkbsKeyWeights& w, const Plan& p, cudaStream_t s) {
 
 template <int kDim, int kRowsPad>
 cudaError_t launch_few(const Plan& p, cudaStream_t s) {
-    weights_few_kernel<kDim, kRowsPad><<<dim3(p.a.splits, p.a.items), kFewThreads, 0, s>>>(p.a);
+    weights_few_kernel<kDim, kRowsPad><<<dim3(p.a.items, p.a.splits), kFewThreads, 0, s>>>(p.a);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     return launch_early(weights_sum_kernel<kRowsPad>, dim3(p.a.splits, p.a.items), dim3(kFewThreads), 0, s, p.a);
 }
