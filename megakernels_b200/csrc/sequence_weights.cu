@@ -8,11 +8,11 @@
 //   keys   a unit is 128 keys (M) and a run of rows, 128 at a time: a thread has a key and a quarter of the rows, so that a key's weight is a
 //          sum in registers; where there are few keys their rows are several units, and a small launch adds the parts.
 // The exponentials bound both (16 a clock and SM: 0.54 us for 128 x 128 scores at 1.9 GHz, products 0.07 - 0.13).  Sums of a row refer to a
-// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 44 us for 1501 queries on 1501
-// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 65 us for 64 queries on 32768 keys (32 heads
-// of 128, exponentials 30 us, keys at 0.5 TB/s): what a unit begins and ends with weighs there, since a key's rows are two steps.
-// Twice the columns a thread (half the warps) took 57 and 78 us, a polynomial for every fourth exponential 45 and 70, the next step's
-// scores fetched ahead 62 and 107 (registers).
+// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 43 us for 1501 queries on 1501
+// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 60 us for 64 queries on 32768 keys (32 heads
+// of 128, exponentials 30 us): what a unit begins and ends with weighs there, since a key's rows are two steps.  The four warps that share
+// a row or key also share a scheduler; had they to meet at a unit's end, it was 44 and 65.  Twice the columns a thread (half the warps) took
+// 57 and 78, a polynomial for every fourth exponential 45 and 70, the next step's scores fetched ahead 62 and 107 (registers).
 // Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the scores go
 // through memory (4 bytes a row where a key has 128 or 256).  One query on 65001 keys (32 heads of 64, 8 of keys): 21 us, 3.4 TB/s.  Blocks
 // that all fit the SMs at once: 26.6 -> 22.9 us against four per SM, of which three fit; the sum's loads issued together and before the
@@ -247,7 +247,33 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             __syncwarp();
             if (lane == 0) mkb::mbar_arrive(read(t));
         };
-        Unit<kKeys> unit;
+        Unit<kKeys> unit, last_unit;
+        auto cross = [&](int i) { return reinterpret_cast<float2*>(at + S::cross) + (i & 1) * kShares * kTile + lanes; };
+        auto join_last = [&] {  // of unit u - 1
+            if (u == 0) return true;
+            if (!wait_all(meeting(quarter), u - 1)) return false;
+            if (share != (u & (kShares - 1))) return true;  // (in turn)
+            const float2* const from = cross(u - 1);
+            const Item it(a, last_unit.item);
+            if constexpr (kKeys) {
+                float sum = from[0].y;
+#pragma unroll
+                for (int c = 1; c < kShares; ++c) sum += from[c * kTile].y;
+                const int j = last_unit.tile * kTile + lanes;
+                if (a.parts > 1) a.sums[(((int64_t)last_unit.item * a.parts + last_unit.part) * a.key_tiles + last_unit.tile) * kTile + lanes] = sum;
+                else if (j < it.n) atomicAdd(it.weights(a) + j, sum);  // (nothing else adds to it: an addition that nobody waits for)
+            } else {
+                const bool there = lanes < of_tile * a.per && last_unit.tile * of_tile * a.per + lanes < a.rows;
+                float2 all = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int c = 0; c < kShares; ++c)
+                    if (there) all = join(all, from[c * kTile]);
+                const int64_t row_tile = (int64_t)last_unit.item * a.row_tiles + last_unit.tile;
+                if (a.splits > 1) a.stats[(row_tile * a.splits + last_unit.part) * kTile + lanes] = all;
+                else a.offs[row_tile * kTile + lanes] = off_of(all.x, all.y);
+            }
+            return true;
+        };
         for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
             if (unit.count == 0 && (kKeys || unit.first < 0)) continue;
             const Item it(a, unit.item);
@@ -328,32 +354,16 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                 }
             }
             if (!ok) break;
-            // the threads of a row or key
-            float2* const cross = reinterpret_cast<float2*>(at + S::cross) + (u & 1) * kShares * kTile + lanes;
-            cross[share * kTile] = mine;
+            // The threads of a row or key: their parts are joined a unit later, so that the warps need not meet
+            ok = join_last();
+            if (!ok) break;
+            cross(u)[share * kTile] = mine;
             __syncwarp();
             if (lane == 0) mkb::mbar_arrive(meeting(quarter));
-            ok = wait_all(meeting(quarter), u);
+            last_unit = unit;
             ++u;
-            if (!ok || share != 0) continue;
-            if constexpr (kKeys) {
-                float sum = cross[0].y;
-#pragma unroll
-                for (int c = 1; c < kShares; ++c) sum += cross[c * kTile].y;
-                const int j = unit.tile * kTile + lanes;
-                if (a.parts > 1) a.sums[(((int64_t)unit.item * a.parts + unit.part) * a.key_tiles + unit.tile) * kTile + lanes] = sum;
-                else if (j < it.n) it.weights(a)[j] += sum;
-            } else {
-                const bool there = lanes < of_tile * a.per && unit.tile * of_tile * a.per + lanes < a.rows;
-                float2 all = make_float2(-INFINITY, 0.f);
-#pragma unroll
-                for (int c = 0; c < kShares; ++c)
-                    if (there) all = join(all, cross[c * kTile]);
-                const int64_t row_tile = (int64_t)unit.item * a.row_tiles + unit.tile;
-                if (a.splits > 1) a.stats[(row_tile * a.splits + unit.part) * kTile + lanes] = all;
-                else a.offs[row_tile * kTile + lanes] = off_of(all.x, all.y);
-            }
         }
+        if (ok) join_last();
     }
     tc_before_sync();
     __syncthreads();
