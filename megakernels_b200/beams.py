@@ -30,13 +30,18 @@ class BeamResult:
 
 def beam_search(gen, prompts, beams: int | None = None, ntok: int = 100, *, eos: int | None = None, length_penalty: float = 0.0,
                 check_interval: int = 16) -> BeamResult:
-    """Up to ``ntok`` tokens behind each prompt (one tensor of token ids, or a list of them).
+    """Up to ``ntok`` tokens behind each prompt: one tensor of token ids, a list of them, or a matrix with a prompt per row.
 
     At every step the ``beams`` best of a prompt's beams x vocabulary continuations go on (equal ones: the lowest
     beam, then the lowest token).  A beam that takes ``eos`` has ended: it competes with its score and is not
-    continued.  In the end beams are ordered by score / length ** ``length_penalty``.
+    continued.  In the end beams are ordered by score / length ** ``length_penalty``.  Every ``check_interval`` steps
+    the host looks whether all beams have ended.
     """
-    prompts = [p.reshape(-1) for p in ([prompts] if isinstance(prompts, Tensor) else prompts)]
+    if isinstance(prompts, Tensor):
+        prompts = list(prompts) if prompts.ndim == 2 else [prompts]
+    if any(p.numel() != max(p.shape, default=1) for p in prompts):
+        raise ValueError("a prompt is one row of token ids")
+    prompts = [p.reshape(-1) for p in prompts]
     sequences, positions = gen.beam_limits()
     beams = sequences // max(len(prompts), 1) if beams is None else beams
     ops = get_mk_module(name="mk_sequences")
@@ -44,6 +49,8 @@ def beam_search(gen, prompts, beams: int | None = None, ntok: int = 100, *, eos:
         raise ValueError("beam search needs prompts of a token and more")
     if not 1 <= beams <= min(ops.MAX_BEAMS, gen.model.config.vocab_size) or len(prompts) * beams > sequences:
         raise ValueError(f"{len(prompts)} prompts with {beams} beams each, of {sequences} sequences in all (at most {ops.MAX_BEAMS} beams)")
+    if check_interval < 1:
+        raise ValueError(f"a look at the beams every {check_interval} steps")
     if ntok < 1 or max(p.numel() for p in prompts) + ntok - 1 > positions:
         raise ValueError(f"{ntok} tokens behind a prompt of {max(p.numel() for p in prompts)}: there are {positions} positions")
     first, rows = min(p.numel() for p in prompts), len(prompts) * beams

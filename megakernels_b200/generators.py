@@ -13,6 +13,7 @@ import torch
 from torch import Tensor
 
 from megakernels_b200.beams import BeamResult, beam_search
+from megakernels_b200.demos.latency.instructions import LayerNorm_QKV_MatVecRopeAppend, RMS_LM_Head
 from megakernels_b200.demos.latency.mk import LatencyMK_Interpreter
 from megakernels_b200.demos.latency.scheduler import covers_model, make_globals
 from megakernels_b200.llama import build_rope_tables
@@ -290,12 +291,11 @@ class MK_Generator(Generator):
         what the cache holds of the sequence (a later turn of a chat); 0 starts a sequence.
         """
         ids = prompt_ids.reshape(1, -1)
-        globs = self.schedule.globs
+        at_once = self._takes_prompts(ids.shape[1], position)
+        if self.schedule.globs.key_weights is not None and not at_once:
+            raise ValueError("only prompts that go through the layers at once are observed")
         if position == 0:
             self._start_sequence()
-        at_once = self._takes_prompts(ids.shape[1], position)
-        if globs.key_weights is not None and not at_once:
-            raise ValueError("only prompts that go through the layers at once are observed")
         return self._prompt(ids, position) if at_once else self._steps(ids, 0, position)
 
     def _steps(self, ids: Tensor, done: int, first: int = 0) -> Tensor:
@@ -374,7 +374,8 @@ class MK_Generator(Generator):
     # -- beam search: the sequences of a batched launch are the beams ----------- #
     def beam_search(self, prompts, beams: int | None = None, ntok: int = 100, **kw) -> BeamResult:
         """The best continuations of one prompt, or of several at once, by beam search (``beams.beam_search`` has the
-        arguments).  The schedule's batch is prompts times beams.
+        arguments).  Beams are the first prompts times beams sequences of the schedule's batch, whose caches they overwrite; of the other
+        sequences' caches the first row is overwritten (a step decodes all of them).
         """
         return beam_search(self, prompts, beams, ntok, **kw)
 
@@ -383,17 +384,23 @@ class MK_Generator(Generator):
         globs = self.schedule.globs
         if globs.batch_size < 2 or not globs.hidden_states.is_cuda or self.skip_mk or self.skip_rest or getattr(self, "_graph", None) is not None:
             raise ValueError("beams need a batched schedule (LatencyScheduleOptions(batch_size=...)) whose steps are whole and not captured")
+        if globs.tp is not None or globs.residual_scale != 1.0:
+            raise ValueError("beams need the whole model on one GPU")
+        words = globs.instructions.reshape(-1, globs.instructions.shape[-1])
+        layers = words[words[:, 0] == LayerNorm_QKV_MatVecRopeAppend.opcode(), 1].unique().numel()
+        if layers != globs.num_hidden_layers or not bool((words[:, 0] == RMS_LM_Head.opcode()).any()):
+            raise ValueError(f"beams need a schedule of all layers and the head (it has {layers} of {globs.num_hidden_layers} layers)")
         return globs.batch_size, min(globs.k_cache.shape[2], globs.rope_cos.shape[0])
 
     def start_beams(self, prompts: list[Tensor], beams: int) -> Tensor:
         """Each prompt through the layers once, its cache rows handed to its beams; returns logits ``[prompts, vocab]``."""
         globs, ops = self.schedule.globs, get_mk_module(name="mk_sequences")
+        self._positions_before = globs.pos_id_device
         device = globs.hidden_states.device
         single = make_globals(self.model, skip_attn_reduction=True, max_attn_partitions=1)
         single.instructions = torch.zeros(1, 1, 32, dtype=torch.int32, device=device)  # (a prompt runs none)
         logits = globs.logits.new_empty(len(prompts), globs.vocab_size)
         slots = torch.arange(globs.k_cache.shape[1], dtype=torch.int32, device=device)
-        self._positions_before = globs.pos_id_device
         globs.pos_id_device = torch.zeros(globs.batch_size, dtype=torch.int32, device=device)
         for p in reversed(range(len(prompts))):  # (prompts go to slot 0: the first one's place)
             ids = prompts[p]
@@ -566,6 +573,9 @@ class Hybrid_Generator(MK_Generator):
     def beam_limits(self) -> tuple[int, int]:
         if getattr(self, "_graph", None) is not None or self.skip_mk or self.skip_rest:
             raise ValueError("beams need whole steps that are not captured")
+        most = get_mk_module(name="mk_sequences").MAX_SLOTS
+        if self.model.slots.count > most:
+            raise ValueError(f"beams need a pool of at most {most} slots")
         return self.model.slots.count - len(self.model.slots), self.model.max_len()
 
     _beam_slots: list[int] = []

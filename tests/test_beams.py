@@ -9,9 +9,11 @@ import torch
 
 from megakernels_b200.beams import beam_search
 from megakernels_b200.demos.latency.scheduler import LatencyScheduleOptions
-from megakernels_b200.dispatch import make_generator
+from megakernels_b200.dispatch import make_generator, make_mk_interpreter, make_schedule_builder
+from megakernels_b200.generators import MK_Generator
 from megakernels_b200.llama import LlamaConfig, LlamaForCausalLM, build_rope_tables
 from megakernels_b200.model_types import ExtraModelConfig
+from megakernels_b200.scheduler import assign_to_sms, tensorize_instructions
 from megakernels_b200.scripts.generate import main, parse_cli
 from tests.oracle_utils import seeded_tokens
 
@@ -66,6 +68,36 @@ class NoGenerator:
 def test_refused_searches(prompts, kw, said):
     with pytest.raises(ValueError, match=said):
         beam_search(NoGenerator(), prompts, **kw)
+
+
+@pytest.mark.parametrize("prompts,kw,said", [
+    ([torch.zeros(2, 3)], {}, "one row"), (torch.zeros(2, 2, 3), {}, "one row"), (torch.zeros(3), dict(check_interval=0, ntok=9), "every 0"), (torch.zeros(9, 3), dict(ntok=9), "beams"),
+    (torch.zeros(2, 0), dict(ntok=9), "prompts"),
+])
+def test_refused_prompts(prompts, kw, said):
+    """(Rows of a matrix are prompts: nine of them are too many for eight sequences.)"""
+    with pytest.raises(ValueError, match=said):
+        beam_search(NoGenerator(), prompts, **kw)
+
+
+class Failing(NoGenerator):
+    """Its prompts cannot run; what it held before comes back all the same."""
+
+    ended = 0
+
+    def start_beams(self, prompts, beams):
+        self.started = [p.tolist() for p in prompts], beams
+        raise RuntimeError("no memory")
+
+    def end_beams(self):
+        self.ended += 1
+
+
+def test_a_matrix_is_a_prompt_per_row_and_a_failed_search_ends():
+    gen = Failing()
+    with pytest.raises(RuntimeError, match="no memory"):
+        beam_search(gen, torch.arange(6).view(2, 3), ntok=5)
+    assert gen.started == ([[0, 1, 2], [3, 4, 5]], 4) and gen.ended == 1
 
 
 # ---- beam search ------------------------------------------------------------------------------------ #
@@ -233,6 +265,38 @@ def test_searches_that_cannot_run():
         batched.observe()
     with pytest.raises(ValueError, match="observed"):
         gen.evict(10, 5)
+
+
+@pytest.mark.gpu
+def test_searches_over_part_of_a_model():
+    """Prompts go through the whole model, so steps that do not are refused; a search that fails leaves positions as they were."""
+    batch = dict(num_attention_partitions=2, batch_size=2)
+    gen = make_generator(llama("1b", 2), LatencyScheduleOptions(**batch))
+    globs = gen.schedule.globs
+    globs.pos_id_device = mine = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(Exception):
+        gen.beam_search(torch.zeros(3, dtype=torch.float32), 2, 3)  # (embeddings are looked up by whole numbers)
+    assert globs.pos_id_device is mine
+    gen.replace_with_noops()
+    with pytest.raises(ValueError, match="0 of 2 layers"):
+        gen.beam_search(prompt(4, 0), 2, 3)
+    model = llama("1b", 2)
+    schedule = make_schedule_builder("latency", LatencyScheduleOptions(**batch)).build(model, layer_limit=1)
+    tensorize_instructions(schedule.globs, assign_to_sms("rr", schedule=schedule))
+    short = MK_Generator(model, make_mk_interpreter("latency"), schedule)
+    with pytest.raises(ValueError, match="layers"):
+        short.beam_search(prompt(4, 0), 2, 3)
+
+
+@pytest.mark.gpu
+def test_a_refused_prompt_leaves_the_sequence_before():
+    model, gen = observed_generator("1b", 64, 8)
+    gen.prefill(prompt(40, 1))
+    gen.evict(40, 30, 2, 4)
+    weights = gen.schedule.globs.key_weights.clone()
+    with pytest.raises(ValueError, match="observed"):
+        gen.prefill(prompt(65, 1))  # (more than the cache has)
+    assert gen.evicted == 10 and torch.equal(gen.schedule.globs.key_weights, weights) and weights.any()
 
 
 # ---- eviction ---------------------------------------------------------------------------------------- #
