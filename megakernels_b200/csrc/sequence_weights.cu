@@ -140,7 +140,6 @@ template <int kDim, bool kKeys>
 __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_constant__ WeightMaps maps, const WeightArgs a) {
     extern __shared__ uint8_t raw[];
     using S = Smem<kDim>;
-    let_next();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t raw32 = mkb::smem_u32(raw), base = (raw32 + 1023u) & ~1023u;
     char* const at = reinterpret_cast<char*>(raw) + (base - raw32);
@@ -179,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     __syncthreads();
     tc_after_sync();
     const uint32_t tmem = (uint32_t)ctl[1];
+    let_next();  // (not before: a block of the next launch that held tensor memory would wait for this one, and this one for the memory)
     if (kKeys) after_previous();  // (the offsets; the rows' launch is an ordinary one)
 
     const int of_tile = kTile / a.per, box_bytes = kDim / 64 * of_tile * a.per * 128;
