@@ -44,7 +44,7 @@ enum MkbsDtype { MKBS_BF16 = 0, MKBS_F32 = 1 };
  *
  * A logit that is minus infinity or not a number is a continuation of score minus infinity; so are all of a beam whose
  * score is not finite, or whose logits are all minus infinity.  They are taken, lowest (b, v) first, where there are no others.
- * Logits of plus infinity share their beam's whole probability.
+ * Logits of plus infinity share their beam's whole probability.  Outputs are not in the place of inputs.
  */
 typedef struct MkbsBeams {
     uint32_t struct_bytes;
@@ -73,7 +73,7 @@ int mkb_beam_select(const MkbsBeams *b, void *cuda_stream);
 /*
  * x[slot] <- x[parents[slot]] for all slots at once, in place, for every region.  Of a slot's rows those from `first` on that its
  * parent holds move (rows below `first` are alike in a slot and its parent: a shared prompt); what lies behind
- * lengths[parent] stays as it was.  A parent outside 0..slots-1 leaves its slot as it is.
+ * lengths[parent] stays as it was.  A parent outside 0..slots-1 leaves its slot as it is.  Regions share no bytes.
  */
 typedef struct MkbsRegion {
     void *base;

@@ -72,6 +72,8 @@ int check(const MkbsReorder* r) {
         if (!g.base || g.outer < 1 || g.rows < 1 || g.row_bytes < 1) return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: region %d is empty", i);
         if (g.row_bytes > (1 << 30) || g.slot_stride < g.rows * g.row_bytes || (g.outer > 1 && g.outer_stride < g.rows * g.row_bytes))
             return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: slots or layers of region %d overlap", i);
+        for (int j = 0; j < i; ++j)  // (blocks would move the same rows at once)
+            if (r->regions[j].base == g.base) return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: regions %d and %d are the same", j, i);
     }
     return MKBS_OK;
 }
@@ -120,6 +122,8 @@ int check(const MkbsSelect* s) {
     if (s->keep < 1 || s->sinks < 0 || s->recent < 0 || (int64_t)s->sinks + s->recent > s->keep)
         return invalid("select: keep must be positive and hold the sinks and the recent rows");
     if (!aligned(s->weights, 4) || !aligned(s->rows, 4) || (s->kept && !aligned(s->kept, 4))) return invalid("select: weights or rows missing or unaligned");
+    if (s->kept && ((s->kv_heads > 1 && s->w_head < s->positions) || (s->sequences > 1 && s->w_sequence < s->positions) || (s->layers > 1 && s->w_layer < s->positions)))
+        return invalid("select: kept weights overlap");
     return MKBS_OK;
 }
 
@@ -131,6 +135,7 @@ int check(const MkbsMove* m) {
         return fail(MKBS_ERR_UNSUPPORTED, "move: a head's part of a row is a multiple of 16 bytes, at most 1024");
     if (!aligned(m->rows, 4) || !aligned(m->caches[0], 16) || (m->caches[1] && !aligned(m->caches[1], 16)) || m->c_layer % 16 || m->c_sequence % 16)
         return invalid("move: rows or caches missing or unaligned");
+    if (m->caches[0] == m->caches[1]) return invalid("move: both caches are the same");
     const int64_t bytes = (int64_t)m->positions * m->kv_heads * m->head_bytes;
     if ((m->layers > 1 && m->c_layer < bytes) || (m->sequences > 1 && m->c_sequence < bytes)) return invalid("move: sequences or layers overlap");
     return MKBS_OK;

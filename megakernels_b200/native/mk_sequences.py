@@ -184,9 +184,9 @@ def _set_lengths(s, lengths, device: int, sequences: int, positions: int):
     if isinstance(lengths, Tensor):
         s.lengths = _check("lengths", lengths, torch.int32, device, (sequences,))
         return lengths
-    s.length = int(lengths)
-    if not 0 <= s.length <= positions:
+    if not 0 <= int(lengths) <= positions:
         raise ValueError(f"length {lengths} outside a cache of {positions} rows")
+    s.length = int(lengths)
     return None
 
 
@@ -269,6 +269,8 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
         r.slot_stride = t.stride(dim) * size if slots > 1 else slot_bytes
         r.rows = shape[dim + 1] if by_rows else 1
         r.row_bytes = slot_bytes // r.rows
+    if len(tensors) > MAX_REGIONS and len({r.base for r in regions}) < len(tensors):  # (the library sees those of a call)
+        raise ValueError("a tensor is listed twice")
     for at in range(0, len(tensors), MAX_REGIONS):
         base.num_regions = min(MAX_REGIONS, len(tensors) - at)
         base.regions = ctypes.cast(ctypes.byref(regions, at * ctypes.sizeof(MkbsRegion)), ctypes.POINTER(MkbsRegion))

@@ -82,10 +82,10 @@ def select_struct(**kw):
 
 def move_struct(**kw):
     s = fill(ops.MkbsMove, layers=2, sequences=2, kv_heads=2, positions=100, length=50, keep=10, head_bytes=128, c_layer=51200, c_sequence=25600)
-    s.caches[0] = s.caches[1] = FAKE
+    s.caches[0], s.caches[1] = FAKE, 2 * FAKE
     for name, v in kw.items():
-        if name == "cache":
-            s.caches[0] = v
+        if name in ("cache", "second"):
+            s.caches[name == "second"] = v
         else:
             setattr(s, name, v)
     return s
@@ -129,12 +129,12 @@ REFUSED = [
     ("select_rows", select_struct, [
         (dict(struct_bytes=8), 1, "struct size"), (dict(sequences=0), 1, "positive"), (dict(kv_heads=40000), 5, "65535"), (dict(length=101), 1, "length"), (dict(keep=0), 1, "keep"),
         (dict(sinks=-1), 1, "keep"), (dict(recent=-1), 1, "keep"), (dict(sinks=8, recent=3), 1, "keep"), (dict(weights=None), 1, "weights"), (dict(rows=FAKE + 2), 1, "rows"),
-        (dict(kept=FAKE + 2), 1, "unaligned"),
+        (dict(kept=FAKE + 2), 1, "unaligned"), (dict(kept=FAKE, w_head=99), 1, "overlap"), (dict(kept=FAKE, w_sequence=99), 1, "overlap"), (dict(kept=FAKE, w_layer=0), 1, "overlap"),
     ]),
     ("move_rows", move_struct, [
         (dict(struct_bytes=8), 1, "struct size"), (dict(layers=0), 1, "positive"), (dict(length=-1), 1, "length"), (dict(keep=0), 1, "keep"), (dict(head_bytes=8), 5, "16 bytes"),
         (dict(head_bytes=1040), 5, "1024"), (dict(rows=None), 1, "rows"), (dict(cache=None), 1, "caches"), (dict(cache=FAKE + 8), 1, "caches"), (dict(c_sequence=25592), 1, "unaligned"),
-        (dict(c_sequence=25584), 1, "overlap"), (dict(c_layer=25584), 1, "overlap"),
+        (dict(c_sequence=25584), 1, "overlap"), (dict(c_layer=25584), 1, "overlap"), (dict(second=FAKE), 1, "the same"),
     ]),
 ]
 
@@ -154,6 +154,27 @@ def test_only_the_device_is_missing_in_the_calls_that_the_refusals_start_from(na
     lib = ops.load_library()
     assert getattr(lib, f"mkb_{name}")(ctypes.byref(make()), None) == 2
     assert getattr(lib, f"mkb_{name}")(None, None) == 1
+
+
+def test_the_same_region_twice_is_refused():
+    """Two regions, then the same one twice."""
+    lib, s = ops.load_library(), reorder_struct()
+    regions = (ops.MkbsRegion * 2)(s._region, ops.MkbsRegion(2 * FAKE, 2, 10, 8000, 1000, 100))
+    s.regions, s.num_regions = ctypes.cast(regions, ctypes.POINTER(ops.MkbsRegion)), 2
+    if not torch.cuda.is_available():  # (with a device it would run)
+        assert lib.mkb_reorder_slots(ctypes.byref(s), None) == 2
+    regions[1].base = FAKE
+    assert lib.mkb_reorder_slots(ctypes.byref(s), None) == 1
+    assert "0 and 1 are the same" in lib.mkb_sequences_last_error().decode()
+
+
+@pytest.mark.parametrize("length", [-1, 101, 2**32 + 5, -(2**32) + 5])
+def test_a_length_outside_the_cache_is_refused(length):
+    s = ops._struct(ops.MkbsSelect)
+    with pytest.raises(ValueError, match="outside"):
+        ops._set_lengths(s, length, 0, 1, 100)
+    ops._set_lengths(s, 100, 0, 1, 100)
+    assert s.length == 100
 
 
 def test_beam_selection_takes_all_it_says_it_takes():
@@ -385,6 +406,18 @@ def test_reorder_of_a_large_cache():
     assert torch.equal(k[:, :, ::1000], rows[:, parents.long()]) and (k[1, 0, -1] == 7).all()
 
 
+@pytest.mark.gpu
+def test_reorder_of_many_tensors():
+    """More than a call of the library takes; none of them twice."""
+    tensors = [draw(i, 3, 16) for i in range(ops.MAX_REGIONS + 2)]
+    old, parents = [t.clone() for t in tensors], torch.tensor([2, 0, 0], dtype=torch.int32).cuda()
+    with pytest.raises(ValueError, match="twice"):
+        ops.reorder_slots([*tensors, tensors[0]], parents)
+    assert all(torch.equal(t, o) for t, o in zip(tensors, old))
+    ops.reorder_slots(tensors, parents)
+    assert all(torch.equal(t, o[parents.long()]) for t, o in zip(tensors, old))
+
+
 # ---- key weights ------------------------------------------------------------------------------------ #
 def weights_case(seed, layers, sequences, queries, heads, kv_heads, dim, positions, lengths, scale=None):
     q = draw(seed, layers, sequences, queries, heads, dim, dtype=BF16)
@@ -586,6 +619,35 @@ def test_move_rows_leaves_alone_what_it_is_not_told():
     for h, pairs in enumerate(({1: 5, 4: 9}, {0: 1, 1: 2, 2: 39})):
         for r in range(40):
             assert torch.equal(k[0, 0, r, h], old[0, 0, pairs.get(r, r), h])
+
+
+@pytest.mark.gpu
+def test_long_caches():
+    """Rows further than 2^31 elements from a cache's beginning (2^32 bytes and more): one key of each head draws all weight, and moves."""
+    kv_heads, dim, n = 32, 128, 530_000
+    k = torch.zeros(1, 1, n + 7, kv_heads, dim, dtype=BF16, device="cuda")
+    at = [n - 1 - 5 * h for h in range(kv_heads)]
+    assert min(at) * kv_heads * dim > 2**31
+    for h, j in enumerate(at):
+        k[0, 0, j, h, h] = 64
+    for queries in (1, 5):  # few rows, and many
+        q = torch.zeros(1, 1, queries, 4 * kv_heads, dim, dtype=BF16, device="cuda")
+        for h in range(kv_heads):
+            q[..., 4 * h : 4 * h + 4, h] = 4
+        w = torch.zeros(1, 1, kv_heads, n + 7, device="cuda")
+        ops.key_weights(q, k, w, n, scale=1.0)
+        want = torch.zeros(kv_heads, n + 7)
+        for h, j in enumerate(at):  # e^256 against n: the others get nothing; queries see the key from its own on
+            want[h, j] = 4 * sum(n - queries + t >= j for t in range(queries))
+        # (a query that does not see its head's key shares its weight out over the n keys that it sees)
+        spread = 4 * queries / (n - queries)
+        assert (w[0, 0].cpu() - want).abs().max() <= 1.01 * spread
+        assert torch.allclose(w[0, 0].double().sum(dim=1).cpu(), torch.full((kv_heads,), 4.0 * queries, dtype=torch.float64), rtol=2.0**-12, atol=0)
+    rows = ops.select_rows(w, n, keep=64, sinks=2, recent=4)
+    old = torch.stack([k[0, 0, rows[0, 0, h].long(), h] for h in range(kv_heads)])
+    assert all(j in rows[0, 0, h].tolist() for h, j in enumerate(at))
+    ops.move_rows(k, None, rows, n)
+    assert torch.equal(k[0, 0, :64].transpose(0, 1), old) and old.any()
 
 
 # ---- together --------------------------------------------------------------------------------------- #
