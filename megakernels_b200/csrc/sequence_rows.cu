@@ -1,4 +1,6 @@
 // Cache rows and states of sequences, moved in place: slots that take another slot's, and a cache cut to the rows that stay.
+#include <type_traits>
+
 #include "hybrid_common.cuh"
 #include "sequence_kernels.h"
 
@@ -267,35 +269,42 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 
 // ---- which rows stay ------------------------------------------------------------------------ //
 // A block per layer, sequence and head.  The weight of the last row that stays is found digit by digit (11, 11 and 10 bits
-// of its order) by counting; rows of that very weight stay in the order of their places.  The weights are read from memory
-// once: their orders lie in shared memory, as far as they fit, for the passes that follow, four at a time.  Then each warp has
-// a run of rows: it counts those that stay, and with the counts of the warps before it writes them.
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kDigits = 2048, kSelectAhead = 8;
+// of its order) by counting, until few rows share its digits: those are listed, and the rest of the digits is found among them.  Rows
+// of that very weight stay in the order of their places.  The weights are read from memory once: their orders lie in shared memory, as
+// far as they fit, for the passes that follow: digits (seldom), list, write.  A warp has a run of the rows in shared memory and one
+// of those behind; it counts those that stay, and with the counts of the runs before it writes them.
+// Instructions and what a pass begins and ends with bound it, not memory: 128 blocks of 65001 rows take 28 us (the weights at 1.2 TB/s;
+// with every digit found by a pass over all rows and no list 39), 448 of 4096 rows 13 (24, with 1024 threads each), 32 of 1500 5.7 (7.7).
+constexpr int kDigits = 2048, kSelectAhead = 8, kAtOnce = 4, kFewRows = 1536, kRanked = 256;
 constexpr int kMostOrders = (227 * 1024 - kStaticShared) / 16 * 4;
 
-__device__ __forceinline__ int inclusive_scan(int v, int lane) {
+__device__ __forceinline__ uint32_t inclusive_scan(uint32_t v, int lane) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int m = __shfl_up_sync(0xffffffffu, v, o);
+        const uint32_t m = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += m;
     }
     return v;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const MkbsSelect s, const int fit) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) select_kernel(const MkbsSelect s, const int fit) {
+    constexpr int kEach = kDigits / kThreads;
     extern __shared__ uint4 orders[];  // (a multiple of four of them)
-    __shared__ int count[kDigits], sums[2][kSelectWarps], found[2];
+    __shared__ __align__(16) int count[kDigits];
+    __shared__ int sums[32], found[3], few[kFewRows], listed;
+    __shared__ int above[2][32], ties[2][32];  // rows of the runs in shared memory, and behind: above the limit, at it
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, head = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
     const int n = length_of(s.lengths, s.length, s.positions, b), kept = min(n, s.keep);
     const int64_t at = layer * s.w_layer + b * s.w_sequence + head * s.w_head;
     const float* const w = s.weights + at;
     int32_t* const rows = s.rows + (((int64_t)layer * s.sequences + b) * s.kv_heads + head) * s.keep;
-    for (int r = kept + t; r < s.keep; r += kSelectThreads) rows[r] = -1;
+    for (int r = kept + t; r < s.keep; r += kThreads) rows[r] = -1;
     if (n <= s.keep) {
-        for (int r = t; r < n; r += kSelectThreads) rows[r] = r;
+        for (int r = t; r < n; r += kThreads) rows[r] = r;
         float* const out = s.kept != nullptr ? s.kept + at : nullptr;
         if (out != nullptr && out != w)
-            for (int r = t; r < n; r += kSelectThreads) out[r] = w[r];
+            for (int r = t; r < n; r += kThreads) out[r] = w[r];
         return;
     }
     const int rivals = n - s.sinks - s.recent, quads = (rivals + 3) / 4;  // rows that compete, from row `sinks` on
@@ -304,117 +313,280 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const MkbsSelect
     const bool some = need > 0;
     // order_of, not a number as minus infinity; what fills the last four up is below everything
     auto from_memory = [&](int i) { return i < rivals ? order_of(fmaxf(of_rivals[i], -INFINITY)) : 0u; };
-    auto four = [&](int q) { return make_uint4(from_memory(4 * q), from_memory(4 * q + 1), from_memory(4 * q + 2), from_memory(4 * q + 3)); };
     const int near = min(quads, fit / 4);  // in shared memory
-    auto fours = [&](int q, int to, int step, auto use) {
-#pragma unroll 4
-        for (; q < min(near, to); q += step) use(orders[q]);
-        for (; q < to; q += step) use(four(q));
+    auto run_of = [&](int part, int& from, int& to) {  // the warp's, whole turns of 32 lanes
+        const int all = part ? quads - near : near, run = (all + kThreads - 1) / kThreads * 32, first = part ? near : 0;
+        from = first + warp * run;
+        to = min(from + run, first + all);
+    };
+    auto load = [&](int part, int q0, int to, uint4 (&o)[kAtOnce]) {  // four rows of a lane, and those of the next turns
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int q = q0 + 32 * u + lane;
+            o[u] = make_uint4(0, 0, 0, 0);
+            if (q >= to) continue;
+            if (part == 0) o[u] = orders[q];
+            else o[u] = make_uint4(from_memory(4 * q), from_memory(4 * q + 1), from_memory(4 * q + 2), from_memory(4 * q + 3));
+        }
+    };
+    auto clear = [&] {
+#pragma unroll
+        for (int i = 0; i < kEach; i += 2) reinterpret_cast<int2*>(count)[i / 2 * kThreads + t] = make_int2(0, 0);
     };
     uint32_t limit = 0;
-    int shift = 32;
-    for (const int bits : {11, 11, 10}) {
-        shift -= bits;
-        for (int d = t; d < kDigits; d += kSelectThreads) count[d] = 0;
+    int shift = 32, size = rivals;  // rows that begin with the digits so far
+    // The digit from the counts, from the largest down, kEach per thread: how many rows lie above a digit
+    auto decide = [&] {
         __syncthreads();
-        if (shift + bits == 32) {
-            uint32_t* const kept_orders = reinterpret_cast<uint32_t*>(orders);
-            int i0 = t;
-            for (const int all = min(rivals, fit) - (kSelectAhead - 1) * kSelectThreads; i0 < all; i0 += kSelectAhead * kSelectThreads) {
-                float x[kSelectAhead];
+        const int d0 = kDigits - kEach * (t + 1);
+        int c[kEach], mine = 0;
 #pragma unroll
-                for (int u = 0; u < kSelectAhead; ++u) x[u] = of_rivals[i0 + u * kSelectThreads];
-#pragma unroll
-                for (int u = 0; u < kSelectAhead; ++u) {
-                    const uint32_t o = order_of(fmaxf(x[u], -INFINITY));
-                    kept_orders[i0 + u * kSelectThreads] = o;
-                    atomicAdd(&count[o >> shift], 1);
-                }
-            }
-            for (; i0 < 4 * quads; i0 += kSelectAhead * kSelectThreads) {
-                uint32_t o[kSelectAhead];
-#pragma unroll
-                for (int u = 0; u < kSelectAhead; ++u) o[u] = from_memory(i0 + u * kSelectThreads);
-#pragma unroll
-                for (int u = 0; u < kSelectAhead; ++u) {
-                    const int i = i0 + u * kSelectThreads;
-                    if (i < 4 * near) kept_orders[i] = o[u];
-                    if (i < rivals) atomicAdd(&count[o[u] >> shift], 1);
-                }
-            }
-        } else {
-            auto look = [&](uint32_t o) {  // (what does not begin with the digits so far is beyond the last one: orders end at 0xff800000)
-                const uint32_t digit = (o - limit) >> shift;
-                if (digit < 1u << bits) atomicAdd(&count[digit], 1);
-            };
-            fours(t, quads, kSelectThreads, [&](const uint4& o) { look(o.x), look(o.y), look(o.z), look(o.w); });
+        for (int i = 0; i < kEach; i += 2) {
+            const int2 two = *reinterpret_cast<const int2*>(count + d0 + i);
+            c[i] = two.x, c[i + 1] = two.y;
+            mine += two.x + two.y;
         }
+        int before = inclusive_scan(mine, lane);
+        if (lane == 31) sums[warp] = before;
         __syncthreads();
-        // digits from the largest down, two per thread: how many rows lie above a digit
-        const int d = kDigits - 1 - 2 * t, c0 = count[d], c1 = count[d - 1];
-        int before = inclusive_scan(c0 + c1, lane);
-        if (lane == 31) sums[0][warp] = before;
+        before += __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0) - mine;
+#pragma unroll
+        for (int i = kEach - 1; i >= 0; --i) {
+            if (before < need && need <= before + c[i]) found[0] = d0 + i, found[1] = before, found[2] = c[i];
+            before += c[i];
+        }
+        clear();  // (all have read)
         __syncthreads();
-        before -= c0 + c1;
-        for (int i = 0; i < warp; ++i) before += sums[0][i];
-        if (before < need && need <= before + c0) found[0] = d, found[1] = before;
-        if (before + c0 < need && need <= before + c0 + c1) found[0] = d - 1, found[1] = before + c0;
-        __syncthreads();
-        if (some) {
-            limit |= (uint32_t)found[0] << shift;
-            need -= found[1];
+        limit |= (uint32_t)found[0] << shift;
+        need -= found[1];
+        size = found[2];
+    };
+    auto next_digit = [&] {
+        const int bits = shift > 10 ? 11 : 10;
+        shift -= bits;
+        return 1u << bits;
+    };
+    clear();
+    if (t < 64) (&above[0][0])[t] = (&ties[0][0])[t] = 0;
+    if (t == 0) listed = 0;
+    __syncthreads();
+    next_digit();
+    {
+        uint32_t* const kept_orders = reinterpret_cast<uint32_t*>(orders);
+        int i0 = t;
+        for (const int all = min(rivals, fit) - (kSelectAhead - 1) * kThreads; i0 < all; i0 += kSelectAhead * kThreads) {
+            float x[kSelectAhead];
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) x[u] = of_rivals[i0 + u * kThreads];
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) {
+                const uint32_t o = order_of(fmaxf(x[u], -INFINITY));
+                kept_orders[i0 + u * kThreads] = o;
+                atomicAdd(&count[o >> shift], 1);
+            }
+        }
+        for (; i0 < 4 * quads; i0 += kSelectAhead * kThreads) {
+            uint32_t o[kSelectAhead];
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) o[u] = from_memory(i0 + u * kThreads);
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) {
+                const int i = i0 + u * kThreads;
+                if (i < 4 * near) kept_orders[i] = o[u];
+                if (i < rivals) atomicAdd(&count[o[u] >> shift], 1);
+            }
         }
     }
     if (some) {
-        // Rows above the limit stay, and the first `need` at it.  A warp's run is whole turns of 32 lanes with four rows each
-        const int run = (quads + kSelectThreads - 1) / kSelectThreads * 32, from = warp * run, to = min(from + run, quads);
-        auto above_and_at = [&](const uint4& o) {  // how many, the latter times 2^16
-            return (o.x > limit) + (o.y > limit) + (o.z > limit) + (o.w > limit) + (((o.x == limit) + (o.y == limit) + (o.z == limit) + (o.w == limit)) << 16);
-        };
-        int above = 0, ties = 0;
-        fours(from + lane, to, 32, [&](const uint4& o) {
-            const int both = above_and_at(o);
-            above += both & 0xffff;
-            ties += both >> 16;
-        });
-        above = __reduce_add_sync(0xffffffffu, above);
-        ties = __reduce_add_sync(0xffffffffu, ties);
-        if (lane == 0) sums[0][warp] = above, sums[1][warp] = ties;
-        __syncthreads();
-        int out = s.sinks, tied = 0;
-        for (int i = 0; i < warp; ++i) {
-            out += sums[0][i];
-            tied += sums[1][i];
-        }
-        for (int q0 = from; q0 < to; q0 += 32) {
-            const int q = q0 + lane;
-            const uint4 o = q >= to ? make_uint4(0, 0, 0, 0) : q < near ? orders[q] : four(q);
-            const int both = above_and_at(o), upto = inclusive_scan(both, lane), before = upto - both;
-            int place = out + (before & 0xffff), tie = tied + (before >> 16);
-            const uint32_t each[4] = {o.x, o.y, o.z, o.w};
+        decide();
+        while (shift > 0 && size > kFewRows) {
+            const uint32_t digits = next_digit();
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+                int from, to;
+                run_of(part, from, to);
+#pragma unroll 1
+                for (int q0 = from; q0 < to; q0 += 32 * kAtOnce) {
+                    uint4 o[kAtOnce];
+                    load(part, q0, to, o);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool is_tie = each[i] == limit;
-                if (each[i] > limit || (is_tie && tie < need)) rows[place + min(tie, need)] = s.sinks + 4 * q + i;
-                place += each[i] > limit;
-                tie += is_tie;
+                    for (int u = 0; u < kAtOnce; ++u) {
+                        const uint32_t each[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {  // (what does not begin with the digits so far is beyond the last one: orders end at 0xff800000)
+                            const uint32_t digit = (each[i] - limit) >> shift;
+                            if (digit < digits) atomicAdd(&count[digit], 1);
+                        }
+                    }
+                }
             }
-            const int all = __shfl_sync(0xffffffffu, upto, 31);
-            out += all & 0xffff;
-            tied += all >> 16;
+            decide();
         }
+        // Rows above all that begin with the digits, of each run, and a list of those that do, or how many they are when no digit is left
+        const uint32_t span = shift > 0 ? (1u << shift) - 1 : 0;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+            int from, to, up = 0, at_it = 0;
+            run_of(part, from, to);
+#pragma unroll 1
+            for (int q0 = from; q0 < to; q0 += 32 * kAtOnce) {
+                uint4 o[kAtOnce];
+                load(part, q0, to, o);
+                uint32_t within = 0;  // a bit for each row
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const uint32_t each[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        up += each[i] > limit + span;
+                        within |= each[i] - limit <= span ? 1u << (4 * u + i) : 0u;
+                    }
+                }
+                const int have = __popc(within);
+                at_it += have;
+                if (have && shift > 0) {
+                    for (int to_list = atomicAdd(&listed, have); within; within &= within - 1) {  // (`size` of them in all)
+                        const int bit = __ffs(within) - 1;
+                        few[to_list++] = 4 * (q0 + 32 * (bit / 4) + lane) + bit % 4;
+                    }
+                }
+            }
+            up = __reduce_add_sync(0xffffffffu, up);
+            if (shift == 0) at_it = __reduce_add_sync(0xffffffffu, at_it);
+            if (lane == 0) {
+                above[part][warp] = up;
+                if (shift == 0) ties[part][warp] = at_it;
+            }
+        }
+        if (shift > 0) {
+            __syncthreads();
+            constexpr int kMine = (kFewRows + kThreads - 1) / kThreads;
+            const int all = size;
+            int place[kMine];
+            uint32_t own[kMine];
+#pragma unroll
+            for (int u = 0; u < kMine; ++u) {
+                const int e = t + u * kThreads;
+                place[u] = e < all ? few[e] : -1;
+                own[u] = e >= all ? 0u : place[u] < 4 * near ? reinterpret_cast<const uint32_t*>(orders)[place[u]] : from_memory(place[u]);
+            }
+            if (size <= kRanked) {  // ranked by counting
+                if (t < kRanked) reinterpret_cast<uint32_t*>(count)[t] = own[0];  // (0 behind the list)
+                __syncthreads();
+                if (t < size) {
+                    int before = 0, alike = 0;
+#pragma unroll 4
+                    for (int e = 0; e < size; e += 4) {
+                        const uint4 o = *reinterpret_cast<const uint4*>(count + e);
+                        before += (o.x > own[0]) + (o.y > own[0]) + (o.z > own[0]) + (o.w > own[0]);
+                        alike += (o.x == own[0]) + (o.y == own[0]) + (o.z == own[0]) + (o.w == own[0]);
+                    }
+                    if (before < need && need <= before + alike) found[0] = (int)own[0], found[1] = before;  // (all that are alike write the same)
+                }
+                __syncthreads();
+                limit = (uint32_t)found[0];
+                need -= found[1];
+                shift = 0;
+            }
+            while (shift > 0) {
+                const uint32_t digits = next_digit();
+#pragma unroll
+                for (int u = 0; u < kMine; ++u) {
+                    const uint32_t digit = (own[u] - limit) >> shift;
+                    if (place[u] >= 0 && digit < digits) atomicAdd(&count[digit], 1);
+                }
+                decide();
+            }
+#pragma unroll
+            for (int u = 0; u < kMine; ++u)
+                if (place[u] >= 0 && own[u] >= limit) {
+                    const bool far = place[u] / 4 >= near;
+                    const int of = far ? quads - near : near, run = (of + kThreads - 1) / kThreads * 32;
+                    atomicAdd(own[u] > limit ? &above[far][(place[u] / 4 - (far ? near : 0)) / run] : &ties[far][(place[u] / 4 - (far ? near : 0)) / run], 1);
+                }
+        }
+        __syncthreads();
+        // Rows above the limit stay, and the first `need` at it: mostly all of those
+        auto in_runs = [&](const int (&of)[2][32], int part) {  // before the warp's run of that part
+            return __reduce_add_sync(0xffffffffu, (part || lane < warp ? of[0][lane] : 0) + (part && lane < warp ? of[1][lane] : 0));
+        };
+        auto write = [&](auto all_stay) {
+            constexpr bool kAllStay = decltype(all_stay)::value;
+            auto stays = [&](uint32_t order) { return kAllStay ? order >= limit : order > limit; };
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+                int from, to;
+                run_of(part, from, to);
+                if (from >= to) continue;
+                const int ties_before = in_runs(ties, part);
+                int out = s.sinks + in_runs(above, part) + (kAllStay ? ties_before : 0), tied = ties_before;
+#pragma unroll 1
+                for (int q0 = from; q0 < to; q0 += 32 * kAtOnce) {
+                    uint4 o[kAtOnce];
+                    load(part, q0, to, o);
+                    uint32_t ups = 0, ats = 0;          // how many of a turn, a byte for each (up to 128 rows of one)
+                    uint32_t up_bits = 0, at_bits = 0;  // which of the lane's
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u) {
+                        const uint32_t each[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (stays(each[i])) up_bits |= 1u << (4 * u + i);
+                            if (!kAllStay && each[i] == limit) at_bits |= 1u << (4 * u + i);
+                        }
+                        ups |= (uint32_t)__popc(up_bits >> 4 * u & 15) << 8 * u;
+                        if (!kAllStay) ats |= (uint32_t)__popc(at_bits >> 4 * u & 15) << 8 * u;
+                    }
+                    const uint32_t ups_upto = inclusive_scan(ups, lane), ups_all = __shfl_sync(0xffffffffu, ups_upto, 31);
+                    uint32_t ats_upto = 0, ats_all = 0;
+                    if (!kAllStay) {
+                        ats_upto = inclusive_scan(ats, lane);
+                        ats_all = __shfl_sync(0xffffffffu, ats_upto, 31);
+                    }
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u) {
+                        uint32_t stay = up_bits >> 4 * u & 15;
+                        int place = out + ((ups_upto - ups) >> 8 * u & 255);
+                        if (!kAllStay) {
+                            const int tie = tied + ((ats_upto - ats) >> 8 * u & 255);
+                            uint32_t at_it = at_bits >> 4 * u & 15;
+                            while (__popc(at_it) > max(need - tie, 0)) at_it &= ~(1u << (31 - __clz(at_it)));  // (the first ones stay)
+                            stay |= at_it;
+                            place += min(tie, need);
+                        }
+                        int32_t* put = rows + place;
+                        const int first = s.sinks + 4 * (q0 + 32 * u + lane);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (stay >> i & 1) *put++ = first + i;
+                        out += ups_all >> 8 * u & 255;
+                        tied += ats_all >> 8 * u & 255;
+                    }
+                }
+            }
+        };
+        if (__reduce_add_sync(0xffffffffu, ties[0][lane] + ties[1][lane]) == need) write(std::true_type());
+        else write(std::false_type());
     }
-    for (int r = t; r < s.sinks; r += kSelectThreads) rows[r] = r;
-    for (int r = t; r < s.recent; r += kSelectThreads) rows[s.keep - s.recent + r] = n - s.recent + r;
+    for (int r = t; r < s.sinks; r += kThreads) rows[r] = r;
+    for (int r = t; r < s.recent; r += kThreads) rows[s.keep - s.recent + r] = n - s.recent + r;
     if (s.kept == nullptr) return;
     // In their order: weights to come lie behind those that have been written
     float* const put = s.kept + at;
-    for (int r0 = 0; r0 < s.keep; r0 += kSelectThreads) {
-        const int r = r0 + t;
+    for (int r0 = 0; r0 < s.keep; r0 += kSelectAhead * kThreads) {
+        float x[kSelectAhead];
         __syncthreads();
-        const float x = r < s.keep ? w[rows[r]] : 0.f;
+#pragma unroll
+        for (int u = 0; u < kSelectAhead; ++u) {
+            const int r = r0 + u * kThreads + t;
+            x[u] = r < s.keep ? w[rows[r]] : 0.f;
+        }
         __syncthreads();
-        if (r < s.keep) put[r] = x;
+#pragma unroll
+        for (int u = 0; u < kSelectAhead; ++u) {
+            const int r = r0 + u * kThreads + t;
+            if (r < s.keep) put[r] = x[u];
+        }
     }
 }
 
@@ -489,6 +661,13 @@ cudaError_t reorder(const ReorderArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+template <int kThreads>
+cudaError_t select(const MkbsSelect& a, int fit, cudaStream_t s) {
+    if (const cudaError_t e = allow_shared_memory<select_kernel<kThreads>>(); e != cudaSuccess) return e;
+    select_kernel<kThreads><<<dim3(a.kv_heads, a.sequences, a.layers), kThreads, fit * 4, s>>>(a, fit);
+    return cudaGetLastError();
+}
+
 }  // namespace
 
 cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
@@ -505,15 +684,15 @@ cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
 }
 
 cudaError_t select_launch(const MkbsSelect& a, cudaStream_t s) {
-    if (const cudaError_t e = allow_shared_memory<select_kernel>(); e != cudaSuccess) return e;
     const int longest = a.lengths != nullptr ? a.positions : a.length, fit = longest <= a.keep ? 0 : longest < kMostOrders ? (longest + 3) / 4 * 4 : kMostOrders;
-    select_kernel<<<dim3(a.kv_heads, a.sequences, a.layers), kSelectThreads, fit * 4, s>>>(a, fit);
-    return cudaGetLastError();
+    // Few warps for few rows: 512 blocks of 4096 rows take 11.8, 17.4, 31.8 us with 256, 512 and 1024 threads, 8 blocks 6.7, 6.7, 8.9; of 16384
+    // rows 31, 30, 37 and 11.8, 10.9, 9.8; of 32768 rows 73, 56, 52 and 18.6, 14.6, 14.2
+    return fit <= 8192 ? select<256>(a, fit, s) : fit <= 16384 ? select<512>(a, fit, s) : select<1024>(a, fit, s);
 }
 
 cudaError_t move_launch(const MkbsMove& m, cudaStream_t s) {
     // A block and more for every SM, none with less than 32 bytes of a row, a sector (64 blocks of 256-byte rows, 512 of 1500 kept: with
-    // 1, 2, 4 parts 14.4, 11.9, 11.4 us with the selection; 256 blocks of 128-byte rows, 8192 of 65001: 152, 157, 160)
+    // 1, 2, 4 parts 14.4, 11.9, 11.4 us with the selection as it was then; 256 blocks of 128-byte rows, 8192 of 65001: 152, 157, 160)
     int parts = 1;
     while (m.kv_heads * 2 * m.sequences * m.layers * parts < kSms && m.head_bytes % (64 * parts) == 0) parts *= 2;
     if (const cudaError_t e = allow_shared_memory<move_kernel>(); e != cudaSuccess) return e;

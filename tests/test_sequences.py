@@ -569,6 +569,16 @@ def test_select_rows(positions, lengths, keep, sinks, recent):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [700, 8191, 8197, 16384, 16385, 54016 + 9, 60_001])
+def test_select_rows_of_weights_that_begin_alike(n):
+    """All of one leading digit, of two, and of few values: none, some or most of the rows share what the limit begins with."""
+    x = draw(n, 1, 2, 3, n).abs() % 1
+    for w in (1 + x / 8, 1 + x * 2**-14, 1 + (x * 50).round() / 512, x * 3):
+        for keep in (n // 10, n - 70):
+            check_rows(w, [n, n - 13], keep, 3, 20)
+
+
+@pytest.mark.gpu
 def test_select_rows_of_unusual_weights():
     n = 2500
     for fill in (0.0, -1.0, -math.inf, math.inf, math.nan):
