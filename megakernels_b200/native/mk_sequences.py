@@ -149,7 +149,7 @@ class _Where:
     def __init__(self, stream, of: Tensor):
         self.device, self.where = torch.cuda.current_device(), of.device
         if stream is None:
-            self.other, self.handle = None, torch.cuda.current_stream(self.device).cuda_stream
+            self.other, self.handle = None, torch._C._cuda_getCurrentRawStream(self.device)  # (0.1 us; as an object 1.3)
         elif isinstance(stream, int):  # (an external stream of handle 0 would be another one from torch's pool)
             self.other = torch.cuda.ExternalStream(stream, device=self.device) if stream else torch.cuda.default_stream(self.device)
             self.handle = stream
@@ -254,10 +254,15 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
     if by_rows:
         base.lengths = _check("lengths", lengths, torch.int32, device, (slots,))
     regions = (MkbsRegion * len(tensors))()
-    for r, (i, t) in zip(regions, enumerate(tensors)):
+    like = strides = None
+    for i, t in enumerate(tensors):
+        if like is not None and isinstance(t, Tensor) and t.shape == shape and t.dtype is like.dtype and t.get_device() == device and t.stride() == strides:
+            regions[i] = regions[i - 1]  # (a layer's states are mostly as the one's before)
+            regions[i].base = t.data_ptr()
+            continue
         if not isinstance(t, Tensor):
             raise TypeError(f"tensor {i} must be a torch.Tensor")
-        shape = t.shape
+        like, shape, strides, r = t, t.shape, t.stride(), regions[i]
         if len(shape) < dim + 1 + by_rows or shape[dim] != slots:
             raise ValueError(f"tensor {i} {list(shape)} does not have {slots} slots in dimension {dim}" + (" and rows behind it" if by_rows else ""))
         if t.numel() == 0:
@@ -265,8 +270,8 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
         r.base = _check(f"tensor {i}", t, t.dtype, device, inner=len(shape) - dim - 1)
         size = t.element_size()
         slot_bytes = math.prod(shape[dim + 1 :]) * size
-        r.outer, r.outer_stride = (shape[0], t.stride(0) * size) if dim else (1, 0)
-        r.slot_stride = t.stride(dim) * size if slots > 1 else slot_bytes
+        r.outer, r.outer_stride = (shape[0], strides[0] * size) if dim else (1, 0)
+        r.slot_stride = strides[dim] * size if slots > 1 else slot_bytes
         r.rows = shape[dim + 1] if by_rows else 1
         r.row_bytes = slot_bytes // r.rows
     if len(tensors) > MAX_REGIONS and len({r.base for r in regions}) < len(tensors):  # (the library sees those of a call)
