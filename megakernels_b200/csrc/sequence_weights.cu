@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             __syncwarp();
             if (lane == 0) mkb::mbar_arrive(read(t));
         };
-        Unit<kKeys> unit, last_unit;
+        Unit<kKeys> unit, last_unit = {};
         auto cross = [&](int i) { return reinterpret_cast<float2*>(at + S::cross) + (i & 1) * kShares * kTile + lanes; };
         auto join_last = [&] {  // of unit u - 1
             if (u == 0) return true;

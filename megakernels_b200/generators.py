@@ -325,7 +325,20 @@ class MK_Generator(Generator):
             globs.key_weights = torch.zeros(L, Hkv, T, dtype=torch.float32, device=globs.k_cache.device)
             # rows and positions part ways with the first eviction: tables by row, of this generator alone
             globs.rope_cos, globs.rope_sin = globs.rope_cos.clone(), globs.rope_sin.clone()
+            self._turns(2 * globs.rope_cos.shape[0])
         self.observed = window
+
+    _more_turns: tuple[Tensor, Tensor] | None = None
+
+    def _turns(self, count: int) -> tuple[Tensor, Tensor]:
+        """Rotation tables of ``count`` positions or more.  (They are made on the host, a few ms for a long cache: ahead of evictions.)"""
+        model = self.model
+        tables = self._more_turns or (model.model.rope_cos, model.model.rope_sin)
+        have, rows = tables[0].shape[0], self.schedule.globs.rope_cos.shape[0]
+        if have < count:
+            more = build_rope_tables(model.config, max(count - have, rows), model.extra_config.interleave_rope, have)
+            tables = self._more_turns = tuple(torch.cat([t, m.to(t)]) for t, m in zip(tables, more))
+        return tables
 
     def _start_sequence(self) -> None:
         globs = self.schedule.globs
@@ -335,14 +348,13 @@ class MK_Generator(Generator):
 
     def _turn_to(self, evicted: int) -> None:
         """Rows of the cache from the next one on are ``evicted`` positions further than they say."""
-        globs, model = self.schedule.globs, self.model
+        globs = self.schedule.globs
         if evicted == self.evicted:
             return
-        tables = (model.model.rope_cos, model.model.rope_sin)
-        if evicted:
-            tables = build_rope_tables(model.config, globs.rope_cos.shape[0], model.extra_config.interleave_rope, evicted)
-        globs.rope_cos.copy_(tables[0])
-        globs.rope_sin.copy_(tables[1])
+        rows = globs.rope_cos.shape[0]
+        cos, sin = self._turns(evicted + rows)
+        globs.rope_cos.copy_(cos[evicted : evicted + rows])
+        globs.rope_sin.copy_(sin[evicted : evicted + rows])
         self.evicted = evicted
 
     def evict(self, length: int, keep: int, sinks: int = 4, recent: int = 64) -> int:

@@ -395,6 +395,23 @@ def test_evicted_cache_goes_on_as_one_laid_out_by_hand(shape, count, keep, sinks
 
 
 @pytest.mark.gpu
+def test_rotations_after_many_evictions():
+    """Tables by row for the position that a row's token has, however many rows have gone; a new sequence begins at 0."""
+    model, gen = observed_generator("1b", 64, 8)
+    globs, at = gen.schedule.globs, 0
+    first = [globs.rope_cos.clone(), globs.rope_sin.clone()]
+    for turn in range(8):
+        gen.prefill(prompt(60 - at, turn), position=at)
+        at = gen.evict(60, 20, 2, 4)
+        assert gen.evicted == 40 * (turn + 1)
+        want = build_rope_tables(model.config, globs.rope_cos.shape[0], True, first=gen.evicted)
+        assert torch.equal(globs.rope_cos.cpu(), want[0]) and torch.equal(globs.rope_sin.cpu(), want[1])
+    gen.prefill(prompt(10, 9))
+    gen.check()
+    assert gen.evicted == 0 and torch.equal(globs.rope_cos, first[0]) and torch.equal(globs.rope_sin, first[1])
+
+
+@pytest.mark.gpu
 def test_tokens_observed_one_at_a_time():
     """A prompt cut into single tokens is weighed as it is at once.  Queries and keys of other products differ by the last bit of bf16 here and
     there: single weights by a few hundredths, a query's sum only by the rounding of its own terms."""
