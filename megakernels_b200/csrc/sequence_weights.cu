@@ -96,13 +96,16 @@ __device__ __forceinline__ void load_queries(uint32_t dst, const CUtensorMap* ma
                      : "memory");
 }
 
-// Shared memory: two operands of units, a ring of operands of their steps with 512 bytes each.
+constexpr int kUnits = 8;  // that are described ahead.  Two operands are held, and scores wait in kBuffers buffers, so no warp is further behind
+static_assert(kUnits >= kBuffers + 3, "units between the copies and the last warp that sums");
+// Shared memory: two operands of units, a ring of operands of their steps with 512 bytes each, units.
 template <int kDim>
 struct Smem {
     static constexpr int kOperand = kDim / 64 * kSlab, kExtra = 512, kHeld = 2;
     static constexpr int stages = kDim == 64 ? 6 : 4;
     static constexpr int ring = kHeld * kOperand, extra = ring + stages * kOperand, cross = extra + stages * kExtra;
-    static constexpr int bars = cross + 2 * kShares * kTile * 8, ctl = bars + (2 * kHeld + 2 * stages + 2 * kBuffers + 4) * 8, total = ctl + 16 + 1024;
+    static constexpr int units = cross + 2 * kShares * kTile * 8, bars = units + kUnits * 32;
+    static constexpr int ctl = bars + (2 * kHeld + 2 * stages + 2 * kBuffers + 4 + kUnits) * 8, total = ctl + 16 + 1024;
     static_assert(total <= 227 * 1024 - kStaticShared, "shared memory of a block");
 };
 
@@ -152,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     auto scored = [&](int t) { return bar(4 + 2 * S::stages + t % kBuffers); };
     auto read = [&](int t) { return bar(4 + 2 * S::stages + kBuffers + t % kBuffers); };
     auto meeting = [&](int i) { return bar(4 + 2 * S::stages + 2 * kBuffers + i); };
+    auto described = [&](int u) { return bar(4 + 2 * S::stages + 2 * kBuffers + 4 + u % kUnits); };
     auto held = [&](int i) { return base + (i & 1) * S::kOperand; };
     auto stage = [&](int t) { return base + S::ring + t % S::stages * S::kOperand; };
     auto wait = [&](uint32_t b, int turn, int role) { return tc_wait(b, (uint32_t)turn & 1u, ctl, a.timeout_ns, a.status, role); };
@@ -166,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         for (int i = 0; i < S::stages; ++i) mkb::mbar_init(full(i), 1), mkb::mbar_init(empty(i), kKeys ? 1 + kWarps : 1);
         for (int i = 0; i < kBuffers; ++i) mkb::mbar_init(scored(i), 1), mkb::mbar_init(read(i), kWarps);
         for (int i = 0; i < 4; ++i) mkb::mbar_init(meeting(i), kShares);
+        for (int i = 0; i < kUnits; ++i) mkb::mbar_init(described(i), 1);
         ctl[0] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -182,58 +187,96 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     if (kKeys) after_previous();  // (the offsets; the rows' launch is an ordinary one)
 
     const int of_tile = kTile / a.per, box_bytes = kDim / 64 * of_tile * a.per * 128;
-    if (warp == 0 && lane == 0) {
+    // (Both roles run as whole warps with a chosen lane: on one lane of a diverged warp every operand of an instruction of this kind is
+    // first moved to a uniform register.)
+    auto wait_whole = [&](uint32_t b, int turn, int role) { return __all_sync(0xffffffffu, wait(b, turn, role)); };
+    if (warp == 0) {
+        const bool chosen = tc_elect();
         bool ok = true;
         int t = 0, u = 0;
         Unit<kKeys> unit;
+        auto describe = [&] {  // unit u, for the other warps; (what the place held before has been read, as held_empty says)
+            if (chosen) {
+                int4* const to = reinterpret_cast<int4*>(at + S::units + u % kUnits * 32);
+                to[0] = make_int4(unit.item, unit.tile, unit.part, unit.first);
+                to[1].x = unit.count;
+                mkb::mbar_arrive(described(u));
+            }
+            __syncwarp();
+        };
         for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
-            if (unit.count == 0) continue;
+            if (unit.count == 0) {
+                if (!kKeys && unit.first >= 0) {  // rows without a key here
+                    const int64_t row_tile = (int64_t)unit.item * a.row_tiles + unit.tile;
+                    for (int i = lane; i < kTile; i += 32)
+                        if (a.splits > 1) a.stats[(row_tile * a.splits + unit.part) * kTile + i] = make_float2(-INFINITY, 0.f);
+                        else a.offs[row_tile * kTile + i] = INFINITY;
+                }
+                continue;
+            }
             const Item it(a, unit.item);
-            ok = wait(held_empty(u), (u >> 1) ^ 1, 0);
+            ok = wait_whole(held_empty(u), (u >> 1) ^ 1, 0);
             if (!ok) break;
-            mkb::mbar_expect_tx(held_full(u), kKeys ? S::kOperand : box_bytes);
-            if (kKeys) load_keys(held(u), &maps.k, it, kDim, unit.tile * kTile, held_full(u));
-            else load_queries(held(u), &maps.q, it, kDim, a.per, unit.tile * of_tile, held_full(u));
+            describe();
+            if (chosen) {
+                mkb::mbar_expect_tx(held_full(u), kKeys ? S::kOperand : box_bytes);
+                if (kKeys) load_keys(held(u), &maps.k, it, kDim, unit.tile * kTile, held_full(u));
+                else load_queries(held(u), &maps.q, it, kDim, a.per, unit.tile * of_tile, held_full(u));
+            }
+            __syncwarp();
             ++u;
             for (int n = unit.first; n < unit.first + unit.count; ++n, ++t) {
-                ok = wait(empty(t), t / S::stages ^ 1, 0);
+                ok = wait_whole(empty(t), t / S::stages ^ 1, 0);
                 if (!ok) break;
-                mkb::mbar_expect_tx(full(t), kKeys ? box_bytes + S::kExtra : S::kOperand);
-                if (kKeys) {
-                    load_queries(stage(t), &maps.q, it, kDim, a.per, n * of_tile, full(t));
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(base + S::extra + t % S::stages * S::kExtra),
-                                 "l"(a.offs + ((int64_t)unit.item * a.row_tiles + n) * kTile), "r"(S::kExtra), "r"(full(t))
-                                 : "memory");
-                } else {
-                    load_keys(stage(t), &maps.k, it, kDim, n * kTile, full(t));
+                if (chosen) {
+                    mkb::mbar_expect_tx(full(t), kKeys ? box_bytes + S::kExtra : S::kOperand);
+                    if (kKeys) {
+                        load_queries(stage(t), &maps.q, it, kDim, a.per, n * of_tile, full(t));
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                         base + S::extra + t % S::stages * S::kExtra),
+                                     "l"(a.offs + ((int64_t)unit.item * a.row_tiles + n) * kTile), "r"(S::kExtra), "r"(full(t))
+                                     : "memory");
+                    } else {
+                        load_keys(stage(t), &maps.k, it, kDim, n * kTile, full(t));
+                    }
                 }
+                __syncwarp();
             }
         }
+        ok = ok && wait_whole(held_empty(u), (u >> 1) ^ 1, 0);
+        unit.count = 0;  // (no more)
+        if (ok) describe();
         // no copy may be in flight when the block's shared memory goes away
         for (int i = max(u - 2, 0); i < u; ++i) tc_wait(held_full(i), (uint32_t)(i >> 1) & 1u, nullptr, a.timeout_ns, a.status, 0);
         for (int i = max(t - S::stages, 0); i < t; ++i) tc_wait(full(i), (uint32_t)(i / S::stages) & 1u, nullptr, a.timeout_ns, a.status, 0);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
+        const bool chosen = tc_elect();
         const uint32_t desc = tc_idesc(kTile, kTile);
         bool ok = true;
         int t = 0, u = 0;
-        Unit<kKeys> unit;
-        for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
-            if (unit.count == 0) continue;
-            ok = wait(held_full(u), u >> 1, 1);
-            for (int n = 0; n < unit.count && ok; ++n, ++t) {
-                ok = wait(full(t), t / S::stages, 1) && wait(read(t), t / kBuffers ^ 1, 1);
+        for (;;) {
+            ok = wait_whole(described(u), u / kUnits, 1);
+            const int count = ok ? *reinterpret_cast<const volatile int*>(at + S::units + u % kUnits * 32 + 16) : 0;
+            if (count == 0) break;
+            ok = wait_whole(held_full(u), u >> 1, 1);
+            for (int n = 0; n < count && ok; ++n, ++t) {
+                ok = wait_whole(full(t), t / S::stages, 1) && wait_whole(read(t), t / kBuffers ^ 1, 1);
                 if (!ok) break;
                 tc_after_sync();
+                if (chosen) {
 #pragma unroll
-                for (int slab = 0; slab < kDim / 64; ++slab)
+                    for (int slab = 0; slab < kDim / 64; ++slab)
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        tc_mma(tmem + t % kBuffers * kTile, tc_desc(held(u) + slab * kSlab + kk * 32), tc_desc(stage(t) + slab * kSlab + kk * 32), desc,
-                               (uint32_t)((slab | kk) != 0));
-                tc_commit(empty(t));
-                if (n == unit.count - 1) tc_commit(held_empty(u));
-                tc_commit(scored(t));
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma(tmem + t % kBuffers * kTile, tc_desc(held(u) + slab * kSlab + kk * 32), tc_desc(stage(t) + slab * kSlab + kk * 32), desc,
+                                   (uint32_t)((slab | kk) != 0));
+                    tc_commit(empty(t));
+                    if (n == count - 1) tc_commit(held_empty(u));
+                    tc_commit(scored(t));
+                }
+                __syncwarp();
             }
+            if (!ok) break;
             ++u;
         }
     } else if (warp >= 2) {
@@ -274,8 +317,14 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             }
             return true;
         };
-        for (uint32_t turn = 0; ok && unit.find(a, turn); ++turn) {
-            if (unit.count == 0 && (kKeys || unit.first < 0)) continue;
+        for (;;) {
+            ok = wait_all(described(u), u / kUnits);
+            if (!ok) break;
+            {
+                const volatile int* const from = reinterpret_cast<const volatile int*>(at + S::units + u % kUnits * 32);
+                unit.item = from[0], unit.tile = from[1], unit.part = from[2], unit.first = from[3], unit.count = from[4];
+            }
+            if (unit.count == 0) break;
             const Item it(a, unit.item);
             const int before = it.n - a.queries;
             float2 mine = make_float2(-INFINITY, 0.f);  // rows: maximum and sum; keys: x is not used
