@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     auto wait = [&](uint32_t b, int turn, int role) { return tc_wait(b, (uint32_t)turn & 1u, ctl, a.timeout_ns, a.status, role); };
     auto wait_all = [&](uint32_t b, int turn) { return __all_sync(0xffffffffu, wait(b, turn, 2)); };
 
+    if (threadIdx.x < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(threadIdx.x ? &maps.k : &maps.q) : "memory");
     if (kTile % a.per != 0) {  // rows that the copies leave out are finite
         for (int i = threadIdx.x; i < S::extra / 16; i += kThreads) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -175,16 +176,20 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + S::ctl + 4), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_before_sync();
     __syncthreads();
-    tc_after_sync();
-    const uint32_t tmem = (uint32_t)ctl[1];
-    let_next();  // (not before: a block of the next launch that held tensor memory would wait for this one, and this one for the memory)
-    if (kKeys) after_previous();  // (the offsets; the rows' launch is an ordinary one)
+    // (the copies begin while the others get the tensor memory)
+    uint32_t tmem = 0;
+    if (warp > 0) {
+        if (warp == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + S::ctl + 4), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        tc_before_sync();
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 32) : "memory");
+        tc_after_sync();
+        tmem = (uint32_t)ctl[1];
+        let_next();  // (not before: a block of the next launch that held tensor memory would wait for this one, and this one for the memory)
+    }
 
     const int of_tile = kTile / a.per, box_bytes = kDim / 64 * of_tile * a.per * 128;
     // (Both roles run as whole warps with a chosen lane: on one lane of a diverged warp every operand of an instruction of this kind is
@@ -225,24 +230,36 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             }
             __syncwarp();
             ++u;
-            for (int n = unit.first; n < unit.first + unit.count; ++n, ++t) {
-                ok = wait_whole(empty(t), t / S::stages ^ 1, 0);
+            auto rows = [&](int step, int n) {
+                mkb::mbar_expect_tx(full(step), box_bytes + S::kExtra);
+                load_queries(stage(step), &maps.q, it, kDim, a.per, n * of_tile, full(step));
+            };
+            int begun = 0;
+            if (kKeys && u == 1) {  // keys and queries are there; the offsets are the launch before's
+                begun = min(unit.count, S::stages);
+                if (chosen)
+                    for (int i = 0; i < begun; ++i) rows(i, unit.first + i);
+                __syncwarp();
+                after_previous();
+            }
+            for (int i = 0; i < unit.count; ++i, ++t) {
+                const int n = unit.first + i;
+                if (i >= begun) ok = wait_whole(empty(t), t / S::stages ^ 1, 0);
                 if (!ok) break;
-                if (chosen) {
-                    mkb::mbar_expect_tx(full(t), kKeys ? box_bytes + S::kExtra : S::kOperand);
-                    if (kKeys) {
-                        load_queries(stage(t), &maps.q, it, kDim, a.per, n * of_tile, full(t));
-                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                         base + S::extra + t % S::stages * S::kExtra),
-                                     "l"(a.offs + ((int64_t)unit.item * a.row_tiles + n) * kTile), "r"(S::kExtra), "r"(full(t))
-                                     : "memory");
-                    } else {
-                        load_keys(stage(t), &maps.k, it, kDim, n * kTile, full(t));
-                    }
+                if (chosen && kKeys) {
+                    if (i >= begun) rows(t, n);
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                     base + S::extra + t % S::stages * S::kExtra),
+                                 "l"(a.offs + ((int64_t)unit.item * a.row_tiles + n) * kTile), "r"(S::kExtra), "r"(full(t))
+                                 : "memory");
+                } else if (chosen) {
+                    mkb::mbar_expect_tx(full(t), S::kOperand);
+                    load_keys(stage(t), &maps.k, it, kDim, n * kTile, full(t));
                 }
                 __syncwarp();
             }
         }
+        if (kKeys && u == 0) after_previous();  // (a launch does not end before the one before it)
         ok = ok && wait_whole(held_empty(u), (u >> 1) ^ 1, 0);
         unit.count = 0;  // (no more)
         if (ok) describe();
