@@ -8,11 +8,13 @@
 //   keys   a unit is 128 keys (M) and a run of rows, 128 at a time: a thread has a key and a quarter of the rows, so that a key's weight is a
 //          sum in registers; where there are few keys their rows are several units, and a small launch adds the parts.
 // The exponentials bound both (16 a clock and SM: 0.54 us for 128 x 128 scores at 1.9 GHz, products 0.07 - 0.13).  Sums of a row refer to a
-// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 43 us for 1501 queries on 1501
-// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 60 us for 64 queries on 32768 keys (32 heads
-// of 128, exponentials 30 us): what a unit begins and ends with weighs there, since a key's rows are two steps.  The four warps that share
-// a row or key also share a scheduler; had they to meet at a unit's end, it was 44 and 65.  Twice the columns a thread (half the warps) took
-// 57 and 78, a polynomial for every fourth exponential 45 and 70, the next step's scores fetched ahead 62 and 107 (registers).
+// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 39.5 us for 1501 queries on 1501
+// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 57 us for 64 queries on 32768 keys (32 heads
+// of 128, exponentials 30 us).  A step of 128 x 128 takes 1,400 cycles: the warps that sum 1,050 of exponentials and 250 of waits and loads, the warp
+// that issues products 580 (64 for each of eight: both operands come from shared memory) and 400 of waits, so that either is near the other's time.
+// Steps: warps of a scheduler need not meet at a unit's end (-5 us), one warp finds the units (-2), chosen lanes of whole warps issue (-0.5).
+// No gain: twice the columns a thread (57 and 78 us then), a polynomial for every fourth exponential, halves of a step's columns loaded while the
+// others are summed (59.5), waits that poll (64).
 // Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the scores go
 // through memory (4 bytes a row where a key has 128 or 256).  One query on 65001 keys (32 heads of 64, 8 of keys): 21 us, 3.4 TB/s.  Blocks
 // that all fit the SMs at once: 26.6 -> 22.9 us against four per SM, of which three fit; the sum's loads issued together and before the
@@ -281,11 +283,12 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                 if (!ok) break;
                 tc_after_sync();
                 if (chosen) {
+                    const uint64_t of_held = tc_desc(held(u)), of_stage = tc_desc(stage(t));
 #pragma unroll
                     for (int slab = 0; slab < kDim / 64; ++slab)
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc_mma(tmem + t % kBuffers * kTile, tc_desc(held(u) + slab * kSlab + kk * 32), tc_desc(stage(t) + slab * kSlab + kk * 32), desc,
+                        for (int kk = 0; kk < 4; ++kk)  // (32 bytes on: the address is in units of 16, and does not carry beyond its field)
+                            tc_mma(tmem + t % kBuffers * kTile, of_held + (slab * kSlab + kk * 32) / 16, of_stage + (slab * kSlab + kk * 32) / 16, desc,
                                    (uint32_t)((slab | kk) != 0));
                     tc_commit(empty(t));
                     if (n == count - 1) tc_commit(held_empty(u));
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             float2 mine = make_float2(-INFINITY, 0.f);  // rows: maximum and sum; keys: x is not used
             if constexpr (kKeys) {
                 const int j = unit.tile * kTile + lanes;
-                const int own_row = max(j - before, 0) * a.per, last_row = max(unit.tile * kTile + quarter * 32 + 31 - before, 0) * a.per;  // the first that sees it
+                const int first_row = max(unit.tile * kTile + quarter * 32 - before, 0) * a.per, own_row = max(j - before, 0) * a.per, last_row = max(unit.tile * kTile + quarter * 32 + 31 - before, 0) * a.per;  // the first that sees it
                 float s4[4] = {0.f, 0.f, 0.f, 0.f};
                 for (int n = 0; n < unit.count; ++n, ++t) {
                     const int r0 = (unit.first + n) * of_tile * a.per + share * kCols;
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                             s4[2] += fast_exp2(fmaf(__uint_as_float(x[4 * c + 2]), a.scale, -o.z));
                             s4[3] += fast_exp2(fmaf(__uint_as_float(x[4 * c + 3]), a.scale, -o.w));
                         }
-                    } else {
+                    } else if (first_row < r0 + kCols) {
                         const int hidden = own_row - r0;  // columns before that do not see the key
 #pragma unroll
                         for (int c = 0; c < kCols / 4; ++c) {
@@ -385,15 +388,15 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
                 mine.y = (s4[0] + s4[1]) + (s4[2] + s4[3]);
             } else {
                 const int r0 = unit.tile * of_tile * a.per, have = min(of_tile * a.per, a.rows - r0), warp_row = quarter * 32;
-                const int last = before + (r0 + lanes) / a.per, warp_last = before + (r0 + warp_row) / a.per;
+                const int last = before + (r0 + lanes) / a.per, warp_last = before + (r0 + warp_row) / a.per, warp_end = before + (r0 + warp_row + 31) / a.per;
                 for (int n = 0; n < unit.count; ++n, ++t) {
                     ok = wait_all(scored(t), t / kBuffers);
                     if (!ok) break;
                     tc_after_sync();
                     uint32_t x[kCols];
                     scores(x);
-                    if (warp_row >= have) continue;
                     const int j0 = (unit.first + n) * kTile + share * kCols;
+                    if (warp_row >= have || j0 > warp_end) continue;  // no row sees any of these keys
                     const bool whole = j0 + kCols - 1 <= warp_last;  // every row sees all of these keys
                     if (whole && __all_sync(0xffffffffu, mine.x > -INFINITY)) {
                         float s4[4] = {0.f, 0.f, 0.f, 0.f};
