@@ -113,6 +113,13 @@ __device__ __noinline__ uint4 edge_vector(const T* base, int at, int shift, int 
     return make_uint4(words[0], words[1], words[2], words[3]);
 }
 
+// 16 bytes of minus infinity
+template <typename T>
+__device__ __forceinline__ uint4 none_of() {
+    constexpr uint32_t word = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    return make_uint4(word, word, word, word);
+}
+
 // The lane's elements of a block: a lane holds 8 bf16 or twice 4 floats next to each other.
 template <typename T>
 struct Elems {
@@ -289,7 +296,7 @@ template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArgs a) {
     extern __shared__ __align__(16) uint64_t raw[];
     const MergeSmem sm(raw, a);
-    __shared__ int listed;
+    __shared__ int listed, listed_soon;
     __shared__ uint32_t bound;
     const int t = threadIdx.x, group_of = blockIdx.x, row0 = group_of * a.beams, warp = t >> 5, lane = t & 31;
     const int segments = a.segments, groups = a.groups, k = a.k, shift_segment = __ffs(a.segment) - 1;
@@ -300,6 +307,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     const uint64_t lowest = order64(-(double)INFINITY);
     auto row_of = [&](int b) { return static_cast<const T*>(a.logits) + (row0 + b) * a.row_stride; };
     auto beam_of = [&](int i) { return (int)((i + 0.5f) * per_segments); };
+    if (t == 0) listed_soon = 0;
     for (int b = t; b < a.beams; b += threads) {
         const float c = a.scores != nullptr ? a.scores[row0 + b] : 0.f;
         const bool over = a.done != nullptr && a.done[row0 + b];
@@ -309,6 +317,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     __syncthreads();
     mkbh::after_previous();
     int chosen = 0, infinite = 0;  // (infinite: some logit is; the bounds below hold for finite ones)
+    float known = -INFINITY;       // a lower bound of the k-th best from the segments
 #pragma unroll 1
     for (int stage = 0; stage < 2; ++stage) {
         int count = stage == 0 ? a.beams * segments : chosen << shift_segment;
@@ -325,6 +334,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             const float x = mkbh::to_f<T>(static_cast<const T*>(sm.chosen_row[i >> shift_segment])[min(max(v, 0), a.vocab - 1)]);
             return b >= 0 && sm.kind[b] == kLive ? order_of(fmaxf(x, -INFINITY)) : 0u;
         };
+        auto stage_all = [&] {
+#pragma unroll 8
+            for (int i = t; i < count; i += threads) sm.staged[i] = fetch(i);
+        };
         auto choose = [&](int n, int b, int s) {  // segment s of beam b, as the n-th; b below 0: none
             const T* const row = row_of(max(b, 0));
             sm.chosen_beam[n] = b;
@@ -332,10 +345,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             sm.chosen_row[n] = row;
         };
         const bool staged = count <= a.staged;
-        if (staged) {
-#pragma unroll 8
-            for (int i = t; i < count; i += threads) sm.staged[i] = fetch(i);
-        }
+        if (staged && known == -INFINITY) stage_all();
         if (stage == 0) {
 #pragma unroll 1
             for (int b = warp; b < a.beams; b += threads / 32) {  // the beams' sums
@@ -415,6 +425,75 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             off = (fabsf(x) + fabsf(y)) * 0x1p-21f;  // (infinite with the score; then the bounds are not numbers, and pass no comparison)
             return x + y;
         };
+        // Listed elements are ranked in 64 bits
+        auto rank_listed = [&](int some) {
+            Candidate own{0, 0};
+            if (t < some) own = candidate(sm.listed[t]);
+            sm.key_a[t] = own.key;
+            sm.at_a[t] = own.at;
+            __syncthreads();
+#pragma unroll 1
+            for (int c = warp; c < some; c += threads / 32) {  // (a warp ranks a candidate)
+                const Candidate it{sm.key_a[c], sm.at_a[c]};
+                int rank = 0;
+                for (int j = lane; j - lane < some; j += 32) rank += __popc(__ballot_sync(0xffffffffu, j < some && Candidate{sm.key_a[j], sm.at_a[j]}.before(it)));
+                if (lane == 0 && rank < k) take(rank, it);
+            }
+        };
+        // the one continuation of beams that have ended
+        auto list_ended = [&](auto list) {
+            if (a.done == nullptr || t >= (stage == 0 ? a.beams : chosen)) return;
+            const int b = stage == 0 ? t : sm.chosen_beam[t];
+            if (b < 0 || sm.kind[b] != kDone) return;
+            const int at = stage == 0 ? 0 : a.eos - sm.chosen_first[t];
+            if (stage == 0) list(0, b, (a.eos + shift_of(row_of(b))) >> shift_segment);
+            else if (at >= 0 && at < a.segment) list((t << shift_segment) + at, 0, 0);
+        };
+        if (known > -INFINITY) {  // elements that the segments' bound lets pass: mostly few
+            auto list = [&](int i, int, int) {
+                const int n = atomicAdd(&listed_soon, 1);
+                if (n < kListed) sm.listed[n] = i;
+            };
+            // 16 bytes at a time, as a segment begins at a multiple of them
+            constexpr int kVector = 16 / sizeof(T), kShift = sizeof(T) == 2 ? 3 : 2, kTogether = 2;
+            const int vectors = count >> kShift, of_segment = a.segment >> kShift;
+#pragma unroll 1
+            for (int q0 = t; q0 < vectors; q0 += kTogether * threads) {
+                uint4 w[kTogether];
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u) {
+                    const int q = q0 + u * threads, c = q >> (shift_segment - kShift), b = q < vectors ? sm.chosen_beam[c] : -1;
+                    w[u] = none_of<T>();
+                    if (b < 0 || sm.kind[b] != kLive) continue;
+                    const int v = sm.chosen_first[c] + (q & (of_segment - 1)) * kVector;
+                    const T* const row = static_cast<const T*>(sm.chosen_row[c]);
+                    if (v >= 0 && v + kVector <= a.vocab) w[u] = mkb::ld_nc_v4(row + v);
+                    else w[u] = edge_vector(row - shift_of(row), v + shift_of(row), shift_of(row), shift_of(row) + a.vocab);
+                }
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u) {
+                    const int q = q0 + u * threads;
+                    if (q >= vectors) break;
+                    const float y = sm.offset[max(sm.chosen_beam[q >> (shift_segment - kShift)], 0)];
+                    const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+                    for (int e = 0; e < kVector; ++e) {
+                        const float x = sizeof(T) == 4 ? __uint_as_float(words[e & 3]) : e & 1 ? mkb::bf16_hi(words[e / 2]) : mkb::bf16_lo(words[e / 2]);
+                        const float off = (fabsf(x) + fabsf(y)) * 0x1p-21f;  // (as in `score`; what is no number passes no comparison)
+                        if (x + y + off >= known) list(q * kVector + e, 0, 0);
+                    }
+                }
+            }
+            list_ended(list);
+            __syncthreads();
+            const int some = listed_soon;
+            if (some >= min(k, count) && some <= kListed) {
+                rank_listed(some);
+                break;
+            }
+            if (staged) stage_all();
+            __syncthreads();
+        }
         float best_score = -INFINITY;
 #pragma unroll 2
         for (int i = t; i < count; i += threads) {
@@ -467,34 +546,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
                 }
                 if (high >= least) list(i, stage == 0 ? beam_of(i) : 0, stage == 0 ? i - beam_of(i) * segments : 0);
             }
-            // beams that have ended: their one continuation
-            if (a.done != nullptr && t < (stage == 0 ? a.beams : chosen)) {
-                const int b = stage == 0 ? t : sm.chosen_beam[t];
-                if (b >= 0 && sm.kind[b] == kDone) {
-                    const int at = stage == 0 ? 0 : a.eos - sm.chosen_first[t];
-                    if (stage == 0) list(0, b, (a.eos + shift_of(row_of(b))) >> shift_segment);
-                    else if (at >= 0 && at < a.segment) list((t << shift_segment) + at, 0, 0);
-                }
-            }
+            list_ended(list);
         }
         __syncthreads();
         const int some = listed;
         const bool few_listed = some >= min(k, count) && some <= most && least > -INFINITY;
         if (stage == 0 && few_listed) {
             chosen = some;
+            known = least;
         } else if (few_listed) {
-            Candidate own{0, 0};
-            if (t < some) own = candidate(sm.listed[t]);
-            sm.key_a[t] = own.key;
-            sm.at_a[t] = own.at;
-            __syncthreads();
-#pragma unroll 1
-            for (int c = warp; c < some; c += threads / 32) {  // (a warp ranks a candidate)
-                const Candidate it{sm.key_a[c], sm.at_a[c]};
-                int rank = 0;
-                for (int j = lane; j - lane < some; j += 32) rank += __popc(__ballot_sync(0xffffffffu, j < some && Candidate{sm.key_a[j], sm.at_a[j]}.before(it)));
-                if (lane == 0 && rank < k) take(rank, it);
-            }
+            rank_listed(some);
         } else {
             // Rounds: into groups by thread, the groups' best ranked, the members of the first k into a list
             int from_list = 0;  // 0: candidate(i), 1: list a, 2: list b
