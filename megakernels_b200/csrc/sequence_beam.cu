@@ -7,14 +7,15 @@
 //          run of segments;
 //   merge  a block per group: the log sums, the k best segments of all beams, and of their elements (still in L2)
 //          the k best.
-// Both selections go through the candidates' scores in fp32 first: a lower bound of the k-th best is the k-th best of the maxima
-// over groups of threads, and what may lie above it is listed, mostly little more than k.  The listed ones' 64-bit scores are
-// ranked by counting.  Where the list is too short for what may lie above (equal logits, fewer than k finite scores), the selection is
-// a knock-out: candidates fall into groups by thread, the groups' best ones are ranked by counting, the members of the k best
+// Both selections go through the candidates' scores in fp32 first: a lower bound of the k-th best is the k-th best of the segments' maxima
+// over groups of threads, and what may lie above it is listed, of segments and of their elements mostly little more than k.  The listed elements'
+// 64-bit scores are ranked by counting.  Where the list is too short for the elements that may lie above, they get a bound of their own; where it still is
+// (equal logits, fewer than k finite scores), the selection is a knock-out: candidates fall into groups by thread, the groups' best ones are ranked by counting, the members of the k best
 // groups go into the next round.  A candidate is a 64-bit key and its index, which are never equal (what is no candidate has the
 // key 0 and comes last), so both are exact, ties included.
-// Measured, replayed as a graph: 4 rows of 128256 bf16 10.8 us (1 MB, 0.2 at memory's rate: two dependent launches and the merge's chain
-// of some twenty meetings of a block bound it), 8 groups of 8 with k = 16 24.4 us (16 MB, 2.5; the scan 8 - 9 of them, 2 TB/s).
+// Measured, replayed as a graph: 4 rows of 128256 bf16 9.8 us (1 MB, 0.2 at memory's rate: two dependent launches and the merge's chain
+// of a dozen meetings of a block bound it), 8 groups of 8 with k = 16 20.6 us (16 MB, 2.5; the scan 8 - 9 of them, 2 TB/s).  With a second bound, for the
+// elements, and one element a load 10.8 and 24.4.
 #include "hybrid_common.cuh"
 #include "sequence_kernels.h"
 
@@ -42,7 +43,7 @@ struct BeamPlan {
         }
         segments = (int)((span + segment - 1) / segment);
         // as few segments per warp as let all blocks run at once, three on an SM (groups of 8 rows of 128256, 8, 12 and
-        // 24 of them, k = 8: with 1 block 21.1, 29.4, 37.3 us, 2 20.0, 22.6, 37.5, 3 20.0, 22.7, 31.0, 4 21.1, 24.4, 30.7)
+        // 24 of them, k = 8, before elements went 16 bytes at a time: with 1 block 21.1, 29.4, 37.3 us, 2 20.0, 22.6, 37.5, 3 20.0, 22.7, 31.0, 4 21.1, 24.4, 30.7)
         for (per_warp = 1; parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps), parts > 1 && (int64_t)rows * parts > 3 * kSms; ++per_warp) {
         }
         // candidates: all segments, then the elements of k of them, or of those that may be among the k

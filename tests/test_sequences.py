@@ -328,6 +328,21 @@ def test_beam_select_of_masked_logits(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("k", [1, 5, 16, 64])
+def test_beam_select_of_logits_in_few_places(dtype, k):
+    """A run of large logits holds more of the best than other runs have: many elements beat every other run's largest one."""
+    x = draw(5, 4, 20_011, dtype=dtype)
+    for row, (first, last) in enumerate([(700, 2300), (0, 300), (19_500, 20_011), (5000, 5003)]):
+        x[row, first:last] += 30
+    for beams in (1, 2, 4):
+        scores = draw(6, 4 // beams, beams)
+        done = torch.tensor([0, 0, 0, 1], dtype=torch.uint8).cuda().view(4 // beams, beams)
+        check_beams(x, scores, beams=beams, k=k)
+        check_beams(x, scores, beams=beams, k=k, done=done, eos=701)
+
+
+@pytest.mark.gpu
 def test_beam_select_far_apart_and_large_logits():
     x = torch.full((2, 5000), -1e4).cuda()
     x[0, 4321], x[1, 7] = 3e38, -3e38
