@@ -92,6 +92,7 @@ typedef struct MkbsReorder {
     const MkbsRegion *regions; /* host */
     const int32_t *parents;    /* [slots] */
     const int32_t *lengths;    /* [slots]: rows that a slot holds (above a region's rows: all); NULL: all */
+    int32_t *status;           /* 16 words that a wait for the call's own copies which gives up (2 s) writes to (code, block), or NULL */
 } MkbsReorder;
 int mkb_reorder_slots(const MkbsReorder *r, void *cuda_stream);
 

@@ -66,7 +66,8 @@ int check(const MkbsReorder* r) {
     if (r->slots < 1 || r->num_regions < 1 || r->first < 0 || !r->regions) return invalid("reorder: slots and regions must be positive, first not negative");
     if (r->slots > MKBS_MAX_SLOTS || r->num_regions > MKBS_MAX_REGIONS)
         return fail(MKBS_ERR_UNSUPPORTED, "reorder: at most %d slots and %d regions", MKBS_MAX_SLOTS, MKBS_MAX_REGIONS);
-    if (!aligned(r->parents, 4) || (r->lengths && !aligned(r->lengths, 4))) return invalid("reorder: parents or lengths missing or unaligned");
+    if (!aligned(r->parents, 4) || (r->lengths && !aligned(r->lengths, 4)) || (r->status && !aligned(r->status, 4)))
+        return invalid("reorder: parents missing, or they, lengths or status unaligned");
     for (int i = 0; i < r->num_regions; ++i) {
         const MkbsRegion& g = r->regions[i];
         if (!g.base || g.outer < 1 || g.rows < 1 || g.row_bytes < 1) return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: region %d is empty", i);

@@ -20,6 +20,7 @@ constexpr int kStages = 4, kStageBytes = 52 * 1024, kShortRun = 2048;
 struct ReorderArgs {
     int slots, num_regions, first;
     const int32_t *parents, *lengths;
+    int32_t* status;
     MkbsRegion regions[MKBS_MAX_REGIONS];
 };
 
@@ -161,6 +162,15 @@ __global__ void __launch_bounds__(kReorderThreads, 1) reorder_bulk_kernel(const 
     __syncwarp();
     Step load(a, k), store = load;
     int issued = 0;
+    auto arrived = [&](int step, unsigned long long limit_ns) {
+        unsigned long long began = 0;
+        while (!mkb::mbar_try_wait(bar0 + step % kStages * 8, (uint32_t)(step / kStages) & 1u)) {
+            const unsigned long long now = mkb::globaltimer_ns();
+            if (began == 0) began = now;
+            if (now - began > limit_ns) return false;
+        }
+        return true;
+    };
     auto issue = [&]() {
         const int st = issued % kStages, from = k.source_begin[load.c], to = k.source_begin[load.c + 1], run = k.run[load.c];
         int bytes = 0;
@@ -181,17 +191,11 @@ __global__ void __launch_bounds__(kReorderThreads, 1) reorder_bulk_kernel(const 
     while (issued < kStages && load.settle(a, k)) issue();
     for (int done = 0; store.settle(a, k); ++done, store.at += gridDim.x) {
         const int st = done % kStages, source0 = k.source_begin[store.c], run = k.run[store.c];
-        unsigned long long began = 0;
-        bool there = true;
-        while (!mkb::mbar_try_wait(bar0 + st * 8, (uint32_t)(done / kStages) & 1u)) {  // (every lane reads what has arrived)
-            const unsigned long long now = mkb::globaltimer_ns();
-            if (began == 0) began = now;
-            if (now - began > 2000000000ull) {
-                there = false;
-                break;
-            }
+        if (!__all_sync(0xffffffffu, arrived(done, 2000000000ull))) {  // (every lane reads what has arrived)
+            if (lane == 0 && a.status != nullptr && atomicCAS(a.status, 0, (int)MKBS_ERR_DEVICE_TIMEOUT) == 0) a.status[1] = blockIdx.x;
+            for (int i = done; i < issued; ++i) arrived(i, 200000000ull);  // (before shared memory goes away)
+            break;
         }
-        if (!__all_sync(0xffffffffu, there)) break;
         for (int i = k.target_begin[store.c] + lane; i < k.target_begin[store.c + 1]; i += 32) {
             const int s = k.target[i], p = k.parent[s], n = store.held(a, k, p);
             if (n > 0)
@@ -675,7 +679,7 @@ cudaError_t select(const MkbsSelect& a, int fit, cudaStream_t s) {
 }  // namespace
 
 cudaError_t reorder_launch(const MkbsReorder& r, cudaStream_t s) {
-    ReorderArgs a{r.slots, r.num_regions, r.first, r.parents, r.lengths, {}};
+    ReorderArgs a{r.slots, r.num_regions, r.first, r.parents, r.lengths, r.status, {}};
     uintptr_t bits = 0;  // what every address and size is a multiple of
     for (int i = 0; i < r.num_regions; ++i) {
         const MkbsRegion& g = a.regions[i] = r.regions[i];

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         const bool chosen = tc_elect();
         bool ok = true;
         int t = 0, u = 0;
-        Unit<kKeys> unit;
+        Unit<kKeys> unit = {};
         auto describe = [&] {  // unit u, for the other warps; (what the place held before has been read, as held_empty says)
             if (chosen) {
                 int4* const to = reinterpret_cast<int4*>(at + S::units + u % kUnits * 32);

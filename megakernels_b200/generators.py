@@ -409,6 +409,7 @@ class MK_Generator(Generator):
         globs, ops = self.schedule.globs, get_mk_module(name="mk_sequences")
         self._positions_before = globs.pos_id_device
         device = globs.hidden_states.device
+        self._moves = torch.zeros(16, dtype=torch.int32, device=device) if self._moves is None else self._moves
         single = make_globals(self.model, skip_attn_reduction=True, max_attn_partitions=1)
         single.instructions = torch.zeros(1, 1, 32, dtype=torch.int32, device=device)  # (a prompt runs none)
         logits = globs.logits.new_empty(len(prompts), globs.vocab_size)
@@ -419,7 +420,8 @@ class MK_Generator(Generator):
             self._prompt(ids.reshape(1, -1).to(device), globs=single)
             logits[p] = single.logits
             parents = torch.where(slots // beams == p, 0, slots)
-            ops.reorder_slots([globs.k_cache, globs.v_cache], parents.int(), dim=1, lengths=torch.full_like(slots, ids.numel()))
+            ops.reorder_slots([globs.k_cache, globs.v_cache], parents.int(), dim=1, lengths=torch.full_like(slots, ids.numel()),
+                              status=self._moves)
         return logits
 
     def step_beams(self, tokens: Tensor, positions: Tensor) -> Tensor:
@@ -445,9 +447,11 @@ class MK_Generator(Generator):
             everyone = torch.arange(slots, dtype=torch.int32, device=parents.device)
             everyone[:n] = parents
             parents, lengths = everyone, torch.cat([lengths, lengths.new_zeros(slots - n)])
-        get_mk_module(name="mk_sequences").reorder_slots([globs.k_cache, globs.v_cache], parents, dim=1, first=first, lengths=lengths)
+        get_mk_module(name="mk_sequences").reorder_slots(
+            [globs.k_cache, globs.v_cache], parents, dim=1, first=first, lengths=lengths, status=self._moves)
 
     _positions_before = None
+    _moves: Tensor | None = None  # status of the beams' reordering
 
     def end_beams(self) -> None:
         self.schedule.globs.pos_id_device = self._positions_before
@@ -470,6 +474,8 @@ class MK_Generator(Generator):
         """Synchronise and raise if any device-side wait gave up."""
         if self.last_call is None:
             return None
+        if self._moves is not None:
+            get_mk_module(name="mk_sequences").raise_status(self._moves)
         return self.interpreter.module.sync_status(self.last_call)
 
 
@@ -596,6 +602,7 @@ class Hybrid_Generator(MK_Generator):
         """Each prompt once, its state handed to its beams' slots, which are taken from the pool until ``end_beams``."""
         model, logits = self.model, []
         self._slot_before, self._beam_slots = self.slot, []
+        self._moves = torch.zeros(16, dtype=torch.int32, device=model.device) if self._moves is None else self._moves
         for _ in range(len(prompts) * beams):
             self._beam_slots.append(model.slots.allocate())
         self._slot_of = torch.tensor(self._beam_slots, dtype=torch.int32, device=model.device)
@@ -627,7 +634,7 @@ class Hybrid_Generator(MK_Generator):
         rows = torch.zeros_like(everyone)
         everyone[mine] = self._slot_of[parents.long()]
         rows[mine] = lengths
-        self.model.state.reorder(everyone, rows)
+        self.model.state.reorder(everyone, rows, self._moves)
 
     def end_beams(self) -> None:
         for slot in self._beam_slots:

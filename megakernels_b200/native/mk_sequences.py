@@ -45,7 +45,7 @@ class MkbsRegion(ctypes.Structure):
 class MkbsReorder(ctypes.Structure):
     _fields_ = [
         ("struct_bytes", _u32), ("slots", _i32), ("num_regions", _i32), ("first", _i32), ("regions", ctypes.POINTER(MkbsRegion)),
-        ("parents", _ptr), ("lengths", _ptr),
+        ("parents", _ptr), ("lengths", _ptr), ("status", _ptr),
     ]
 
 
@@ -179,6 +179,21 @@ def _struct(kind):
     return s
 
 
+def _check_status(status, device: int) -> int:
+    at = _check("status", status, torch.int32, device)
+    if status.numel() < 16:
+        raise ValueError("status must hold 16 words")
+    return at
+
+
+def raise_status(status: Tensor) -> None:
+    """Synchronise, and raise if a wait of the calls that were given ``status`` has given up; it is cleared then."""
+    code, block = status[:2].tolist()
+    if code:
+        status.zero_()
+        raise SequenceError(code, f"a wait on the device gave up (block {block})")
+
+
 def _set_lengths(s, lengths, device: int, sequences: int, positions: int):
     """Rows that each sequence holds: an int32 tensor on the device, or one number for all."""
     if isinstance(lengths, Tensor):
@@ -228,12 +243,14 @@ def beam_select(logits: Tensor, scores: Tensor | None = None, *, beams: int, k: 
     return tuple(out)
 
 
-def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first: int = 0, lengths: Tensor | None = None, stream=None) -> None:
+def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first: int = 0, lengths: Tensor | None = None, status: Tensor | None = None,
+                  stream=None) -> None:
     """``t[..., slot, ...] <- t[..., parents[slot], ...]`` for every slot at once and in place, ``dim`` being the slots'
     dimension (0, or 1 behind the layers') of every tensor.
 
     With ``lengths`` (int32 ``[slots]``) the dimension behind it is rows: a slot takes its parent's rows ``first ..
     lengths[parent] - 1``; the others stay.  ``parents`` int32 ``[slots]``; one outside the slots leaves its slot as it is.
+    ``status``: int32 ``[16]``, zero, for a wait that gives up (:func:`raise_status`).
     """
     tensors = list(tensors)
     if not tensors:
@@ -251,6 +268,8 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
     base.slots, base.first = slots, first
     base.parents = _check("parents", parents, torch.int32, device)
     by_rows = lengths is not None
+    if status is not None:
+        base.status = _check_status(status, device)
     if by_rows:
         base.lengths = _check("lengths", lengths, torch.int32, device, (slots,))
     regions = (MkbsRegion * len(tensors))()
@@ -279,13 +298,13 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
     for at in range(0, len(tensors), MAX_REGIONS):
         base.num_regions = min(MAX_REGIONS, len(tensors) - at)
         base.regions = ctypes.cast(ctypes.byref(regions, at * ctypes.sizeof(MkbsRegion)), ctypes.POINTER(MkbsRegion))
-        where.launch("mkb_reorder_slots", base, parents, lengths, *tensors)
+        where.launch("mkb_reorder_slots", base, parents, lengths, status, *tensors)
 
 
 def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int, *, scale: float, status: Tensor | None = None, wait_timeout_ms: int = 0,
                 stream=None) -> None:
     """Add to ``weights`` (float32 ``[layers, sequences, kv_heads, positions]``) the softmax weight that each cached key
-    receives from the queries, summed over them and over the query heads that share the key.
+    receives from the queries, summed over them and over the query heads that share the key.  ``status``: as in :func:`reorder_slots`.
 
     ``q`` bf16 ``[layers, sequences, queries, heads, dim]``: the queries of the sequences' last rows; ``keys`` bf16 ``[layers,
     sequences, positions, kv_heads, dim]``, dim 64 or 128; ``lengths``: rows that each sequence holds, an int32 tensor
@@ -308,9 +327,7 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
     lengths = _set_lengths(s, lengths, device, sequences, positions)
     s.scale, s.wait_timeout_ms = scale, wait_timeout_ms
     if status is not None:
-        s.status = _check("status", status, torch.int32, device)
-        if status.numel() < 16:
-            raise ValueError("status must hold 16 words")
+        s.status = _check_status(status, device)
     size = lib.mkb_key_weights_bytes(s)
     if not size:
         where.launch("mkb_key_weights", s)  # (says what is wrong)

@@ -113,7 +113,7 @@ class HybridState:
             if getattr(m, "conv_taps", 0):
                 self.projected[i], self.projected_terms[i] = f32(max(m.conv_taps - 1, 1), m.in_rows), f32(m.in_rows)
 
-    def reorder(self, parents: Tensor, lengths: Tensor) -> None:
+    def reorder(self, parents: Tensor, lengths: Tensor, status: Tensor | None = None) -> None:
         """Every slot takes its parent's state, all at once and in place: ``parents`` int32 ``[slots]`` on the device (a slot's
         own number: it stays), ``lengths`` int32 ``[slots]``: positions that a slot's sequence has, all rows of longer rings."""
         from megakernels_b200.mk import get_mk_module
@@ -124,11 +124,11 @@ class HybridState:
         by_head = [t.transpose(0, 1) for t in caches(self.by_head)]
         by_row = caches(i for i in self.keys if i not in self.by_head)
         if whole:
-            ops.reorder_slots(whole, parents)
+            ops.reorder_slots(whole, parents, status=status)
         if by_row:
-            ops.reorder_slots(by_row, parents, lengths=lengths)
+            ops.reorder_slots(by_row, parents, lengths=lengths, status=status)
         if by_head:
-            ops.reorder_slots(by_head, parents, dim=1, lengths=lengths)
+            ops.reorder_slots(by_head, parents, dim=1, lengths=lengths, status=status)
 
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size()

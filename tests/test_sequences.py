@@ -114,7 +114,7 @@ REFUSED = [
     ]),
     ("reorder_slots", reorder_struct, [
         (dict(struct_bytes=8), 1, "struct size"), (dict(slots=0), 1, "positive"), (dict(num_regions=0), 1, "positive"), (dict(first=-1), 1, "negative"),
-        (dict(slots=257), 5, "at most"), (dict(num_regions=49), 5, "at most"), (dict(parents=None), 1, "parents"), (dict(lengths=FAKE + 1), 1, "lengths"),
+        (dict(slots=257), 5, "at most"), (dict(num_regions=49), 5, "at most"), (dict(parents=None), 1, "parents"), (dict(lengths=FAKE + 1), 1, "lengths"), (dict(status=FAKE + 2), 1, "status"),
         (dict(region=dict(base=None)), 1, "empty"), (dict(region=dict(rows=0)), 1, "empty"), (dict(region=dict(row_bytes=0)), 1, "empty"),
         (dict(region=dict(slot_stride=999)), 1, "overlap"), (dict(region=dict(outer_stride=999)), 1, "overlap"), (dict(region=dict(row_bytes=1 << 31)), 1, "overlap"),
     ]),
@@ -166,6 +166,17 @@ def test_the_same_region_twice_is_refused():
     regions[1].base = FAKE
     assert lib.mkb_reorder_slots(ctypes.byref(s), None) == 1
     assert "0 and 1 are the same" in lib.mkb_sequences_last_error().decode()
+
+
+def test_a_wait_that_gave_up_is_raised_and_cleared():
+    """(The record as a kernel leaves it; no call here waits in vain.)"""
+    status = torch.zeros(16, dtype=torch.int32)
+    ops.raise_status(status)
+    status[0], status[1] = 3, 77
+    with pytest.raises(ops.SequenceError, match="block 77") as e:
+        ops.raise_status(status)
+    assert e.value.code == 3 and not status.any()
+    ops.raise_status(status)
 
 
 @pytest.mark.parametrize("length", [-1, 101, 2**32 + 5, -(2**32) + 5])
