@@ -13,9 +13,10 @@
 // (equal logits, fewer than k finite scores), the selection is a knock-out: candidates fall into groups by thread, the groups' best ones are ranked by counting, the members of the k best
 // groups go into the next round.  A candidate is a 64-bit key and its index, which are never equal (what is no candidate has the
 // key 0 and comes last), so both are exact, ties included.
-// Measured, replayed as a graph: 4 rows of 128256 bf16 9.8 us (1 MB, 0.2 at memory's rate: two dependent launches and the merge's chain
-// of a dozen meetings of a block bound it), 8 groups of 8 with k = 16 20.6 us (16 MB, 2.5; the scan 8 - 9 of them, 2 TB/s).  With a second bound, for the
-// elements, and one element a load 10.8 and 24.4.
+// Measured, replayed as a graph: 4 rows of 128256 bf16 8.8 us (1 MB, 0.2 at memory's rate: two dependent launches and the merge's chain
+// of a dozen meetings of a block bound it), 8 groups of 8 with k = 16 17.5 us (16 MB, 2.5; the scan 8 - 9 of them, 2 TB/s).  With a second bound, for the
+// elements, and one element a load 10.8 and 24.4; with segments of 256 elements there too, 9.8 and 20.6; with neighbouring segments in one group of the bound
+// 16 instead of 8.8 where one of 11 beams of 5814 has most of the best (the list overflows).
 #include "hybrid_common.cuh"
 #include "sequence_kernels.h"
 
@@ -35,11 +36,16 @@ struct BeamPlan {
     int chosen;                                    // segments whose elements are candidates, at most
     size_t part_offset, bytes;
     explicit BeamPlan(const MkbsBeams& b) {
+        lay_out(b, true);
+        if (merge_smem() > kMostShared) lay_out(b, false);
+    }
+    // Ample: room for segments that tie, and segments so long that there are not many more of them than 16-byte loads of the chosen ones.  (Where
+    // the knock-out's lists have no room beside that, as many segments as elements.)
+    void lay_out(const MkbsBeams& b, bool ample) {
         rows = b.groups * b.beams;
         const int64_t span = b.vocab + 15;  // (a row may start anywhere in 16 bytes)
-        // about as many segments as the chosen ones have elements, of 256 at least
-        chosen = most_chosen(b.k);
-        for (segment = kBlockElems; (int64_t)b.beams * ((span + segment - 1) / segment) > 2 * (int64_t)chosen * segment; segment *= 2) {
+        chosen = ample ? b.k + b.k / 2 + 16 : b.k + b.k / 4 + 8;
+        for (segment = kBlockElems; (int64_t)b.beams * ((span + segment - 1) / segment) > (int64_t)chosen * segment * 2 / (ample ? 8 : 1); segment *= 2) {
         }
         segments = (int)((span + segment - 1) / segment);
         // as few segments per warp as let all blocks run at once, three on an SM (groups of 8 rows of 128256, 8, 12 and
@@ -62,7 +68,6 @@ struct BeamPlan {
         if (m <= groups) return 0;
         return k * (m <= kMergeThreads ? (m + groups - 1) / groups : (m + kMergeThreads - 1) / kMergeThreads * (kMergeThreads / groups));
     }
-    static constexpr int most_chosen(int k) { return k + k / 4 + 8; }
     size_t merge_smem() const {  // (bounds and lists take turns)
         const size_t lists = (size_t)(list_a + list_b) * kCandidateBytes, bounds = (size_t)staged * 4;
         return (lists > bounds ? lists : bounds) + (size_t)groups * (kCandidateBytes + 4) + (size_t)chosen * 16 + MKBS_MAX_BEAMS * 28 + kListed * 4;
@@ -503,10 +508,14 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             best_score = fmaxf(best_score, x - off);
             if (staged) sm.staged[i] = __float_as_uint(x + off);
         }
-        for (int o = lanes / 2; o; o >>= 1) best_score = fmaxf(best_score, __shfl_xor_sync(0xffffffffu, best_score, o));
-        if (t % lanes == 0) {
-            sm.group_at[group] = order_of(best_score);
-            sm.rank[group] = 0;
+        // (neighbours fall into different groups: often one beam, or one run of tokens, has most of the best)
+        sm.listed[t] = order_of(best_score);
+        __syncthreads();
+        if (t < groups) {
+            uint32_t most = sm.listed[t];
+            for (int j = t + groups; j < threads; j += groups) most = max(most, sm.listed[j]);
+            sm.group_at[t] = most;
+            sm.rank[t] = 0;
         }
         __syncthreads();
         // ranks of the groups' maxima: a thread compares one of them with a share of the others
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             if (before) atomicAdd(&sm.rank[mine], before);
         }
         __syncthreads();
-        if (t % lanes == 0 && sm.rank[group] == k - 1) bound = order_of(best_score);
+        if (t < groups && sm.rank[t] == k - 1) bound = sm.group_at[t];
         __syncthreads();
         const float least = value_of(bound);
         // What may be among the k best: of the segments all are chosen, in any order, of the elements the k best

@@ -354,6 +354,21 @@ def test_beam_select_of_logits_in_few_places(dtype, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("beams,vocab,k", [(11, 5814, 11), (8, 1000, 8), (4, 32003, 16), (64, 3001, 64), (8, 128256, 16)])
+def test_beam_select_where_one_beam_is_ahead(beams, vocab, k, dtype):
+    """All of the best, or most of them, are one beam's continuations."""
+    x = draw(vocab, 2 * beams, vocab, dtype=dtype, std=2)
+    for gap in (3, 12, 200):
+        scores = draw(k, 2, beams) - gap
+        scores[0, beams - 1] = scores[1, 0] = 0
+        done = torch.zeros(2, beams, dtype=torch.uint8)
+        done[0, 0] = done[1, 0] = 1  # (in the second group the one that is ahead has ended)
+        check_beams(x, scores, beams=beams, k=k)
+        check_beams(x, scores, beams=beams, k=k, done=done.cuda(), eos=vocab - 1)
+
+
+@pytest.mark.gpu
 def test_beam_select_far_apart_and_large_logits():
     x = torch.full((2, 5000), -1e4).cuda()
     x[0, 4321], x[1, 7] = 3e38, -3e38
