@@ -174,9 +174,11 @@ class MK_Generator(Generator):
         return self._graph_out
 
     def run(self, input_ids: Tensor, pos_id):
+        globs = self.schedule.globs
+        if globs.key_weights is not None:
+            self._forget(int(pos_id))
         if getattr(self, "_graph", None) is not None:
             return self._replay(input_ids, pos_id)
-        globs = self.schedule.globs
         if not self.skip_rest:
             post = self.model.model.embed_tokens(BatchState(input_ids=input_ids))
             assert post.hidden_states is not None
@@ -288,14 +290,18 @@ class MK_Generator(Generator):
         The reference prefills with its torch model (scripts/generate.py:125-137).  Here the tokens go
         through the layers at once, in portions, or where that does not apply (``_takes_prompts``) or memory
         for a portion is lacking, through the decode kernel one at a time.  ``position``: of the first token, behind
-        what the cache holds of the sequence (a later turn of a chat); 0 starts a sequence.
+        what the cache holds of the sequence (a later turn of a chat) or, to replace rows, before its end; 0 starts a sequence.
         """
         ids = prompt_ids.reshape(1, -1)
         at_once = self._takes_prompts(ids.shape[1], position)
-        if self.schedule.globs.key_weights is not None and not at_once:
+        observed = self.schedule.globs.key_weights is not None
+        if observed and not at_once:
             raise ValueError("only prompts that go through the layers at once are observed")
         if position == 0:
             self._start_sequence()
+        if observed:
+            self._forget(position)
+            self._weighed = position + ids.shape[1]
         return self._prompt(ids, position) if at_once else self._steps(ids, 0, position)
 
     def _steps(self, ids: Tensor, done: int, first: int = 0) -> Tensor:
@@ -307,11 +313,19 @@ class MK_Generator(Generator):
     # -- long caches cut to the keys that are looked at ----------------------- #
     observed: int | None = None
     evicted = 0
+    _weighed = 0  # rows from here on have no weight
+
+    def _forget(self, row: int) -> None:
+        """Rows from ``row`` on are not those any more that were given weight."""
+        if row < self._weighed:
+            self.schedule.globs.key_weights[..., row : self._weighed] = 0
+            self._weighed = row
 
     def observe(self, window: int | None = None) -> None:
         """From the next prompt on keep the softmax weight that its last ``window`` tokens (None: all of them) give each
         cached key, per layer and key/value head (``globs.key_weights``), for :meth:`evict`.  Of decoded tokens none is
-        kept.  Call it before ``enable_cuda_graph``.
+        kept.  A row that is written again, by a prompt or by decoding, loses what its earlier key was given; what discarded
+        tokens gave to rows before them stays.  Call it before ``enable_cuda_graph``.
         """
         globs = self.schedule.globs
         if globs.batch_size != 1 or globs.tp is not None or self._whole is None or not globs.hidden_states.is_cuda:
@@ -344,6 +358,7 @@ class MK_Generator(Generator):
         globs = self.schedule.globs
         if globs.key_weights is not None:
             globs.key_weights.zero_()
+            self._weighed = 0
             self._turn_to(0)
 
     def _turn_to(self, evicted: int) -> None:
@@ -363,7 +378,8 @@ class MK_Generator(Generator):
 
         Every layer and key/value head keeps its first ``sinks`` rows, its last ``recent``, and of the others those that the
         observed prompts (:meth:`observe`) gave the most weight.  Keys stay rotated by the position they had, and tokens to come
-        are rotated by theirs.
+        are rotated by theirs.  Rows behind ``length`` count as gone.  A row is another token in every head then, but for the first
+        ``sinks`` and the last ``recent``: a turn that replaces rows before those replaces each head's own last ones.
         """
         globs = self.schedule.globs
         if globs.key_weights is None:
@@ -372,6 +388,7 @@ class MK_Generator(Generator):
             raise ValueError(f"{length} rows of a cache of {globs.k_cache.shape[2]}")
         if not (keep >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= keep):
             raise ValueError(f"{sinks} first and {recent} last of {keep} rows")
+        self._forget(length)
         if length <= keep:
             return length
         ops = get_mk_module(name="mk_sequences")
@@ -380,6 +397,7 @@ class MK_Generator(Generator):
         rows = ops.select_rows(weights, length, keep=keep, sinks=sinks, recent=recent, kept=weights)
         ops.move_rows(k, v, rows, length)
         weights[..., keep:length] = 0
+        self._weighed = min(self._weighed, keep)
         self._turn_to(self.evicted + length - keep)
         return keep
 

@@ -412,6 +412,52 @@ def test_rotations_after_many_evictions():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("replaced,count", [(50, 40), (20, 40), (40, 40)])
+def test_weights_of_a_replaced_turn_are_the_new_keys(replaced, count):
+    """Rows of a turn that is written again, longer or shorter, have the weights that they have where the first one never was."""
+    weights, start, turn = [], prompt(60, 1), prompt(count, 2)
+    for turns in ([prompt(replaced, 3), turn], [turn]):
+        model, gen = observed_generator("1b", 128, None)
+        gen.prefill(start)
+        for ids in turns:
+            gen.prefill(ids, position=60)
+        gen.check()
+        weights.append(gen.schedule.globs.key_weights)
+    assert torch.equal(weights[0][..., 60:], weights[1][..., 60:]) and weights[0][..., 60 : 60 + count].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_decoding_over_observed_rows_takes_their_weights(graph):
+    model, gen = observed_generator("1b", 128, None)
+    if graph:
+        gen.enable_cuda_graph()
+    globs = gen.schedule.globs
+    token = gen.prefill(prompt(100, 1))
+    before = globs.key_weights.clone()
+    for i in range(3):  # behind the prompt: nothing changes
+        gen.run(token.view(1, 1), 100 + i)
+    assert torch.equal(globs.key_weights, before)
+    for i in range(3):
+        gen.run(token.view(1, 1), 80 + i)
+    gen.check()
+    assert torch.equal(globs.key_weights[..., :80], before[..., :80]) and not globs.key_weights[..., 80:].any()
+
+
+@pytest.mark.gpu
+def test_rows_behind_what_is_evicted_lose_their_weights():
+    model, gen = observed_generator("1b", 128, None)
+    weights = gen.schedule.globs.key_weights
+    gen.prefill(prompt(100, 1))
+    before = weights.clone()
+    assert gen.evict(90, 95, 2, 4) == 90
+    assert torch.equal(weights[..., :90], before[..., :90]) and not weights[..., 90:].any()
+    assert gen.evict(70, 40, 2, 4) == 40 and gen.evicted == 30
+    assert not weights[..., 40:].any()
+    assert torch.equal(weights[..., 36:40], before[..., 66:70])  # the last of the 70
+
+
+@pytest.mark.gpu
 def test_tokens_observed_one_at_a_time():
     """A prompt cut into single tokens is weighed as it is at once.  Queries and keys of other products differ by the last bit of bf16 here and
     there: single weights by a few hundredths, a query's sum only by the rounding of its own terms."""
