@@ -630,17 +630,14 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
 
 template <typename T>
 cudaError_t launch(const BeamPlan& p, const MkbsBeams& b, const BeamArgs& a, cudaStream_t s) {
-    const size_t smem = p.merge_smem();
-    if (smem > 48 * 1024) {
-        const cudaError_t e = allow_shared_memory<beam_merge_kernel<T>>();
-        if (e != cudaSuccess) return e;
-    }
+    // (in any case: what a kernel may have without asking counts its static words too)
+    if (const cudaError_t e = allow_shared_memory<beam_merge_kernel<T>>(); e != cudaSuccess) return e;
     beam_scan_kernel<T><<<dim3(p.parts, p.rows), 32 * kScanWarps, 0, s>>>(a);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(b.groups);
     c.blockDim = dim3(kMergeThreads);
-    c.dynamicSmemBytes = smem;
+    c.dynamicSmemBytes = p.merge_smem();
     c.stream = s;
     cudaLaunchAttribute early = mkbh::may_begin_early();
     c.attrs = &early;

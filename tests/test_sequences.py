@@ -6,6 +6,8 @@ Every operator against a plain implementation in 64 bits; whole numbers and move
 import ctypes
 import math
 import re
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -366,6 +368,20 @@ def test_beam_select_where_one_beam_is_ahead(beams, vocab, k, dtype):
         done[0, 0] = done[1, 0] = 1  # (in the second group the one that is ahead has ended)
         check_beams(x, scores, beams=beams, k=k)
         check_beams(x, scores, beams=beams, k=k, done=done.cuda(), eos=vocab - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_first_selection_of_a_process_may_need_any_amount_of_shared_memory(dtype):
+    """48 KB less a few bytes, 48 KB exactly and more; each shape in a process of its own, since one selection's permission serves the next."""
+    for beams, vocab, k in ((1, 8200, 128), (3, 2600, 128), (2, 6200, 96), (33, 100, 128), (1, 7000, 128), (1, 9000, 128)):
+        code = f"""
+import sys; sys.path.insert(0, {str(ROOT)!r})
+import torch
+from tests.test_sequences import check_beams, draw
+check_beams(draw(1, {2 * beams}, {vocab}, dtype={dtype}, std=2), beams={beams}, k={k})
+"""
+        subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
 
 
 @pytest.mark.gpu
