@@ -959,7 +959,7 @@ cudaError_t Prefill<T>::canon_norm(const MkbhGlobals& g, const MkbhLayer& L, T* 
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (smem > 48 * 1024 && set[dev & 63] < smem) {
+    if (smem > 47 * 1024 && set[dev & 63] < smem) {  // (the limit of 48 KB is on static words too)
         e = cudaFuncSetAttribute(canon_norm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         set[dev & 63] = smem;

@@ -435,3 +435,17 @@ def test_rotated_values_round_one_product(tmp_path, vdim, conv):
     fma = lambda a, b, z: (a.double() * b.double() + z.double()).float()  # noqa: E731
     assert torch.equal(held[:, 0::2], fma(x, c, -(y * s)))
     assert torch.equal(held[:, 1::2], fma(x, s, y * c) if vdim <= 64 else fma(y, c, x * s))
+
+
+@pytest.mark.parametrize("dtype,tol", DTYPES)
+def test_inputs_of_a_convolution_that_fill_the_shared_memory_that_is_there_unasked(bench, dtype, tol):
+    """Six taps of 2048 inputs are 48 KB; in a process of its own, since what one launch asks for serves the next."""
+    raw, w, path, toks, want = bench("taps", model_config([chunked(4, 2, 16, 16, size=9, ff=32)], width=2048, taps=6), n=20)
+    code = f"""
+import sys; sys.path.insert(0, {str(ROOT)!r})
+import torch
+from tests.dumalix_utils import load, run_cut
+torch.save(run_cut(load({str(path)!r}, {dtype}, max_len=64), {toks}, [20]).cpu(), {str(path)!r} + "/out.pt")
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+    assert rel(torch.load(path / "out.pt"), want) < tol
