@@ -589,7 +589,7 @@ int mkb_prompt(const MkbGlobals* g, const MkbPrompt* caller, void* cuda_stream) 
         return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: hidden or workspace missing, unaligned or too small");
     if (p->key_weights) {
         if (p->observed < 1 || p->observed > p->tokens) return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: %d of %d tokens observed", p->observed, p->tokens);
-        if (((uintptr_t)p->key_weights & 3) || p->weights_head < g->kv_max_len || p->weights_layer < g->kv_max_len)
+        if (((uintptr_t)p->key_weights & 3) || !mkbs::apart(g->kv_max_len, {{g->num_layers, p->weights_layer}, {g->num_kv_heads, p->weights_head}}))
             return fail(MKB_ERR_INVALID_ARGUMENT, "prompt: key weights unaligned, or heads or layers of them overlap");
         if (!p->weights_workspace || ((uintptr_t)p->weights_workspace & 255) ||
             p->weights_workspace_bytes < mkb_prompt_weights_bytes(g, p->tokens, p->pos0, p->observed))

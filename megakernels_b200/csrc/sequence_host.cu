@@ -71,7 +71,7 @@ int check(const MkbsReorder* r) {
     for (int i = 0; i < r->num_regions; ++i) {
         const MkbsRegion& g = r->regions[i];
         if (!g.base || g.outer < 1 || g.rows < 1 || g.row_bytes < 1) return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: region %d is empty", i);
-        if (g.row_bytes > (1 << 30) || g.slot_stride < g.rows * g.row_bytes || (g.outer > 1 && g.outer_stride < g.rows * g.row_bytes))
+        if (g.row_bytes > (1 << 30) || g.slot_stride < g.rows * g.row_bytes || !mkbs::apart(g.rows * g.row_bytes, {{g.outer, g.outer_stride}, {r->slots, g.slot_stride}}))
             return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: slots or layers of region %d overlap", i);
         for (int j = 0; j < i; ++j)  // (blocks would move the same rows at once)
             if (r->regions[j].base == g.base) return fail(MKBS_ERR_INVALID_ARGUMENT, "reorder: regions %d and %d are the same", j, i);
@@ -109,8 +109,7 @@ int check(const MkbsKeyWeights* w) {
     if ((w->layers > 1 && (w->q_layer < w->queries * q_row || w->k_layer < w->positions * k_row)) ||
         (w->sequences > 1 && (w->q_sequence < w->queries * q_row || w->k_sequence < w->positions * k_row)))
         return invalid("key weights: sequences or layers of q or k overlap");
-    if ((w->kv_heads > 1 && w->w_head < w->positions) || (w->sequences > 1 && w->w_sequence < w->positions) || (w->layers > 1 && w->w_layer < w->positions))
-        return invalid("key weights: weights overlap");
+    if (!mkbs::apart(w->positions, {{w->layers, w->w_layer}, {w->sequences, w->w_sequence}, {w->kv_heads, w->w_head}})) return invalid("key weights: weights overlap");
     if (!(w->scale - w->scale == 0.f)) return invalid("key weights: scale is not finite");
     if (!aligned(w->workspace, 256) || w->workspace_bytes < mkbs::key_weights_bytes(*w))
         return invalid("key weights: workspace missing, unaligned or too small");
@@ -123,7 +122,7 @@ int check(const MkbsSelect* s) {
     if (s->keep < 1 || s->sinks < 0 || s->recent < 0 || (int64_t)s->sinks + s->recent > s->keep)
         return invalid("select: keep must be positive and hold the sinks and the recent rows");
     if (!aligned(s->weights, 4) || !aligned(s->rows, 4) || (s->kept && !aligned(s->kept, 4))) return invalid("select: weights or rows missing or unaligned");
-    if (s->kept && ((s->kv_heads > 1 && s->w_head < s->positions) || (s->sequences > 1 && s->w_sequence < s->positions) || (s->layers > 1 && s->w_layer < s->positions)))
+    if (s->kept && !mkbs::apart(s->positions, {{s->layers, s->w_layer}, {s->sequences, s->w_sequence}, {s->kv_heads, s->w_head}}))
         return invalid("select: kept weights overlap");
     return MKBS_OK;
 }
@@ -137,8 +136,8 @@ int check(const MkbsMove* m) {
     if (!aligned(m->rows, 4) || !aligned(m->caches[0], 16) || (m->caches[1] && !aligned(m->caches[1], 16)) || m->c_layer % 16 || m->c_sequence % 16)
         return invalid("move: rows or caches missing or unaligned");
     if (m->caches[0] == m->caches[1]) return invalid("move: both caches are the same");
-    const int64_t bytes = (int64_t)m->positions * m->kv_heads * m->head_bytes;
-    if ((m->layers > 1 && m->c_layer < bytes) || (m->sequences > 1 && m->c_sequence < bytes)) return invalid("move: sequences or layers overlap");
+    if (!mkbs::apart((int64_t)m->positions * m->kv_heads * m->head_bytes, {{m->layers, m->c_layer}, {m->sequences, m->c_sequence}}))
+        return invalid("move: sequences or layers overlap");
     return MKBS_OK;
 }
 

@@ -1,6 +1,11 @@
 // Launchers of the operators between two decoding steps (one translation unit per group); arguments have been checked.
 #pragma once
+#include <algorithm>
 #include <atomic>
+#include <initializer_list>
+#include <memory>
+#include <new>
+#include <utility>
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -37,6 +42,40 @@ inline cudaError_t allow_shared_memory() {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStaticShared);
     if (e == cudaSuccess) set[dev & 63].store(dev < 64, std::memory_order_relaxed);
     return e;
+}
+
+// Whether blocks of `size` are apart that begin at i s[0] + j s[1] + k s[2], i below n[0] and so on (s, of a dimension of one: anything).
+inline bool apart(int64_t size, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+    std::pair<int64_t, int64_t> d[3];  // (stride, count)
+    int m = 0;
+    int64_t blocks = 1;
+    for (const auto& [n, s] : dims) {
+        if (n < 2) continue;
+        if (s < size) return false;
+        d[m++] = {s, n};
+        blocks *= n;
+    }
+    std::sort(d, d + m);
+    int64_t extent = size;
+    bool nested = true;  // each stride steps over all that the smaller ones reach: the usual case
+    for (int i = 0; i < m; ++i) {
+        nested = nested && d[i].first >= extent;
+        extent += d[i].first * (d[i].second - 1);
+    }
+    if (nested || m < 2) return nested;
+    if (blocks > 1 << 24) return false;  // (interleaved: every block is looked at)
+    const std::unique_ptr<int64_t[]> at(new (std::nothrow) int64_t[blocks]);
+    if (!at) return false;
+    int64_t have = 1;
+    at[0] = 0;
+    for (int i = 0; i < m; ++i) {
+        for (int64_t j = have; j < have * d[i].second; ++j) at[j] = at[j - have] + d[i].first;
+        have *= d[i].second;
+    }
+    std::sort(at.get(), at.get() + blocks);
+    for (int64_t j = 1; j < blocks; ++j)
+        if (at[j] - at[j - 1] < size) return false;
+    return true;
 }
 
 cudaError_t beam_launch(const MkbsBeams& b, cudaStream_t s);

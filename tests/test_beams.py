@@ -475,6 +475,20 @@ def test_tokens_observed_one_at_a_time():
 
 
 @pytest.mark.gpu
+def test_weights_of_layers_that_meet_are_refused():
+    model, gen = observed_generator("1b", 64, 8)
+    globs, (layers, heads, rows) = gen.schedule.globs, gen.schedule.globs.key_weights.shape
+    for layer in (rows, rows * (heads - 1), rows * heads - 4):
+        globs.key_weights = torch.zeros(layers * heads * rows, device="cuda").as_strided((layers, heads, rows), (layer, rows, 1))
+        with pytest.raises(RuntimeError, match="overlap"):
+            gen.prefill(prompt(10, 1))
+    globs.key_weights = torch.zeros(heads, layers, rows, device="cuda").transpose(0, 1)
+    gen.prefill(prompt(10, 1))
+    gen.check()
+    assert globs.key_weights.any(dim=-1).all()
+
+
+@pytest.mark.gpu
 def test_observing_needs_whole_prompts():
     model, gen = observed_generator("1b", 64, 8)
     gen.replace_with_noops()

@@ -158,6 +158,36 @@ def test_only_the_device_is_missing_in_the_calls_that_the_refusals_start_from(na
     assert getattr(lib, f"mkb_{name}")(None, None) == 1
 
 
+OVERLAPPING = [  # strides of more than one block's size, that several blocks share all the same
+    ("key_weights", weights_struct, [dict(w_sequence=100), dict(w_sequence=150), dict(w_layer=100), dict(w_layer=200), dict(w_layer=399), dict(w_head=200), dict(w_head=250, w_layer=1000)]),
+    ("select_rows", select_struct, [dict(kept=FAKE, w_sequence=100), dict(kept=FAKE, w_layer=300), dict(kept=FAKE, w_layer=200), dict(kept=FAKE, kv_heads=3, w_head=200, w_sequence=350, w_layer=2000)]),
+    ("move_rows", move_struct, [dict(c_layer=25600), dict(c_layer=25616), dict(c_layer=38400), dict(c_sequence=51200), dict(sequences=3, c_layer=38400, c_sequence=51200)]),
+    ("reorder_slots", reorder_struct, [dict(region=dict(outer_stride=1000)), dict(region=dict(outer_stride=7000)), dict(region=dict(outer_stride=1500)), dict(region=dict(slot_stride=8000))]),
+]
+
+
+@pytest.mark.parametrize("name,make,kw", [(n, m, kw) for n, m, cases in OVERLAPPING for kw in cases], ids=lambda v: str(v)[:60] if isinstance(v, (str, dict)) else "")
+def test_strides_that_meet_are_refused(name, make, kw):
+    lib, s = ops.load_library(), make(**kw)
+    assert getattr(lib, f"mkb_{name}")(ctypes.byref(s), None) == 1
+    assert "overlap" in lib.mkb_sequences_last_error().decode()
+
+
+APART = [
+    ("key_weights", weights_struct, [dict(w_layer=100, w_sequence=200, w_head=400), dict(w_layer=200, w_sequence=400, w_head=100), dict(w_layer=1, layers=1), dict(w_head=0, kv_heads=1)]),
+    ("select_rows", select_struct, [dict(w_head=0, w_layer=0), dict(kept=FAKE, w_layer=100, w_sequence=200, w_head=400), dict(kept=FAKE, kv_heads=3, w_head=200, w_sequence=300, w_layer=800)]),
+    ("move_rows", move_struct, [dict(c_layer=25600, c_sequence=51200), dict(sequences=3, c_layer=38400, c_sequence=76800), dict(sequences=1, c_sequence=0)]),
+    ("reorder_slots", reorder_struct, [dict(region=dict(outer_stride=1000, slot_stride=2000)), dict(region=dict(outer_stride=1500, slot_stride=3000)), dict(region=dict(outer=1, outer_stride=0))]),
+]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls are right: with a device they would run")
+@pytest.mark.parametrize("name,make,kw", [(n, m, kw) for n, m, cases in APART for kw in cases], ids=lambda v: str(v)[:60] if isinstance(v, (str, dict)) else "")
+def test_any_order_of_dimensions_is_taken_that_keeps_blocks_apart(name, make, kw):
+    """(Also interleaved ones, where no dimension steps over all of another.)"""
+    assert getattr(ops.load_library(), f"mkb_{name}")(ctypes.byref(make(**kw)), None) == 2
+
+
 def test_the_same_region_twice_is_refused():
     """Two regions, then the same one twice."""
     lib, s = ops.load_library(), reorder_struct()
