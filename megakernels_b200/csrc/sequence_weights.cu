@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         tc_after_sync();
         tmem = (uint32_t)ctl[1];
         let_next();  // (not before: a block of the next launch that held tensor memory would wait for this one, and this one for the memory)
+        if (kKeys) after_previous();  // (the limit of waits is not for the launch before this one)
     }
 
     const int of_tile = kTile / a.per, box_bytes = kDim / 64 * of_tile * a.per * 128;

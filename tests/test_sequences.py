@@ -596,6 +596,26 @@ def test_key_weights_of_parts_of_larger_tensors():
 
 
 @pytest.mark.gpu
+def test_waits_do_not_count_the_time_of_the_launch_before():
+    """One sequence's rows pass takes some 3 ms, while the blocks of the keys pass already wait on all other SMs: 1 ms is a limit for each wait of
+    a block for its own copies and products."""
+    others, long = 74, 600_000
+    lengths = [long] + [100] * others
+    q = draw(1, 1, 1 + others, 17, 1, 64, dtype=BF16)
+    k = torch.empty(1, 1 + others, long, 1, 64, dtype=BF16, device="cuda")
+    k[:, 0] = torch.randn(long, 1, 64, generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(BF16)
+    k[:, 1:, :100] = draw(2, 1, others, 100, 1, 64, dtype=BF16)
+    w = torch.zeros(1, 1 + others, 1, long, device="cuda")
+    status = torch.zeros(16, dtype=torch.int32, device="cuda")
+    ops.key_weights(q, k, w, torch.tensor(lengths, dtype=torch.int32).cuda(), scale=0.125, status=status, wait_timeout_ms=1)
+    torch.cuda.synchronize()
+    assert not status.any(), status.tolist()
+    want, tol = weights_reference(q[:, 1:], k[:, 1:, :100], torch.zeros(1, others, 1, 100, device="cuda"), [100] * others, 0.125)
+    assert ((w[:, 1:, :, :100].double() - want).abs() <= tol * want).all() and not w[:, 1:, :, 100:].any()
+    assert abs(float(w[0, 0].double().sum()) - 17) <= 17 * (tol + 2 * HALF)
+
+
+@pytest.mark.gpu
 def test_key_weights_are_the_same_bits_every_time():
     q, k, w, scale = weights_case(5, 1, 1, 100, 8, 2, 128, 3000, [3000])
     lengths, first = torch.tensor([3000], dtype=torch.int32).cuda(), None
