@@ -15,10 +15,13 @@
 // Steps: warps of a scheduler need not meet at a unit's end (-5 us), one warp finds the units (-2), chosen lanes of whole warps issue (-0.5).
 // No gain: twice the columns a thread (57 and 78 us then), a polynomial for every fourth exponential, halves of a step's columns loaded while the
 // others are summed (59.5), waits that poll (64).
-// Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the scores go
-// through memory (4 bytes a row where a key has 128 or 256).  One query on 65001 keys (32 heads of 64, 8 of keys): 21 us, 3.4 TB/s.  Blocks
+// Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the products go
+// through memory (4 bytes a row where a key has 128 or 256), not yet scaled: with scaled scores, rounded before a row's logarithm was taken
+// from them, large scores lost a weight's last digits (1.4e-3 of it at scores of 2^15; 20.4 us instead of 20.7 for 4 rows, 33.5 instead of 33.0 for 16).  One query on 65001 keys (32 heads of 64, 8 of keys): 21 us, 3.4 TB/s.  Blocks
 // that all fit the SMs at once: 26.6 -> 22.9 us against four per SM, of which three fit; the sum's loads issued together and before the
 // statistics: 21.3; heads of the same keys in neighbouring blocks: 21.0.  Twice the loads of a warp, or two batches in turn: 24.
+#include <cfloat>
+
 #include "hybrid_kernels.h"
 #include "hybrid_tcgen05.cuh"
 #include "sequence_kernels.h"
@@ -47,7 +50,8 @@ struct WeightArgs {
     float2* stats;  // [item][row tile][split][128]: maximum and sum;  few rows: [item][split][16]
     float* offs;    // [item][row tile][128]: log2 of a row's sum, infinite where a row sees no key or there is no row
     float* sums;    // [item][part][key tile][128]: weights, where there are parts
-    float* scores;  // few rows: [item][position][row], rows rounded up to 4, 8 or 16
+    float* scores;  // few rows: products, [item][position][row], rows rounded up to 4, 8 or 16
+    float hidden;   // the product of a key that a row does not see: minus infinity when scaled
     int* status;
     unsigned long long timeout_ns;
 };
@@ -530,13 +534,15 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(kDim)) weights_few_ker
             const int j = (g0 + u) * 8 + 2 * c;
 #pragma unroll
             for (int h = 0; h < kRowsPad / 8 + (kRowsPad == 4); ++h) {
-                const float z0 = j <= last[h] ? d[2 * h] * a.scale : -INFINITY, z1 = j + 1 <= last[h] ? d[2 * h + 1] * a.scale : -INFINITY;
-                const float top = fmaxf(fmaxf(z0, z1), stats[h].x);
+                // (products, not scores, are kept: scaled and taken from a reference in one operation they are rounded once, near the result)
+                const float x0 = j <= last[h] ? d[2 * h] : a.hidden, x1 = j + 1 <= last[h] ? d[2 * h + 1] : a.hidden;
+                const float top = fmaxf(fmaxf(x0 * a.scale, x1 * a.scale), stats[h].x);
                 if (n + 8 * h < kRowsPad) {
-                    if (j < it.n) scores[(int64_t)j * kRowsPad + n + 8 * h] = z0;
-                    if (j + 1 < it.n) scores[(int64_t)(j + 1) * kRowsPad + n + 8 * h] = z1;
+                    if (j < it.n) scores[(int64_t)j * kRowsPad + n + 8 * h] = x0;
+                    if (j + 1 < it.n) scores[(int64_t)(j + 1) * kRowsPad + n + 8 * h] = x1;
                 }
-                if (top > -INFINITY) stats[h] = make_float2(top, stats[h].y * fast_exp2(stats[h].x - top) + fast_exp2(z0 - top) + fast_exp2(z1 - top));
+                if (top > -INFINITY)
+                    stats[h] = make_float2(top, stats[h].y * fast_exp2(stats[h].x - top) + fast_exp2(fmaf(x0, a.scale, -top)) + fast_exp2(fmaf(x1, a.scale, -top)));
             }
         }
     }
@@ -557,7 +563,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(kDim)) weights_few_ker
 
 template <int kRowsPad>
 __global__ void __launch_bounds__(kFewThreads) weights_sum_kernel(const WeightArgs a) {
-    __shared__ float off[kFew];
+    __shared__ float2 of_row[kFew];  // its largest score, one over its sum
     const Item it(a, blockIdx.y);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float* const scores = a.scores + (int64_t)blockIdx.y * a.positions * kRowsPad;
@@ -584,20 +590,24 @@ __global__ void __launch_bounds__(kFewThreads) weights_sum_kernel(const WeightAr
         for (int i = lane; i < a.splits; i += 32) all = join(all, parts[i * kFew]);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) all = join(all, make_float2(__shfl_xor_sync(0xffffffffu, all.x, o), __shfl_xor_sync(0xffffffffu, all.y, o)));
-        if (lane == 0) off[r] = off_of(all.x, all.y);
+        if (lane == 0) of_row[r] = all.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(all.x, 1.f / all.y);  // (one that sees no key: no weights)
     }
     __syncthreads();
+    float2 row[kRowsPad];
+#pragma unroll
+    for (int r = 0; r < kRowsPad; ++r) row[r] = of_row[r];
+    auto add = [&](float& sum, int r, float x) { sum = fmaf(fast_exp2(fmaf(x, a.scale, -row[r].x)), row[r].y, sum); };
     while (j < it.n) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
             if (j + (int64_t)i * step < it.n) {
-                float sum = 0.f;
+                float two[2] = {0.f, 0.f};
 #pragma unroll
                 for (int r = 0; r < kRowsPad; r += 4) {
                     const float4 x = z[i][r / 4];
-                    sum += (fast_exp2(x.x - off[r]) + fast_exp2(x.y - off[r + 1])) + (fast_exp2(x.z - off[r + 2]) + fast_exp2(x.w - off[r + 3]));
+                    add(two[0], r, x.x), add(two[1], r + 1, x.y), add(two[0], r + 2, x.z), add(two[1], r + 3, x.w);
                 }
-                weights[j + i * step] = w[i] + sum;
+                weights[j + i * step] = w[i] + (two[0] + two[1]);
             }
         j += (int64_t)kBatch * step;
         if (j < it.n) load(j);
@@ -630,6 +640,8 @@ struct Plan {
         a.rows = w.queries * a.per;
         a.items = w.layers * w.sequences * w.kv_heads;
         a.scale = w.scale * kLog2e;
+        if (a.scale == 0.f) a.scale = FLT_MIN;  // (what is hidden stays so; products below 2^100 all have the same weight)
+        a.hidden = a.scale > 0.f ? -INFINITY : INFINITY;
         a.q = static_cast<const bf16*>(w.q);
         a.k = static_cast<const bf16*>(w.k);
         a.q_layer = w.q_layer, a.q_sequence = w.q_sequence, a.k_layer = w.k_layer, a.k_sequence = w.k_sequence;

@@ -596,6 +596,24 @@ def test_key_weights_of_parts_of_larger_tensors():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("queries,heads,kv_heads", [(1, 4, 1), (1, 16, 2), (3, 10, 2), (16, 1, 1)])
+def test_weights_of_few_rows_of_large_scores(queries, heads, kv_heads):
+    """Every score is some 32768 and differs from others by 0 to 6: products are exact whole numbers, and what is rounded is small."""
+    n, per = 2000, heads // kv_heads
+    q = torch.full((1, 1, queries, heads, 64), 16.0)
+    k = torch.full((1, 1, n, kv_heads, 64), 16.0)
+    q[..., 63] = 1
+    k[..., 63] = torch.randint(0, 4, (1, 1, n, kv_heads), generator=torch.Generator().manual_seed(queries)).float()
+    q, k, w = q.to(BF16).cuda(), k.to(BF16).cuda(), torch.zeros(1, 1, kv_heads, n, device="cuda")
+    want, _ = weights_reference(q, k, w, [n], 2.0)
+    ops.key_weights(q, k, w, n, scale=2.0)
+    # The scale is rounded twice and multiplies differences of 6; an exponential is off by 2^-22, a row's sum by that, by what changing its reference
+    # takes (the same, up to three times in each of 8 lanes' and warps' joins) and by its additions
+    tol = 6 * 2.0**-22 + 2.0**-22 * (2 + 3 * 8) + (n / 32 + 64 + per * queries) * HALF
+    assert ((w.double() - want).abs() <= tol * want).all(), float(((w.double() - want).abs() / want).max())
+
+
+@pytest.mark.gpu
 def test_waits_do_not_count_the_time_of_the_launch_before():
     """One sequence's rows pass takes some 3 ms, while the blocks of the keys pass already wait on all other SMs: 1 ms is a limit for each wait of
     a block for its own copies and products."""
