@@ -339,20 +339,29 @@ class MK_Generator(Generator):
             globs.key_weights = torch.zeros(L, Hkv, T, dtype=torch.float32, device=globs.k_cache.device)
             # rows and positions part ways with the first eviction: tables by row, of this generator alone
             globs.rope_cos, globs.rope_sin = globs.rope_cos.clone(), globs.rope_sin.clone()
-            self._turns(2 * globs.rope_cos.shape[0])
+            self._turns(0, globs.rope_cos.shape[0])
         self.observed = window
 
-    _more_turns: tuple[Tensor, Tensor] | None = None
+    _near_turns: tuple[int, Tensor, Tensor] | None = None  # (first position, cosines, sines)
+    _far_turns: tuple[int, Tensor, Tensor] | None = None
 
-    def _turns(self, count: int) -> tuple[Tensor, Tensor]:
-        """Rotation tables of ``count`` positions or more.  (They are made on the host, a few ms for a long cache: ahead of evictions.)"""
-        model = self.model
-        tables = self._more_turns or (model.model.rope_cos, model.model.rope_sin)
-        have, rows = tables[0].shape[0], self.schedule.globs.rope_cos.shape[0]
-        if have < count:
-            more = build_rope_tables(model.config, max(count - have, rows), model.extra_config.interleave_rope, have)
-            tables = self._more_turns = tuple(torch.cat([t, m.to(t)]) for t, m in zip(tables, more))
-        return tables
+    def _turns(self, first: int, count: int) -> tuple[Tensor, Tensor]:
+        """Rotation tables of ``count`` positions from ``first`` on.  (They are made on the host, a few ms for a long cache: those that the first
+        evictions of a sequence need when observing begins, later ones a cache's rows ahead, and what lies before ``first`` goes.)"""
+        model, rows = self.model, self.schedule.globs.rope_cos.shape[0]
+        for start, *tables in filter(None, (self._near_turns, self._far_turns)):
+            if start <= first and first + count <= start + tables[0].shape[0]:
+                return tuple(t[first - start : first - start + count] for t in tables)
+        start, *tables = self._far_turns or self._near_turns or (0, model.model.rope_cos, model.model.rope_sin)
+        old = [t[max(first - start, 0) :] for t in tables]
+        have = max(start + tables[0].shape[0], first)
+        more = build_rope_tables(model.config, max(first + count + rows - have, 0), model.extra_config.interleave_rope, have)
+        made = (first, *(torch.cat([t, m.to(t)]) for t, m in zip(old, more)))
+        if first == 0:
+            self._near_turns = made
+        else:
+            self._far_turns = made
+        return tuple(t[:count] for t in made[1:])
 
     def _start_sequence(self) -> None:
         globs = self.schedule.globs
@@ -367,10 +376,12 @@ class MK_Generator(Generator):
         if evicted == self.evicted:
             return
         rows = globs.rope_cos.shape[0]
-        cos, sin = self._turns(evicted + rows)
-        globs.rope_cos.copy_(cos[evicted : evicted + rows])
-        globs.rope_sin.copy_(sin[evicted : evicted + rows])
+        cos, sin = self._turns(evicted, rows)
+        globs.rope_cos.copy_(cos)
+        globs.rope_sin.copy_(sin)
         self.evicted = evicted
+        if evicted == 0:
+            self._far_turns = None
 
     def evict(self, length: int, keep: int, sinks: int = 4, recent: int = 64) -> int:
         """Cut a cache of ``length`` rows to ``keep`` in place; returns the rows that it holds then, which is the position to

@@ -458,6 +458,25 @@ def test_rows_behind_what_is_evicted_lose_their_weights():
 
 
 @pytest.mark.gpu
+def test_rotations_of_positions_that_have_gone_are_not_kept():
+    """Forty evictions of 40 rows in a cache of 64: what is held for rotations stays a few caches' rows, and goes with the sequence."""
+    model, gen = observed_generator("1b", 64, 8)
+    globs, at, held = gen.schedule.globs, 0, []
+    table = globs.rope_cos.numel() * globs.rope_cos.element_size() * 2
+    for turn in range(40):
+        gen.prefill(prompt(60 - at, turn), position=at)
+        at = gen.evict(60, 20, 2, 4)
+        assert gen.evicted == 40 * (turn + 1)
+        want = build_rope_tables(model.config, globs.rope_cos.shape[0], True, first=gen.evicted)
+        assert torch.equal(globs.rope_cos.cpu(), want[0]) and torch.equal(globs.rope_sin.cpu(), want[1])
+        held.append(torch.cuda.memory_allocated())
+    assert max(held) - held[0] <= 3 * table + 4096  # (a window of two caches' rows, and what its making may leave for a moment)
+    gen.prefill(prompt(10, 9))
+    gen.check()
+    assert torch.cuda.memory_allocated() <= held[0] + 4096 and gen.evicted == 0
+
+
+@pytest.mark.gpu
 def test_tokens_observed_one_at_a_time():
     """A prompt cut into single tokens is weighed as it is at once.  Queries and keys of other products differ by the last bit of bf16 here and
     there: single weights by a few hundredths, a query's sum only by the rounding of its own terms."""
