@@ -181,6 +181,12 @@ class _Where:
                     t.record_stream(self.other)
 
 
+def _fit(*numbers: int) -> None:
+    """What goes into a struct's 32 bits: ctypes cuts other numbers without a word.  (Asked only where some number is negative or large.)"""
+    if min(numbers) < -(2**31) or max(numbers) >= 2**31:
+        raise ValueError(f"a number or a size does not fit 32 bits: {max(numbers, key=abs)}")
+
+
 def _struct(kind):
     s = kind()
     s.struct_bytes = ctypes.sizeof(kind)
@@ -229,6 +235,8 @@ def beam_select(logits: Tensor, scores: Tensor | None = None, *, beams: int, k: 
     rows, vocab = logits.shape
     if beams < 1 or rows < 1 or rows % beams:
         raise ValueError(f"{rows} rows of logits are no groups of {beams}")
+    if (rows | vocab | k | (eos or 0)) >> 31:
+        _fit(rows, vocab, k, eos or 0)
     _refuse_host("logits", logits)
     lib, where, groups = load_library(), _Where(stream, logits), rows // beams
     s, device = _struct(MkbsBeams), where.device
@@ -267,6 +275,8 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
         raise ValueError("first counts rows: it is not negative and needs lengths")
     if not isinstance(parents, Tensor) or parents.ndim != 1:
         raise ValueError("parents must be int32 [slots]")
+    if (first | parents.shape[0]) >> 31:
+        _fit(first, parents.shape[0])
     _refuse_host("parents", parents)
     load_library()
     slots, where = parents.shape[0], _Where(stream, parents)
@@ -292,6 +302,8 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
             raise ValueError(f"tensor {i} {list(shape)} does not have {slots} slots in dimension {dim}" + (" and rows behind it" if by_rows else ""))
         if t.numel() == 0:
             raise ValueError(f"tensor {i} is empty")
+        if (shape[0] | shape[dim + by_rows]) >> 31:
+            _fit(shape[0], shape[dim + by_rows])
         r.base = _check(f"tensor {i}", t, t.dtype, device, inner=len(shape) - dim - 1)
         size = t.element_size()
         slot_bytes = math.prod(shape[dim + 1 :]) * size
@@ -318,12 +330,15 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
     """
     if not all(isinstance(t, Tensor) for t in (q, keys, weights)) or q.ndim != 5 or keys.ndim != 5:
         raise ValueError("q must be [layers, sequences, queries, heads, dim], keys [layers, sequences, positions, kv_heads, dim]")
+    layers, sequences, queries, heads, dim = q.shape
+    positions, kv_heads = keys.shape[2:4]
+    if (wait_timeout_ms | layers | sequences | queries | heads | positions | kv_heads) >> 31:
+        _fit(wait_timeout_ms, *q.shape, *keys.shape)
+        raise ValueError(f"a limit of {wait_timeout_ms} ms")
     _refuse_host("q", q)
     lib, where, bf16 = load_library(), _Where(stream, q), torch.bfloat16
     s, device = _struct(MkbsKeyWeights), where.device
-    layers, sequences, s.queries, s.heads, dim = q.shape
-    positions, kv_heads = keys.shape[2:4]
-    s.layers, s.sequences, s.dim, s.positions, s.kv_heads = layers, sequences, dim, positions, kv_heads
+    s.layers, s.sequences, s.queries, s.heads, s.dim, s.positions, s.kv_heads = layers, sequences, queries, heads, dim, positions, kv_heads
     s.q = _check("q", q, bf16, device, inner=3)
     s.k = _check("keys", keys, bf16, device, (layers, sequences, positions, kv_heads, dim), inner=3)
     s.weights = _check("weights", weights, torch.float32, device, (layers, sequences, kv_heads, positions), inner=1)
@@ -350,11 +365,13 @@ def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int
     """
     if not isinstance(weights, Tensor) or weights.ndim != 4:
         raise ValueError("weights must be [layers, sequences, kv_heads, positions]")
+    layers, sequences, kv_heads, positions = weights.shape
+    if (keep | sinks | recent | layers | sequences | kv_heads | positions) >> 31:
+        _fit(keep, sinks, recent, *weights.shape)
     _refuse_host("weights", weights)
     load_library()
     s, where = _struct(MkbsSelect), _Where(stream, weights)
     device = where.device
-    layers, sequences, kv_heads, positions = weights.shape
     s.layers, s.sequences, s.kv_heads, s.positions = layers, sequences, kv_heads, positions
     s.weights = _check("weights", weights, torch.float32, device, inner=1)
     s.w_layer, s.w_sequence, s.w_head = weights.stride()[:3]
@@ -376,20 +393,22 @@ def move_rows(keys: Tensor, values: Tensor | None, rows: Tensor, lengths: Tensor
     kv_heads, dim]`` of one shape; ``rows`` as :func:`select_rows` returns them, ``lengths`` as it was given there."""
     if not all(isinstance(t, Tensor) for t in (keys, rows)) or keys.ndim != 5 or rows.ndim != 4:
         raise ValueError("caches must be [layers, sequences, positions, kv_heads, dim], rows [layers, sequences, kv_heads, keep]")
+    layers, sequences, positions, kv_heads, dim = keys.shape
+    keep, size = rows.shape[3], keys.element_size()
+    if (layers | sequences | positions | kv_heads | dim * size | keep) >> 31:
+        _fit(*keys.shape, dim * size, keep)
     _refuse_host("keys", keys)
     load_library()
     s, where = _struct(MkbsMove), _Where(stream, keys)
     device = where.device
-    layers, sequences, positions, kv_heads, dim = keys.shape
     s.layers, s.sequences, s.positions, s.kv_heads = layers, sequences, positions, kv_heads
     s.caches[0] = _check("keys", keys, keys.dtype, device, inner=3)
     if values is not None:
         s.caches[1] = _check("values", values, keys.dtype, device, keys.shape, inner=3)
         if values.stride() != keys.stride():
             raise ValueError("keys and values must have the same strides")
-    size = keys.element_size()
     s.head_bytes, s.c_layer, s.c_sequence = dim * size, keys.stride(0) * size, keys.stride(1) * size
-    s.keep = rows.shape[3]
-    s.rows = _check("rows", rows, torch.int32, device, (layers, sequences, kv_heads, s.keep))
+    s.keep = keep
+    s.rows = _check("rows", rows, torch.int32, device, (layers, sequences, kv_heads, keep))
     lengths = _set_lengths(s, lengths, device, sequences, positions)
     where.launch("mkb_move_rows", s, keys, values, rows, lengths)

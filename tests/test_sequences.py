@@ -220,6 +220,38 @@ def test_a_length_outside_the_cache_is_refused(length):
     assert s.length == 100
 
 
+FAR = 2**32 + 5  # five, when it is cut to 32 bits
+
+
+@pytest.mark.parametrize("call", [
+    lambda z: ops.beam_select(z(2, 100), beams=2, k=FAR), lambda z: ops.beam_select(z(2, FAR), beams=2, k=3), lambda z: ops.beam_select(z(2, 100), beams=2, k=3, eos=FAR),
+    lambda z: ops.beam_select(z(2, 100), beams=2, k=5 - 2**32), lambda z: ops.reorder_slots([z(4, 9)], z(4).int(), first=FAR, lengths=z(4).int()),
+    lambda z: ops.key_weights(z(1, 1, 1, 8, 64), z(1, 1, FAR, 2, 64), z(1, 1, 2, FAR), 5, scale=1.0), lambda z: ops.key_weights(z(1, 1, FAR, 8, 64), z(1, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0),
+    lambda z: ops.key_weights(z(1, 1, 1, 8, 64), z(1, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0, wait_timeout_ms=FAR),
+    lambda z: ops.key_weights(z(1, 1, 1, 8, 64), z(1, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0, wait_timeout_ms=-1 - 2**31),
+    lambda z: ops.select_rows(z(1, 1, 2, 100), 50, keep=FAR), lambda z: ops.select_rows(z(1, 1, 2, 100), 50, keep=9, sinks=FAR), lambda z: ops.select_rows(z(1, 1, 2, 100), 50, keep=9, recent=5 - 2**32),
+    lambda z: ops.select_rows(z(FAR, 1, 2, 100), 50, keep=9), lambda z: ops.move_rows(z(1, FAR, 9, 2, 64), None, z(1, 1, 2, 9), 50), lambda z: ops.key_weights(z(FAR, 1, 1, 8, 64), z(FAR, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0),
+    lambda z: ops.select_rows(z(1, 1, 2, FAR), 50, keep=9), lambda z: ops.move_rows(z(1, 1, FAR, 2, 64), None, z(1, 1, 2, 9), 50), lambda z: ops.move_rows(z(1, 1, 9, 2, 64), None, z(1, 1, 2, FAR), 5),
+])
+def test_numbers_that_do_not_fit_are_refused(call):
+    with pytest.raises(ValueError, match="32 bits"):
+        call(lambda *shape: torch.zeros(()).expand(shape))
+
+
+def test_a_negative_limit_is_refused():
+    z = lambda *shape: torch.zeros(()).expand(shape)  # noqa: E731
+    with pytest.raises(ValueError, match="limit"):
+        ops.key_weights(z(1, 1, 1, 8, 64), z(1, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0, wait_timeout_ms=-1)
+
+
+@pytest.mark.gpu
+def test_rows_of_a_region_that_do_not_fit_are_refused():
+    """(8 GB of bytes, that nothing touches.)"""
+    t = torch.empty(2, FAR, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.reorder_slots([t], torch.tensor([1, 0], dtype=torch.int32).cuda(), lengths=torch.tensor([5, 5], dtype=torch.int32).cuda())
+
+
 def test_beam_selection_takes_all_it_says_it_takes():
     """Every shape at the limits has a plan that fits shared memory."""
     lib = ops.load_library()
