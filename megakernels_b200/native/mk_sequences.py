@@ -8,13 +8,15 @@ sizes; a missing library is an ImportError, never a fallback.
 Every function enqueues its work on ``stream`` (a stream, a handle, or None for the current one) of the
 current device, where all tensors must live, and neither synchronises nor reads anything back, so all of
 them can be captured into a CUDA graph.  Arguments that the library does not take raise ``ValueError`` /
-``TypeError`` here or ``SequenceError`` from its own checks, before anything is launched.
+``TypeError`` here or ``SequenceError`` from its own checks, before anything is launched.  A wait on the device that
+gives up is recorded there, and :func:`raise_status` looks.
 """
 
 from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from pathlib import Path
 
 import torch
@@ -200,8 +202,31 @@ def _check_status(status, device: int) -> int:
     return at
 
 
-def raise_status(status: Tensor) -> None:
-    """Synchronise, and raise if a wait of the calls that were given ``status`` has given up; it is cleared then."""
+_records: dict[int, Tensor] = {}  # of the calls that are given no status, by device
+_making = threading.Lock()
+
+
+def _record(device: int) -> int:
+    record = _records.get(device)
+    if record is None:
+        with _making:
+            if device not in _records:
+                record = torch.empty(16, dtype=torch.int32, device=torch.device("cuda", device))
+                with torch.cuda.stream(torch.cuda.Stream(device)):  # (the current one may be under capture, and a replay shall not clear the record)
+                    record.zero_()
+                _records[device] = record
+        record = _records[device]
+    return record.data_ptr()
+
+
+def raise_status(status: Tensor | None = None) -> None:
+    """Synchronise, and raise if a wait of the calls that were given ``status`` has given up (None: of the calls on the current
+    device that were given none); it is cleared then."""
+    if status is None:
+        status = _records.get(torch.cuda.current_device())
+        if status is None:
+            return
+        torch.cuda.synchronize()
     code, block = status[:2].tolist()
     if code:
         status.zero_()
@@ -264,7 +289,7 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
 
     With ``lengths`` (int32 ``[slots]``) the dimension behind it is rows: a slot takes its parent's rows ``first ..
     lengths[parent] - 1``; the others stay.  ``parents`` int32 ``[slots]``; one outside the slots leaves its slot as it is.
-    ``status``: int32 ``[16]``, zero, for a wait that gives up (:func:`raise_status`).
+    ``status``: int32 ``[16]``, zero, for a wait that gives up, after which not all rows have moved (:func:`raise_status`).
     """
     tensors = list(tensors)
     if not tensors:
@@ -284,8 +309,7 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
     base.slots, base.first = slots, first
     base.parents = _check("parents", parents, torch.int32, device)
     by_rows = lengths is not None
-    if status is not None:
-        base.status = _check_status(status, device)
+    base.status = _record(device) if status is None else _check_status(status, device)
     if by_rows:
         base.lengths = _check("lengths", lengths, torch.int32, device, (slots,))
     regions = (MkbsRegion * len(tensors))()
@@ -322,7 +346,8 @@ def reorder_slots(tensors: list[Tensor], parents: Tensor, *, dim: int = 0, first
 def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int, *, scale: float, status: Tensor | None = None, wait_timeout_ms: int = 0,
                 stream=None) -> None:
     """Add to ``weights`` (float32 ``[layers, sequences, kv_heads, positions]``) the softmax weight that each cached key
-    receives from the queries, summed over them and over the query heads that share the key.  ``status``: as in :func:`reorder_slots`.
+    receives from the queries, summed over them and over the query heads that share the key.  ``status``: as in :func:`reorder_slots`
+    (not all weights have been added then).
 
     ``q`` bf16 ``[layers, sequences, queries, heads, dim]``: the queries of the sequences' last rows; ``keys`` bf16 ``[layers,
     sequences, positions, kv_heads, dim]``, dim 64 or 128; ``lengths``: rows that each sequence holds, an int32 tensor
@@ -347,8 +372,7 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
     s.w_layer, s.w_sequence, s.w_head = weights.stride()[:3]
     lengths = _set_lengths(s, lengths, device, sequences, positions)
     s.scale, s.wait_timeout_ms = scale, wait_timeout_ms
-    if status is not None:
-        s.status = _check_status(status, device)
+    s.status = _record(device) if status is None else _check_status(status, device)
     size = lib.mkb_key_weights_bytes(s)
     if not size:
         where.launch("mkb_key_weights", s)  # (says what is wrong)

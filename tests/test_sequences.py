@@ -666,6 +666,53 @@ def test_waits_do_not_count_the_time_of_the_launch_before():
 
 
 @pytest.mark.gpu
+def test_a_wait_that_gives_up_is_recorded_without_a_status(monkeypatch):
+    """Calls that are given no status name the device's own record, which is raised and cleared.  (No call here waits in vain.)"""
+    q, k, w = draw(1, 1, 1, 20, 4, 64, dtype=BF16), draw(2, 1, 1, 50, 2, 64, dtype=BF16), torch.zeros(1, 1, 2, 50, device="cuda")
+    named, launch = [], ops._Where.launch
+    monkeypatch.setattr(ops._Where, "launch", lambda self, name, s, *used: (named.append(s.status), launch(self, name, s, *used)))
+    ops.key_weights(q, k, w, 50, scale=0.1)
+    ops.reorder_slots([draw(1, 4, 16)], torch.tensor([1, 0, 0, 2], dtype=torch.int32).cuda())
+    record = ops._records[torch.cuda.current_device()]
+    assert named == [record.data_ptr()] * 2
+    ops.raise_status()
+    record[:2] = torch.tensor([3, 41])
+    with pytest.raises(ops.SequenceError, match="block 41") as e:
+        ops.raise_status()
+    assert e.value.code == 3
+    ops.raise_status()
+    given = torch.zeros(16, dtype=torch.int32, device="cuda")
+    ops.key_weights(q, k, w, 50, scale=0.1, status=given)
+    assert named[2] == given.data_ptr()
+
+
+@pytest.mark.gpu
+def test_a_call_without_a_status_may_be_the_first_and_captured():
+    code = f"""
+import sys; sys.path.insert(0, {str(ROOT)!r})
+import torch
+from megakernels_b200.native import mk_sequences as ops
+a, b = torch.arange(12.0, device="cuda").view(3, 4), torch.tensor([2, 0, 0], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.reorder_slots([a], b)
+graph.replay()
+ops.raise_status()
+assert a[:, 0].tolist() == [8.0, 0.0, 0.0], a
+next(iter(ops._records.values()))[0] = 3  # (as a kernel leaves it; a replay does not clear it)
+graph.replay()
+try:
+    ops.raise_status()
+except ops.SequenceError as e:
+    assert e.code == 3
+else:
+    raise AssertionError
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+@pytest.mark.gpu
 def test_key_weights_are_the_same_bits_every_time():
     q, k, w, scale = weights_case(5, 1, 1, 100, 8, 2, 128, 3000, [3000])
     lengths, first = torch.tensor([3000], dtype=torch.int32).cuda(), None
