@@ -156,6 +156,8 @@ class _Where:
             self.other = torch.cuda.ExternalStream(stream, device=self.device) if stream else torch.cuda.default_stream(self.device)
             self.handle = stream
         else:
+            if stream.device_index != self.device:  # (a launch goes to the current device)
+                raise ValueError(f"the stream is cuda:{stream.device_index}'s but the current device is cuda:{self.device}")
             self.other, self.handle = stream, stream.cuda_stream
 
     def empty(self, shape: tuple[int, ...], strides: tuple[int, ...], dtype) -> Tensor:

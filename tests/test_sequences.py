@@ -9,6 +9,7 @@ import re
 import subprocess
 import sys
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -250,6 +251,14 @@ def test_rows_of_a_region_that_do_not_fit_are_refused():
     t = torch.empty(2, FAR, dtype=torch.uint8, device="cuda")
     with pytest.raises(ValueError, match="32 bits"):
         ops.reorder_slots([t], torch.tensor([1, 0], dtype=torch.int32).cuda(), lengths=torch.tensor([5, 5], dtype=torch.int32).cuda())
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    """(Of a device that need not be there.)"""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="stream is cuda:1's"):
+        ops._Where(SimpleNamespace(device_index=1, cuda_stream=5), torch.zeros(1))
+    assert ops._Where(SimpleNamespace(device_index=0, cuda_stream=5), torch.zeros(1)).handle == 5
 
 
 def test_beam_selection_takes_all_it_says_it_takes():
