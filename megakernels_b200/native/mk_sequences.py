@@ -144,6 +144,17 @@ def _check(name: str, t, dtype, device: int, shape=None, inner: int | None = Non
     _refuse(name, t, dtype, device, shape, inner)
 
 
+def _entry_points(c):
+    """The current stream's handle, memory of a stream and its return.  torch has entry points of little host time for these that it does
+    not document; without them its public ones serve."""
+    return (getattr(c, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream),
+            getattr(c, "_cuda_cudaCachingAllocator_raw_alloc", None) or (lambda size, handle: torch.cuda.caching_allocator_alloc(size, stream=handle)),
+            getattr(c, "_cuda_cudaCachingAllocator_raw_delete", None) or torch.cuda.caching_allocator_delete)
+
+
+_raw_stream, _raw_alloc, _raw_free = _entry_points(torch._C)
+
+
 class _Where:
     """The stream of a call, and the tensors that it allocates there: given back when the call returns they go to
     that stream alone, whose later work runs after the kernels."""
@@ -151,7 +162,7 @@ class _Where:
     def __init__(self, stream, of: Tensor):
         self.device, self.where = torch.cuda.current_device(), of.device
         if stream is None:
-            self.other, self.handle = None, torch._C._cuda_getCurrentRawStream(self.device)  # (0.1 us; as an object 1.3)
+            self.other, self.handle = None, _raw_stream(self.device)  # (0.1 us; as an object 1.3)
         elif isinstance(stream, int):  # (an external stream of handle 0 would be another one from torch's pool)
             self.other = torch.cuda.ExternalStream(stream, device=self.device) if stream else torch.cuda.default_stream(self.device)
             self.handle = stream
@@ -168,11 +179,11 @@ class _Where:
 
     def launch_with(self, size: int, name: str, struct, *used) -> None:
         """A launch with ``size`` bytes of workspace, which go back to the stream behind it (as a tensor's would, in half the time)."""
-        struct.workspace, struct.workspace_bytes = torch._C._cuda_cudaCachingAllocator_raw_alloc(size, self.handle), size
+        struct.workspace, struct.workspace_bytes = _raw_alloc(size, self.handle), size
         try:
             self.launch(name, struct, *used)
         finally:
-            torch._C._cuda_cudaCachingAllocator_raw_delete(struct.workspace)
+            _raw_free(struct.workspace)
 
     def launch(self, name: str, struct, *used) -> None:
         """``used``: tensors that are not given out again before this stream has used them."""

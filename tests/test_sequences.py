@@ -261,6 +261,32 @@ def test_a_stream_of_another_device_is_refused(monkeypatch):
     assert ops._Where(SimpleNamespace(device_index=0, cuda_stream=5), torch.zeros(1)).handle == 5
 
 
+def test_torch_without_its_quick_entry_points():
+    """All three are replaced, each by itself, and what is there is taken."""
+    names = ("_cuda_getCurrentRawStream", "_cuda_cudaCachingAllocator_raw_alloc", "_cuda_cudaCachingAllocator_raw_delete")
+    assert all(callable(f) for f in ops._entry_points(SimpleNamespace()))
+    for i, name in enumerate(names):
+        points = ops._entry_points(SimpleNamespace(**{name: "quick"}))
+        assert points[i] == "quick" and all(callable(f) for j, f in enumerate(points) if j != i)
+
+
+@pytest.mark.gpu
+def test_calls_by_torch_s_public_entry_points(monkeypatch):
+    for name, f in zip(("_raw_stream", "_raw_alloc", "_raw_free"), ops._entry_points(SimpleNamespace())):
+        monkeypatch.setattr(ops, name, f)
+    side, held = torch.cuda.Stream(), []
+    for _ in range(2):  # (the first pass may leave what torch itself keeps)
+        check_beams(draw(1, 4, 3001), beams=2, k=5)
+        check_beams(draw(1, 4, 3001), beams=2, k=5, stream=side)
+        with torch.cuda.stream(side):
+            check_beams(draw(1, 4, 3001), beams=2, k=5)
+        q, k, w, scale = weights_case(3, 1, 1, 30, 8, 2, 64, 200, [200])
+        check_weights(q, k, w, [200], scale)
+        del q, k, w
+        held.append(torch.cuda.memory_allocated())
+    assert held[0] == held[1]  # (workspaces go back)
+
+
 def test_beam_selection_takes_all_it_says_it_takes():
     """Every shape at the limits has a plan that fits shared memory."""
     lib = ops.load_library()
