@@ -148,7 +148,7 @@ int mkb_select_rows(const MkbsSelect *s, void *cuda_stream);
 
 /*
  * Cache row r of every key/value head <- its row rows[r], r = 0 .. min(n, keep) - 1, in place.  `rows` as mkb_select_rows gives
- * them: ascending.  An entry outside the sequence's rows leaves row r as it is.
+ * them: ascending.  An entry outside the sequence's rows or below r leaves row r as it is.
  */
 typedef struct MkbsMove {
     uint32_t struct_bytes;

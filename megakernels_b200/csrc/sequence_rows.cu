@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MkbsMove m, co
             const int r = i * step + k * per + mine;
             if (mine >= per || r >= kept) continue;
             const int source = from[i % kMoveFrom * step + k * per + mine];
-            if (source < 0 || source >= n || source == r) continue;  // (it stays)
+            if (source <= r || source >= n) continue;  // (it stays: rows before r may have been written)
             moving |= 1u << k;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mkb::smem_u32(fetched + (i % kMoveStages * kMoveRows + k) * kMoveThreads + threadIdx.x)),
                          "l"(base + source * row_bytes)

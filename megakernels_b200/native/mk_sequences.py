@@ -427,7 +427,8 @@ def select_rows(weights: Tensor, lengths: Tensor | int, *, keep: int, sinks: int
 
 def move_rows(keys: Tensor, values: Tensor | None, rows: Tensor, lengths: Tensor | int, *, stream=None) -> None:
     """Row r of every key/value head <- its row ``rows[..., r]``, in place, in caches ``[layers, sequences, positions,
-    kv_heads, dim]`` of one shape; ``rows`` as :func:`select_rows` returns them, ``lengths`` as it was given there."""
+    kv_heads, dim]`` of one shape; ``rows`` as :func:`select_rows` returns them, ``lengths`` as it was given there.  An entry below r or
+    outside the sequence's rows leaves row r as it is."""
     if not all(isinstance(t, Tensor) for t in (keys, rows)) or keys.ndim != 5 or rows.ndim != 4:
         raise ValueError("caches must be [layers, sequences, positions, kv_heads, dim], rows [layers, sequences, kv_heads, keep]")
     layers, sequences, positions, kv_heads, dim = keys.shape

@@ -871,6 +871,26 @@ def test_move_rows_leaves_alone_what_it_is_not_told():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", [5, 700, 2500])
+def test_rows_in_any_order_move_at_once(keep):
+    """Entries that are no selection: descending, the same one many times, from all over.  Those below their own row leave it as it is, the
+    others take what the row held before the call."""
+    positions, gen = 3000, torch.Generator().manual_seed(keep)
+    rows = torch.stack([torch.arange(positions - 1, positions - 1 - keep, -1), torch.full((keep,), keep // 2), torch.randint(-5, positions + 5, (keep,), generator=gen),
+                        torch.zeros(keep, dtype=torch.int64)]).view(1, 2, 2, keep)
+    k, v = draw(1, 1, 2, positions, 2, 64, dtype=BF16), draw(2, 1, 2, positions, 2, 64, dtype=BF16)
+    want = [k.clone(), v.clone()]
+    for b in range(2):
+        for h in range(2):
+            r = torch.arange(keep)
+            take = (rows[0, b, h] > r) & (rows[0, b, h] < positions)
+            for new, old in zip(want, (k, v)):
+                new[0, b, r[take], h] = old[0, b, rows[0, b, h][take], h]
+    ops.move_rows(k, v, rows.int().cuda(), positions)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+@pytest.mark.gpu
 def test_long_caches():
     """Rows further than 2^31 elements from a cache's beginning (2^32 bytes and more): one key of each head draws all weight, and moves."""
     kv_heads, dim, n = 32, 128, 530_000
