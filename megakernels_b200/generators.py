@@ -442,14 +442,14 @@ class MK_Generator(Generator):
         single = make_globals(self.model, skip_attn_reduction=True, max_attn_partitions=1)
         single.instructions = torch.zeros(1, 1, 32, dtype=torch.int32, device=device)  # (a prompt runs none)
         logits = globs.logits.new_empty(len(prompts), globs.vocab_size)
-        slots = torch.arange(globs.k_cache.shape[1], dtype=torch.int32, device=device)
+        slots = torch.arange(len(prompts) * beams, dtype=torch.int32, device=device)
         globs.pos_id_device = torch.zeros(globs.batch_size, dtype=torch.int32, device=device)
         for p in reversed(range(len(prompts))):  # (prompts go to slot 0: the first one's place)
             ids = prompts[p]
             self._prompt(ids.reshape(1, -1).to(device), globs=single)
             logits[p] = single.logits
             parents = torch.where(slots // beams == p, 0, slots)
-            ops.reorder_slots([globs.k_cache, globs.v_cache], parents.int(), dim=1, lengths=torch.full_like(slots, ids.numel()),
+            ops.reorder_slots(self._beam_caches(slots.numel()), parents.int(), dim=1, lengths=torch.full_like(slots, ids.numel()),
                               status=self._moves)
         return logits
 
@@ -470,14 +470,13 @@ class MK_Generator(Generator):
 
     def reorder_beams(self, parents: Tensor, first: int, lengths: Tensor) -> None:
         """Every beam goes on from its parent's rows; rows below ``first`` are alike."""
-        globs, n = self.schedule.globs, parents.numel()
-        slots = globs.k_cache.shape[1]
-        if n < slots:
-            everyone = torch.arange(slots, dtype=torch.int32, device=parents.device)
-            everyone[:n] = parents
-            parents, lengths = everyone, torch.cat([lengths, lengths.new_zeros(slots - n)])
         get_mk_module(name="mk_sequences").reorder_slots(
-            [globs.k_cache, globs.v_cache], parents, dim=1, first=first, lengths=lengths, status=self._moves)
+            self._beam_caches(parents.numel()), parents, dim=1, first=first, lengths=lengths, status=self._moves)
+
+    def _beam_caches(self, count: int) -> list[Tensor]:
+        """What the first ``count`` sequences hold (a cache may have more slots than a call takes)."""
+        globs = self.schedule.globs
+        return [globs.k_cache[:, :count], globs.v_cache[:, :count]]
 
     _positions_before = None
     _moves: Tensor | None = None  # status of the beams' reordering

@@ -190,6 +190,19 @@ def test_first_beam_of_one_is_greedy_decoding():
 
 
 @pytest.mark.gpu
+def test_beams_in_a_cache_of_many_slots():
+    """300 of them, where a call that moves rows takes 256; those that hold no beam keep all but their first row."""
+    model = llama("1b", 300, max_len=60)
+    gen = make_generator(model, LatencyScheduleOptions(num_attention_partitions=2, batch_size=8))
+    cache = model.stacked_kv_cache
+    for c in cache:
+        c[:, 6:].fill_(3.0)
+    check_search(gen, Plain(gen, lambda: cache, 1), [prompt(20, 1), prompt(11, 2)], 3, 10)
+    for c in cache:
+        assert (c[:, 6:8, 1:] == 3.0).all() and (c[:, 8:] == 3.0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("family,name", [("torirax", "odd"), ("torirax", "ragged"), ("dumalix", "odd"), ("dumalix", "ragged"), ("dumalix", "groups")])
 def test_layer_list_beams_go_on_as_if_alone(tmp_path, family, name, dtype):
