@@ -293,6 +293,8 @@ class MK_Generator(Generator):
         what the cache holds of the sequence (a later turn of a chat) or, to replace rows, before its end; 0 starts a sequence.
         """
         ids = prompt_ids.reshape(1, -1)
+        if position < 0:
+            raise ValueError(f"a prompt from position {position} on")
         at_once = self._takes_prompts(ids.shape[1], position)
         observed = self.schedule.globs.key_weights is not None
         if observed and not at_once:
@@ -610,6 +612,8 @@ class Hybrid_Generator(MK_Generator):
     def prefill(self, prompt_ids: Tensor, position: int = 0) -> Tensor:
         """Run a prompt from ``position`` on (0 starts a sequence); returns the first generated token ``[1]``."""
         n = prompt_ids.numel()
+        if position < 0:
+            raise ValueError(f"a prompt from position {position} on")
         return self.feed(prompt_ids, position, [n - 1]).argmax(dim=-1)
 
     def observe(self, window: int | None = None) -> None:

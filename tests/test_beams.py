@@ -10,7 +10,7 @@ import torch
 from megakernels_b200.beams import beam_search
 from megakernels_b200.demos.latency.scheduler import LatencyScheduleOptions
 from megakernels_b200.dispatch import make_generator, make_mk_interpreter, make_schedule_builder
-from megakernels_b200.generators import MK_Generator
+from megakernels_b200.generators import Hybrid_Generator, MK_Generator
 from megakernels_b200.llama import LlamaConfig, LlamaForCausalLM, build_rope_tables
 from megakernels_b200.model_types import ExtraModelConfig
 from megakernels_b200.scheduler import assign_to_sms, tensorize_instructions
@@ -49,6 +49,13 @@ def test_rope_tables_from_a_position():
         whole = build_rope_tables(cfg, 300, interleave)
         part = build_rope_tables(cfg, 100, interleave, first=200)
         assert all(torch.equal(w[200:], p) for w, p in zip(whole, part))
+
+
+@pytest.mark.parametrize("family", [MK_Generator, Hybrid_Generator])
+def test_a_prompt_before_the_first_position_is_refused(family):
+    """Before anything of the sequence is looked at or forgotten."""
+    with pytest.raises(ValueError, match="position -3"):
+        family.prefill(SimpleNamespace(), torch.zeros(5), position=-3)
 
 
 class NoGenerator:
