@@ -112,7 +112,7 @@ typedef struct MkbsKeyWeights {
     float scale;
     const int32_t *lengths;    /* [sequences] or NULL; below 0 counts as 0, above `positions` as that */
     const void *q;             /* bf16 [layers, sequences, queries, heads * dim], 16-byte aligned */
-    int64_t q_layer, q_sequence; /* strides in elements, multiples of 8 */
+    int64_t q_layer, q_sequence; /* strides in elements, multiples of 8 (of a dimension of one: any) */
     const void *k;             /* bf16 [layers, sequences, positions, kv_heads * dim], 16-byte aligned */
     int64_t k_layer, k_sequence;
     float *weights;            /* [layers, sequences, kv_heads, positions] */
@@ -158,7 +158,7 @@ typedef struct MkbsMove {
     const int32_t *lengths;    /* rows before the move */
     const int32_t *rows;
     void *caches[2];           /* [layers, sequences, positions, kv_heads, head], 16-byte aligned; the second may be NULL */
-    int64_t c_layer, c_sequence; /* strides in bytes, multiples of 16 */
+    int64_t c_layer, c_sequence; /* strides in bytes, multiples of 16 (of a dimension of one: any) */
 } MkbsMove;
 int mkb_move_rows(const MkbsMove *m, void *cuda_stream);
 

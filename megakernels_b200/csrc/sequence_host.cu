@@ -105,7 +105,8 @@ int check(const MkbsKeyWeights* w) {
     const int64_t q_row = (int64_t)w->heads * w->dim, k_row = (int64_t)w->kv_heads * w->dim;
     if (!aligned(w->q, 16) || !aligned(w->k, 16) || !aligned(w->weights, 4) || (w->status && !aligned(w->status, 4)))
         return invalid("key weights: q, k or weights missing or unaligned");
-    if (w->q_layer % 8 || w->q_sequence % 8 || w->k_layer % 8 || w->k_sequence % 8) return invalid("key weights: strides of q and k are multiples of 8");
+    if ((w->layers > 1 && (w->q_layer % 8 || w->k_layer % 8)) || (w->sequences > 1 && (w->q_sequence % 8 || w->k_sequence % 8)))
+        return invalid("key weights: strides of q and k are multiples of 8");
     if ((w->layers > 1 && (w->q_layer < w->queries * q_row || w->k_layer < w->positions * k_row)) ||
         (w->sequences > 1 && (w->q_sequence < w->queries * q_row || w->k_sequence < w->positions * k_row)))
         return invalid("key weights: sequences or layers of q or k overlap");
@@ -133,7 +134,8 @@ int check(const MkbsMove* m) {
     if (m->keep < 1) return invalid("move: keep must be positive");
     if (m->head_bytes < 16 || m->head_bytes % 16 || m->head_bytes > 1024)
         return fail(MKBS_ERR_UNSUPPORTED, "move: a head's part of a row is a multiple of 16 bytes, at most 1024");
-    if (!aligned(m->rows, 4) || !aligned(m->caches[0], 16) || (m->caches[1] && !aligned(m->caches[1], 16)) || m->c_layer % 16 || m->c_sequence % 16)
+    if (!aligned(m->rows, 4) || !aligned(m->caches[0], 16) || (m->caches[1] && !aligned(m->caches[1], 16)) || (m->layers > 1 && m->c_layer % 16) ||
+        (m->sequences > 1 && m->c_sequence % 16))
         return invalid("move: rows or caches missing or unaligned");
     if (m->caches[0] == m->caches[1]) return invalid("move: both caches are the same");
     if (!mkbs::apart((int64_t)m->positions * m->kv_heads * m->head_bytes, {{m->layers, m->c_layer}, {m->sequences, m->c_sequence}}))

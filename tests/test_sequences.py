@@ -189,6 +189,16 @@ def test_any_order_of_dimensions_is_taken_that_keeps_blocks_apart(name, make, kw
     assert getattr(ops.load_library(), f"mkb_{name}")(ctypes.byref(make(**kw)), None) == 2
 
 
+ONE = [("key_weights", weights_struct, dict(layers=1, q_layer=1, k_layer=7, w_layer=0)), ("key_weights", weights_struct, dict(sequences=1, q_sequence=3, k_sequence=1, w_sequence=0)),
+       ("move_rows", move_struct, dict(layers=1, c_layer=2)), ("move_rows", move_struct, dict(sequences=1, c_sequence=2))]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls are right: with a device they would run")
+@pytest.mark.parametrize("name,make,kw", ONE, ids=lambda v: str(v)[:60] if isinstance(v, (str, dict)) else "")
+def test_a_dimension_of_one_has_any_stride(name, make, kw):
+    assert getattr(ops.load_library(), f"mkb_{name}")(ctypes.byref(make(**kw)), None) == 2
+
+
 def test_the_same_region_twice_is_refused():
     """Two regions, then the same one twice."""
     lib, s = ops.load_library(), reorder_struct()
@@ -631,6 +641,21 @@ def check_weights(q, k, w, lengths, scale, as_number=False, stream=None):
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (8, 2, 128), (4, 4, 64), (16, 2, 128)])
 def test_key_weights(queries, positions, lengths, heads, kv_heads, dim):
     check_weights(*weights_case(queries, 2, len(lengths), queries, heads, kv_heads, dim, positions, lengths)[:3], lengths, dim**-0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 40])
+def test_key_weights_of_dimensions_of_one_with_odd_strides(queries):
+    """Tensors whose layers' and sequences' dimensions of one came from elsewhere: a stride of 1."""
+    q, k, w, scale = weights_case(5, 1, 1, queries, 8, 2, 64, 300, [300])
+    q, k, w = (t[0, 0].unsqueeze(-1).unsqueeze(-1).permute(-1, -2, *range(t.ndim - 2)) for t in (q, k, w))
+    assert q.stride()[:2] == (1, 1) and k.stride()[:2] == (1, 1)
+    check_weights(q, k, w, [300], scale)
+    old = k.clone()
+    rows = ops.select_rows(w, 300, keep=50)
+    ops.move_rows(k, None, rows, 300)
+    for h in range(2):
+        assert torch.equal(k[0, 0, :50, h], old[0, 0, rows[0, 0, h].long(), h])
 
 
 @pytest.mark.gpu
