@@ -319,7 +319,7 @@ class MK_Generator(Generator):
 
     def _forget(self, row: int) -> None:
         """Rows from ``row`` on are not those any more that were given weight."""
-        if row < self._weighed:
+        if 0 <= row < self._weighed:  # (another row's step is refused)
             self.schedule.globs.key_weights[..., row : self._weighed] = 0
             self._weighed = row
 

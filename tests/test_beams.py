@@ -465,6 +465,18 @@ def test_decoding_over_observed_rows_takes_their_weights(graph):
 
 
 @pytest.mark.gpu
+def test_a_refused_step_leaves_the_weights():
+    model, gen = observed_generator("1b", 64, None)
+    token = gen.prefill(prompt(64, 1))
+    weights = gen.schedule.globs.key_weights
+    before = weights.clone()
+    for position in (-1, 64):
+        with pytest.raises((RuntimeError, ValueError)):
+            gen.run(token.view(1, 1), position)
+    assert torch.equal(weights, before)
+
+
+@pytest.mark.gpu
 def test_rows_behind_what_is_evicted_lose_their_weights():
     model, gen = observed_generator("1b", 128, None)
     weights = gen.schedule.globs.key_weights
