@@ -617,7 +617,10 @@ class Hybrid_Generator(MK_Generator):
         return self.feed(prompt_ids, position, [n - 1]).argmax(dim=-1)
 
     def observe(self, window: int | None = None) -> None:
-        raise NotImplementedError("layer-list models' caches are not cut: their windows, chunks and latents bound them")
+        raise NotImplementedError("layer-list models' caches are not cut: their prompts do not weigh the keys they attend to")
+
+    def evict(self, length: int, keep: int, sinks: int = 4, recent: int = 64) -> int:
+        self.observe()  # (refuses)
 
     # -- beam search: beams are slots that take turns ---------------------------- #
     def beam_limits(self) -> tuple[int, int]:

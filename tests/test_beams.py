@@ -58,6 +58,13 @@ def test_a_prompt_before_the_first_position_is_refused(family):
         family.prefill(SimpleNamespace(), torch.zeros(5), position=-3)
 
 
+def test_layer_list_caches_are_not_cut():
+    gen = object.__new__(Hybrid_Generator)
+    for call in (lambda: gen.observe(16), lambda: gen.evict(100, 80)):
+        with pytest.raises(NotImplementedError, match="not cut"):
+            call()
+
+
 class NoGenerator:
     """A generator that has sequences, and may not be asked to run them."""
 
