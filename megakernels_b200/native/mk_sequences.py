@@ -239,7 +239,8 @@ def raise_status(status: Tensor | None = None) -> None:
         status = _records.get(torch.cuda.current_device())
         if status is None:
             return
-        torch.cuda.synchronize()
+    if status.is_cuda:
+        torch.cuda.synchronize(status.device)  # (all streams: the calls may have had others than the current one)
     code, block = status[:2].tolist()
     if code:
         status.zero_()
