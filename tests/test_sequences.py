@@ -749,13 +749,17 @@ def test_a_wait_that_gives_up_is_recorded_without_a_status(monkeypatch):
 @pytest.mark.gpu
 def test_a_status_is_read_when_other_streams_have_ended():
     """(A record that a stream writes a tenth of a second late.)"""
-    status, side = torch.zeros(16, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
-    torch.cuda.synchronize()
-    with torch.cuda.stream(side):
-        torch.cuda._sleep(200_000_000)
-        status[:2] = torch.ones(2, dtype=torch.int32, device="cuda") * 3
-    with pytest.raises(ops.SequenceError, match="block 3"):
+    status, gave_up, side = torch.zeros(16, dtype=torch.int32, device="cuda"), torch.full((16,), 3, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+    for cycles in (10, 200_000_000):  # (first the loading of what runs, which waits for the device)
+        status.zero_()
         ops.raise_status(status)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(cycles)
+            status.copy_(gave_up)
+        if cycles == 10:
+            torch.cuda.synchronize()
+        with pytest.raises(ops.SequenceError, match="block 3"):
+            ops.raise_status(status)
 
 
 @pytest.mark.gpu
