@@ -176,18 +176,26 @@ typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Map of a row-major bf16 or float matrix; what lies outside it reads as zero.
-template <typename T>
-inline cudaError_t tc_map(CUtensorMap* map, const T* ptr, int cols, int rows, int64_t ld, int box_cols, int box_rows) {
-    static EncodeFn encode = nullptr;
-    if (encode == nullptr) {
+// The driver's function that makes tensor maps.
+inline cudaError_t tc_encoder(EncodeFn* encode) {
+    static EncodeFn known = nullptr;
+    if (known == nullptr) {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q;
         cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
         if (e != cudaSuccess) return e;
         if (q != cudaDriverEntryPointSuccess || fn == nullptr) return cudaErrorNotSupported;
-        encode = reinterpret_cast<EncodeFn>(fn);
+        known = reinterpret_cast<EncodeFn>(fn);
     }
+    *encode = known;
+    return cudaSuccess;
+}
+
+// Map of a row-major bf16 or float matrix; what lies outside it reads as zero.
+template <typename T>
+inline cudaError_t tc_map(CUtensorMap* map, const T* ptr, int cols, int rows, int64_t ld, int box_cols, int box_rows) {
+    EncodeFn encode = nullptr;
+    if (const cudaError_t e = tc_encoder(&encode); e != cudaSuccess) return e;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * sizeof(T)};
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, elem[2] = {1, 1};

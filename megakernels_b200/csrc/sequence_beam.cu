@@ -94,12 +94,6 @@ __device__ __forceinline__ int shift_of(const T* row) { return (int)((reinterpre
 
 __device__ __forceinline__ bool is_live(float c) { return c > -INFINITY && c < INFINITY; }
 
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // 16 bytes of a row from element `at` on; what lies outside the row is minus infinity.  (Out of line: a launch fetches its code
 // anew, and few vectors lie at a row's ends.)
 template <typename T>

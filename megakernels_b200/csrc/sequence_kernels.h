@@ -27,6 +27,12 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu)); }
 
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Rows that sequence `b` holds.
 __device__ __forceinline__ int length_of(const int32_t* lengths, int length, int positions, int b) {
     return min(max(lengths != nullptr ? __ldg(lengths + b) : length, 0), positions);

@@ -70,11 +70,6 @@ struct Item {
     __device__ __forceinline__ float* weights(const WeightArgs& a) const { return a.weights + layer * a.w_layer + b * a.w_sequence + g * a.w_head; }
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // (not a number stays that)
 __device__ __forceinline__ float off_of(float top, float sum) { return sum == 0.f ? INFINITY : top + log2f(sum); }
 // (maximum, sum) of two parts
@@ -678,14 +673,8 @@ struct Plan {
 
 // 4 or 5 dimensions of bf16 with the 128-byte swizzle; what lies outside reads as zero
 cudaError_t encode(CUtensorMap* map, const bf16* ptr, int dims, const cuuint64_t* size, const cuuint64_t* stride_bytes, const cuuint32_t* box) {
-    static EncodeFn fn = nullptr;
-    if (fn == nullptr) {
-        void* found = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &found, cudaEnableDefault, &q); e != cudaSuccess) return e;
-        if (q != cudaDriverEntryPointSuccess || found == nullptr) return cudaErrorNotSupported;
-        fn = reinterpret_cast<EncodeFn>(found);
-    }
+    EncodeFn fn = nullptr;
+    if (const cudaError_t e = tc_encoder(&fn); e != cudaSuccess) return e;
     const cuuint32_t one[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, const_cast<bf16*>(ptr), size, stride_bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
