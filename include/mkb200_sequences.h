@@ -92,7 +92,7 @@ typedef struct MkbsReorder {
     const MkbsRegion *regions; /* host */
     const int32_t *parents;    /* [slots] */
     const int32_t *lengths;    /* [slots]: rows that a slot holds (above a region's rows: all); NULL: all */
-    int32_t *status;           /* 16 words that a wait for the call's own copies which gives up (2 s) writes to (code, block), or NULL */
+    int32_t *status;           /* 16 words that a wait for the call's own copies which gives up (2 s; not all rows have moved then) writes to (code, block), or NULL: not recorded */
 } MkbsReorder;
 int mkb_reorder_slots(const MkbsReorder *r, void *cuda_stream);
 
@@ -119,8 +119,8 @@ typedef struct MkbsKeyWeights {
     int64_t w_layer, w_sequence, w_head;
     void *workspace;           /* mkb_key_weights_bytes, 256-byte aligned */
     size_t workspace_bytes;
-    int32_t *status;           /* 16 words that a wait which gives up writes to (code, ...), or NULL */
-    uint32_t wait_timeout_ms;  /* 0: 2000 */
+    int32_t *status;           /* 16 words that a wait which gives up (not all has been added then) writes to (code, ...), or NULL: not recorded */
+    uint32_t wait_timeout_ms;  /* of a wait for a launch's own copies and products; 0: 2000 */
     uint32_t reserved;
 } MkbsKeyWeights;
 size_t mkb_key_weights_bytes(const MkbsKeyWeights *w); /* 0: not valid */

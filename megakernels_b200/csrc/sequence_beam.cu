@@ -49,7 +49,7 @@ struct BeamPlan {
         }
         segments = (int)((span + segment - 1) / segment);
         // as few segments per warp as let all blocks run at once, three on an SM (groups of 8 rows of 128256, 8, 12 and
-        // 24 of them, k = 8, before elements went 16 bytes at a time: with 1 block 21.1, 29.4, 37.3 us, 2 20.0, 22.6, 37.5, 3 20.0, 22.7, 31.0, 4 21.1, 24.4, 30.7)
+        // 24 of them, k = 8: with 1 block 17.1, 25.6, 30.8 us, 2 14.9, 17.6, 30.9, 3 15.3, 17.5, 25.1, 4 16.4, 19.6, 25.8)
         for (per_warp = 1; parts = (segments + per_warp * kScanWarps - 1) / (per_warp * kScanWarps), parts > 1 && (int64_t)rows * parts > 3 * kSms; ++per_warp) {
         }
         // candidates: all segments, then the elements of k of them, or of those that may be among the k

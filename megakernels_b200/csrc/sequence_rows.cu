@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 // of that very weight stay in the order of their places.  The weights are read from memory once: their orders lie in shared memory, as
 // far as they fit, for the passes that follow: digits (seldom), list, write.  A warp has a run of the rows in shared memory and one
 // of those behind; it counts those that stay, and with the counts of the runs before it writes them.
-// Instructions and what a pass begins and ends with bound it, not memory: 128 blocks of 65001 rows take 28 us (the weights at 1.2 TB/s;
-// with every digit found by a pass over all rows and no list 39), 448 of 4096 rows 13 (24, with 1024 threads each), 32 of 1500 5.7 (7.7).
+// Instructions and what a pass begins and ends with bound it, not memory: 128 blocks of 65001 rows take 30 us (the weights at 1.1 TB/s;
+// with every digit found by a pass over all rows and no list 39), 448 of 4096 rows 10 (24, with 1024 threads each), 32 of 1500 5.4 (7.7).
 constexpr int kDigits = 2048, kSelectAhead = 8, kAtOnce = 4, kFewRows = 1536, kRanked = 256;
 constexpr int kMostOrders = (227 * 1024 - kStaticShared) / 16 * 4;
 
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) select_kernel(const
 // read before the first is written.  Later rows come from behind what is written, so the next ones are on their way meanwhile:
 // copies into shared memory, of which each thread writes what it has fetched itself.  Where rows come from travels the same way,
 // some steps further ahead.
-// Memory bounds it, at 6.0 TB/s in pieces of 256 bytes (448 heads, 1024 rows of each cache: 79 us) and 5.0 in pieces of 128, a kilobyte apart
+// Memory bounds it, at 6.0 TB/s in pieces of 256 bytes (448 heads, 1024 rows of each cache: 80 us) and 5.0 in pieces of 128, a kilobyte apart
 // (128 heads, 8192 rows: 108 us).
 constexpr int kMoveThreads = 256, kMoveRows = 4, kMoveStages = 4, kMoveFrom = 8, kMoveBytes = kMoveStages * kMoveRows * kMoveThreads * 16;
 

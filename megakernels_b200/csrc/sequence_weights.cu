@@ -8,8 +8,8 @@
 //   keys   a unit is 128 keys (M) and a run of rows, 128 at a time: a thread has a key and a quarter of the rows, so that a key's weight is a
 //          sum in registers; where there are few keys their rows are several units, and a small launch adds the parts.
 // The exponentials bound both (16 a clock and SM: 0.54 us for 128 x 128 scores at 1.9 GHz, products 0.07 - 0.13).  Sums of a row refer to a
-// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 39.5 us for 1501 queries on 1501
-// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 57 us for 64 queries on 32768 keys (32 heads
+// maximum that is looked for in a row's first keys only, and again where a sum gets too large.  Measured: 39.1 us for 1501 queries on 1501
+// keys (32 heads of 64, exponentials of the causal half 16 us; a cluster per tile instead 59), 57.6 us for 64 queries on 32768 keys (32 heads
 // of 128, exponentials 30 us).  A step of 128 x 128 takes 1,400 cycles: the warps that sum 1,050 of exponentials and 250 of waits and loads, the warp
 // that issues products 580 (64 for each of eight: both operands come from shared memory) and 400 of waits, so that either is near the other's time.
 // Steps: warps of a scheduler need not meet at a unit's end (-5 us), one warp finds the units (-2), chosen lanes of whole warps issue (-0.5).
@@ -17,7 +17,7 @@
 // others are summed (59.5), waits that poll (64).
 // Up to 16 rows (a token's heads): the keys' traffic bounds it.  They are read once, straight into mma.sync fragments; the products go
 // through memory (4 bytes a row where a key has 128 or 256), not yet scaled: with scaled scores, rounded before a row's logarithm was taken
-// from them, large scores lost a weight's last digits (1.4e-3 of it at scores of 2^15; 20.4 us instead of 20.7 for 4 rows, 33.5 instead of 33.0 for 16).  One query on 65001 keys (32 heads of 64, 8 of keys): 21 us, 3.4 TB/s.  Blocks
+// from them, large scores lost a weight's last digits (1.4e-3 of it at scores of 2^15; 20.4 us instead of 20.7 for 4 rows, 33.5 instead of 33.0 for 15).  One query on 65001 keys (32 heads of 64, 8 of keys): 21.7 us, 3.3 TB/s.  Blocks
 // that all fit the SMs at once: 26.6 -> 22.9 us against four per SM, of which three fit; the sum's loads issued together and before the
 // statistics: 21.3; heads of the same keys in neighbouring blocks: 21.0.  Twice the loads of a warp, or two batches in turn: 24.
 #include <cfloat>

@@ -2,6 +2,7 @@
 
 import importlib
 import math
+from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
@@ -17,6 +18,7 @@ from megakernels_b200.scheduler import assign_to_sms, tensorize_instructions
 from megakernels_b200.scripts.generate import main, parse_cli
 from tests.oracle_utils import seeded_tokens
 
+ROOT = Path(__file__).resolve().parent.parent
 VOCAB = 4096
 CONFIGS = {
     "1b": lambda **kw: LlamaConfig.llama_3_2_1b(**{"num_hidden_layers": 2, "vocab_size": VOCAB, **kw}),
@@ -561,6 +563,26 @@ def test_observing_needs_whole_prompts():
     gen.enable_cuda_graph()
     with pytest.raises(ValueError, match="before"):
         gen.observe(4)
+
+
+@pytest.mark.gpu
+def test_the_documented_calls_run_as_written():
+    """The lines of INTEGRATION.md, on small models."""
+    text = (ROOT / "INTEGRATION.md").read_text().split("## Between steps")[1]
+    code = text.split("```python")[1].split("```")[0]
+    assert "beam_search" in code and "evict" in code
+
+    def make(model, options):
+        options.num_attention_partitions = 2
+        return make_generator(llama("1b", options.batch_size), options)
+
+    out = torch.zeros(1, 6, dtype=torch.long, device="cuda")
+    names = dict(make_generator=make, LatencyScheduleOptions=LatencyScheduleOptions, model=None, prompts=[prompt(9, 1), prompt(4, 2)], prompt=prompt(100, 3), output_tokens=out,
+                 ntok=5, next_turn=prompt(7, 4), rows_now=105)
+    exec(code.replace("ntok=200", "ntok=6"), names)
+    names["gen"].check()
+    names["several"].check()
+    assert names["found"].tokens.shape[:2] == (2, 4) and names["rows"] == 100 and out[0, 1:].any()
 
 
 @pytest.mark.gpu
