@@ -243,7 +243,8 @@ def raise_status(status: Tensor | None = None) -> None:
         torch.cuda.synchronize(status.device)  # (all streams: the calls may have had others than the current one)
     code, block = status[:2].tolist()
     if code:
-        status.zero_()
+        with torch.inference_mode():  # (a record that was made there can be written nowhere else)
+            status.zero_()
         raise SequenceError(code, f"a wait on the device gave up (block {block})")
 
 

@@ -222,6 +222,15 @@ def test_a_wait_that_gave_up_is_raised_and_cleared():
     ops.raise_status(status)
 
 
+def test_a_record_of_inference_mode_is_raised_and_cleared():
+    with torch.inference_mode():
+        status = torch.zeros(16, dtype=torch.int32)
+        status[:2] = torch.tensor([3, 9], dtype=torch.int32)
+    with pytest.raises(ops.SequenceError, match="block 9"):
+        ops.raise_status(status)
+    assert not status.any()
+
+
 @pytest.mark.parametrize("length", [-1, 101, 2**32 + 5, -(2**32) + 5])
 def test_a_length_outside_the_cache_is_refused(length):
     s = ops._struct(ops.MkbsSelect)
