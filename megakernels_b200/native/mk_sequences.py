@@ -372,9 +372,10 @@ def key_weights(q: Tensor, keys: Tensor, weights: Tensor, lengths: Tensor | int,
         raise ValueError("q must be [layers, sequences, queries, heads, dim], keys [layers, sequences, positions, kv_heads, dim]")
     layers, sequences, queries, heads, dim = q.shape
     positions, kv_heads = keys.shape[2:4]
-    if (wait_timeout_ms | layers | sequences | queries | heads | positions | kv_heads) >> 31:
-        _fit(wait_timeout_ms, *q.shape, *keys.shape)
-        raise ValueError(f"a limit of {wait_timeout_ms} ms")
+    if (layers | sequences | queries | heads | positions | kv_heads) >> 31:
+        _fit(*q.shape, *keys.shape)
+    if wait_timeout_ms >> 32:
+        raise ValueError(f"a limit of {wait_timeout_ms} ms does not fit 32 bits")
     _refuse_host("q", q)
     lib, where, bf16 = load_library(), _Where(stream, q), torch.bfloat16
     s, device = _struct(MkbsKeyWeights), where.device

@@ -264,6 +264,13 @@ def test_a_negative_limit_is_refused():
         ops.key_weights(z(1, 1, 1, 8, 64), z(1, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0, wait_timeout_ms=-1)
 
 
+def test_the_longest_limit_is_taken():
+    """(What is refused then is where the tensors are.)"""
+    z = lambda *shape: torch.zeros(()).expand(shape)  # noqa: E731
+    with pytest.raises(ValueError, match="CUDA device"):
+        ops.key_weights(z(1, 1, 1, 8, 64), z(1, 1, 9, 2, 64), z(1, 1, 2, 9), 5, scale=1.0, wait_timeout_ms=2**32 - 1)
+
+
 @pytest.mark.gpu
 def test_rows_of_a_region_that_do_not_fit_are_refused():
     """(8 GB of bytes, that nothing touches.)"""
